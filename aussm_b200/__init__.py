@@ -13,6 +13,8 @@ from .s6 import selective_scan_fn
 from .variants import project, scan_complex, ssm_adaptive_complex, ssm_adaptive_preal
 from .host import HostBatchStep, bind_process_to_gpu_cpus
 from .linear import SplitLinear, split_linear
+from .delta import gated_delta_rule, gated_delta_step
+from .rotary import qk_norm_rotate, rotary_frequencies
 
 __all__ = ["ops", "HostBatchStep", "SplitLinear", "split_linear", "selective_scan_fn", "scan_complex", "project", "ssm_adaptive_complex", "ssm_adaptive_preal", "ssm_adaptive_interface", "ssm_adaptive_unitary", "scan_unitary", "install_as_extension_cpp",
-           "device_status"]
+           "device_status", "gated_delta_rule", "gated_delta_step", "qk_norm_rotate", "rotary_frequencies"]

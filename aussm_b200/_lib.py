@@ -16,6 +16,23 @@ _I = ctypes.c_int
 _Z = ctypes.c_size_t
 _LL = ctypes.c_longlong
 
+
+class DeltaProblem(ctypes.Structure):
+    """aussm_b200_delta_t"""
+    _fields_ = ([(n, _I) for n in ("B", "L", "HK", "HV", "DK", "DV", "dtype")] + [("scale", ctypes.c_float)]
+                + [(n, _LL * 3) for n in ("q_stride", "k_stride", "v_stride", "go_stride")])
+
+
+class RotateProblem(ctypes.Structure):
+    """aussm_b200_rotate_t"""
+    _fields_ = ([(n, _I) for n in ("B", "L", "HQ", "HK", "d", "rot", "dtype", "norm", "interleaved")]
+                + [("eps", ctypes.c_float), ("magnitude", ctypes.c_float), ("position_stride", _LL)]
+                + [(n, _LL * 3) for n in ("q_stride", "k_stride", "gq_stride", "gk_stride")])
+
+
+_DP = ctypes.POINTER(DeltaProblem)
+_RP = ctypes.POINTER(RotateProblem)
+
 # name -> (restype, argtypes); mirrors include/aussm_b200.h one to one
 SIGNATURES = {
     "aussm_b200_version": (_I, []),
@@ -59,6 +76,14 @@ SIGNATURES = {
     "aussm_b200_unitary_bwd": (_I, [_P] * 29 + [_I] * 4 + [_P, _Z, _P]),
     "aussm_b200_unitary_keep_bytes": (_Z, [_I] * 4),
     "aussm_b200_unitary_fwd_keep": (_I, [_P] * 15 + [_I] * 4 + [_P, _Z, _P, _Z, _P]),
+    "aussm_b200_delta_keep_bytes": (_Z, [_DP]),
+    "aussm_b200_delta_workspace_bytes": (_Z, [_DP, _I]),
+    "aussm_b200_delta_fwd": (_I, [_DP] + [_P] * 9 + [_Z, _P, _Z, _P]),
+    "aussm_b200_delta_bwd": (_I, [_DP] + [_P] * 8 + [_Z] + [_P] * 7 + [_Z, _P]),
+    "aussm_b200_delta_step": (_I, [_DP] + [_P] * 9),
+    "aussm_b200_rotate_fwd": (_I, [_RP] + [_P] * 9),
+    "aussm_b200_rotate_bwd_workspace_bytes": (_Z, [_RP]),
+    "aussm_b200_rotate_bwd": (_I, [_RP] + [_P] * 13 + [_Z, _P]),
     "aussm_b200_unitary_bwd_kept": (_I, [_P] * 29 + [_I] * 4 + [_P, _Z, _P, _Z, _P]),
 }
 

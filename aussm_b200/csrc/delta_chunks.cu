@@ -1,0 +1,339 @@
+// Gated delta rule over chunks, the plain way: products of small matrices element by element, operands in global
+// memory, float32 throughout.
+#include "delta.cuh"
+#include "host_common.cuh"
+
+namespace aussm {
+namespace {
+
+constexpr int C = kDeltaChunk;
+constexpr int NT = 256;
+constexpr int SLICE = 32;            // value columns of a block of the recurrences
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+int chunks_of(const aussm_b200_delta_t& p) { return (p.L + C - 1) / C; }
+size_t heads_of(const aussm_b200_delta_t& p) { return (size_t)p.B * p.HV * chunks_of(p); }
+
+// per chunk and value head
+struct Record {
+    double *G;       // (C) sums of g: differences of large sums have to be right to 24 bits
+    float *T, *P;    // (C, C)
+    float *W;        // (C, DK)
+    float *N;        // (C, DV): V'
+    float *S;        // (DK, DV): entry state
+};
+Record record_at(const aussm_b200_delta_t& p, void* keep) {
+    const size_t n = heads_of(p);
+    Record r;
+    r.G = static_cast<double*>(keep);
+    float* f = reinterpret_cast<float*>(r.G + n * C);
+    r.T = f; f += n * C * C;
+    r.P = f; f += n * C * C;
+    r.W = f; f += n * C * p.DK;
+    r.N = f; f += n * C * p.DV;
+    r.S = f;
+    return r;
+}
+
+struct Params {
+    aussm_b200_delta_t p;
+    DeltaInputs in;
+    const void* go;
+    const float *s0, *gs1;
+    void* o;
+    float *s1, *ds0;
+    Record r;
+    float *X, *dN, *dS;        // backward: (C, DV) twice, (DK, DV) per chunk and head
+    void *dq, *dk, *dv;
+    float *dg, *dbeta;
+    int n;                     // chunks
+};
+
+template <typename T>
+struct Rows {                  // rows of one head from step t0 on; zero behind the end
+    const T* p;
+    long long step;
+    int rows;
+    __device__ float operator()(int i, int j) const { return i < rows ? to_f32(p[i * step + j]) : 0.f; }
+};
+template <typename T>
+__device__ Rows<T> rows_of(const void* base, const long long (&s)[3], int b, int t0, int h, int L) {
+    return {static_cast<const T*>(base) + b * s[0] + t0 * s[1] + h * s[2], s[1], min(C, L - t0)};
+}
+
+template <typename F, typename G>
+__device__ void products(int M, int N, int K, F term, G store) {
+    for (int e = threadIdx.x; e < M * N; e += NT) {
+        const int i = e / N, j = e % N;
+        float a = 0.f;
+        for (int k = 0; k < K; ++k) a += term(i, j, k);
+        store(i, j, a);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT) prepare_kernel(const Params a) {
+    __shared__ float A[C][C + 1], be[C];
+    __shared__ double G[C];
+    const aussm_b200_delta_t& p = a.p;
+    const int c = blockIdx.x % a.n, bh = blockIdx.x / a.n, b = bh / p.HV, h = bh % p.HV, hk = h / (p.HV / p.HK);
+    const int t0 = c * C, rows = min(C, p.L - t0);
+    const Rows<T> q = rows_of<T>(a.in.q, p.q_stride, b, t0, hk, p.L), k = rows_of<T>(a.in.k, p.k_stride, b, t0, hk, p.L);
+    const size_t at = blockIdx.x;
+    float *Tm = a.r.T + at * C * C, *P = a.r.P + at * C * C, *W = a.r.W + at * C * p.DK;
+    if (threadIdx.x == 0) {
+        double s = 0;
+        for (int i = 0; i < C; ++i) {
+            const long long o = ((long long)b * p.L + t0 + i) * p.HV + h;
+            s += i < rows ? clamp_log_decay(a.in.g[o]) : 0.f;
+            G[i] = s;
+            be[i] = i < rows ? a.in.beta[o] : 0.f;
+            a.r.G[at * C + i] = G[i];
+        }
+    }
+    __syncthreads();
+    products(C, C, p.DK, [&](int i, int j, int x) { return j < i ? k(i, x) * k(j, x) : 0.f; },
+             [&](int i, int j, float v) { A[i][j] = j < i ? be[i] * expf((float)(G[i] - G[j])) * v : 0.f; });
+    products(C, C, p.DK, [&](int i, int j, int x) { return j <= i ? q(i, x) * k(j, x) : 0.f; },
+             [&](int i, int j, float v) { P[i * C + j] = j <= i ? p.scale * expf((float)(G[i] - G[j])) * v : 0.f; });
+    __syncthreads();
+    if (threadIdx.x < C) {           // column j of T by forward substitution
+        const int j = threadIdx.x;
+        for (int i = 0; i < C; ++i) {
+            float s = i == j ? 1.f : 0.f;
+            for (int m = j; m < i; ++m) s -= A[i][m] * Tm[m * C + j];
+            Tm[i * C + j] = i < j ? 0.f : s;
+        }
+    }
+    __syncthreads();
+    products(C, p.DK, C, [&](int i, int x, int j) { return j <= i ? Tm[i * C + j] * be[j] * expf((float)(G[j])) * k(j, x) : 0.f; },
+             [&](int i, int x, float v) { W[i * p.DK + x] = v; });
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT) forward_kernel(const Params a) {
+    extern __shared__ float S[];     // (DK, SLICE)
+    const aussm_b200_delta_t& p = a.p;
+    const int bh = blockIdx.x, b = bh / p.HV, h = bh % p.HV, hk = h / (p.HV / p.HK);
+    const int v0 = blockIdx.y * SLICE, nv = min(SLICE, p.DV - v0);
+    for (int e = threadIdx.x; e < p.DK * nv; e += NT)
+        S[e / nv * SLICE + e % nv] = a.s0 ? a.s0[((size_t)bh * p.DK + e / nv) * p.DV + v0 + e % nv] : 0.f;
+    __syncthreads();
+    for (int c = 0; c < a.n; ++c) {
+        const int t0 = c * C, rows = min(C, p.L - t0);
+        const size_t at = (size_t)bh * a.n + c;
+        const double* G = a.r.G + at * C;
+        const float *Tm = a.r.T + at * C * C, *P = a.r.P + at * C * C, *W = a.r.W + at * C * p.DK;
+        float* N = a.r.N + at * C * p.DV + v0;
+        const Rows<T> q = rows_of<T>(a.in.q, p.q_stride, b, t0, hk, p.L), k = rows_of<T>(a.in.k, p.k_stride, b, t0, hk, p.L),
+                      v = rows_of<T>(a.in.v, p.v_stride, b, t0, h, p.L);
+        const float* be = a.in.beta + ((long long)b * p.L + t0) * p.HV + h;
+        for (int e = threadIdx.x; e < p.DK * nv; e += NT)
+            a.r.S[(at * p.DK + e / nv) * p.DV + v0 + e % nv] = S[e / nv * SLICE + e % nv];
+        products(C, nv, C + p.DK, [&](int i, int j, int m) {
+            if (m >= C) return -W[i * p.DK + m - C] * S[(m - C) * SLICE + j];
+            return m <= i && m < rows ? Tm[i * C + m] * be[(long long)m * p.HV] * v(m, v0 + j) : 0.f;
+        }, [&](int i, int j, float x) { N[(size_t)i * p.DV + j] = x; });
+        __syncthreads();
+        products(rows, nv, C + p.DK, [&](int i, int j, int m) {
+            if (m >= C) return p.scale * expf((float)(G[i])) * q(i, m - C) * S[(m - C) * SLICE + j];
+            return m <= i ? P[i * C + m] * N[(size_t)m * p.DV + j] : 0.f;
+        }, [&](int i, int j, float x) {
+            static_cast<T*>(a.o)[(((long long)b * p.L + t0 + i) * p.HV + h) * p.DV + v0 + j] = from_f32<T>(x);
+        });
+        __syncthreads();
+        products(p.DK, nv, C, [&](int x, int j, int i) { return expf((float)(G[C - 1] - G[i])) * k(i, x) * N[(size_t)i * p.DV + j]; },
+                 [&](int x, int j, float s) { S[x * SLICE + j] = expf((float)(G[C - 1])) * S[x * SLICE + j] + s; });
+        __syncthreads();
+    }
+    if (a.s1)
+        for (int e = threadIdx.x; e < p.DK * nv; e += NT)
+            a.s1[((size_t)bh * p.DK + e / nv) * p.DV + v0 + e % nv] = S[e / nv * SLICE + e % nv];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT) backward_kernel(const Params a) {
+    extern __shared__ float dS[];    // (DK, SLICE)
+    const aussm_b200_delta_t& p = a.p;
+    const int bh = blockIdx.x, b = bh / p.HV, h = bh % p.HV, hk = h / (p.HV / p.HK);
+    const int v0 = blockIdx.y * SLICE, nv = min(SLICE, p.DV - v0);
+    for (int e = threadIdx.x; e < p.DK * nv; e += NT)
+        dS[e / nv * SLICE + e % nv] = a.gs1 ? a.gs1[((size_t)bh * p.DK + e / nv) * p.DV + v0 + e % nv] : 0.f;
+    __syncthreads();
+    for (int c = a.n - 1; c >= 0; --c) {
+        const int t0 = c * C, rows = min(C, p.L - t0);
+        const size_t at = (size_t)bh * a.n + c;
+        const double* G = a.r.G + at * C;
+        const float *Tm = a.r.T + at * C * C, *P = a.r.P + at * C * C, *W = a.r.W + at * C * p.DK;
+        float *dN = a.dN + at * C * p.DV + v0, *X = a.X + at * C * p.DV + v0;
+        const Rows<T> q = rows_of<T>(a.in.q, p.q_stride, b, t0, hk, p.L), k = rows_of<T>(a.in.k, p.k_stride, b, t0, hk, p.L),
+                      go = rows_of<T>(a.go, p.go_stride, b, t0, h, p.L);
+        const float* be = a.in.beta + ((long long)b * p.L + t0) * p.HV + h;
+        for (int e = threadIdx.x; e < p.DK * nv; e += NT)
+            a.dS[(at * p.DK + e / nv) * p.DV + v0 + e % nv] = dS[e / nv * SLICE + e % nv];
+        products(C, nv, C + p.DK, [&](int i, int j, int m) {
+            if (m >= C) return expf((float)(G[C - 1] - G[i])) * k(i, m - C) * dS[(m - C) * SLICE + j];
+            return m >= i ? P[m * C + i] * go(m, v0 + j) : 0.f;
+        }, [&](int i, int j, float x) { dN[(size_t)i * p.DV + j] = x; });
+        __syncthreads();
+        products(C, nv, C, [&](int i, int j, int m) { return m >= i ? Tm[m * C + i] * dN[(size_t)m * p.DV + j] : 0.f; },
+                 [&](int i, int j, float x) {
+                     X[(size_t)i * p.DV + j] = x;
+                     if (i < rows)
+                         static_cast<T*>(a.dv)[(((long long)b * p.L + t0 + i) * p.HV + h) * p.DV + v0 + j] =
+                             from_f32<T>(be[(long long)i * p.HV] * x);
+                 });
+        products(p.DK, nv, C, [&](int x, int j, int i) {
+            return p.scale * expf((float)(G[i])) * q(i, x) * go(i, v0 + j) - W[i * p.DK + x] * dN[(size_t)i * p.DV + j];
+        }, [&](int x, int j, float s) { dS[x * SLICE + j] = expf((float)(G[C - 1])) * dS[x * SLICE + j] + s; });
+        __syncthreads();
+    }
+    if (a.ds0)
+        for (int e = threadIdx.x; e < p.DK * nv; e += NT)
+            a.ds0[((size_t)bh * p.DK + e / nv) * p.DV + v0 + e % nv] = dS[e / nv * SLICE + e % nv];
+}
+
+// Gradients of q, k, g and beta of a chunk; a block loops over the value heads of a key head.
+template <typename T>
+__global__ void __launch_bounds__(NT) gradients_kernel(const Params a) {
+    extern __shared__ float sm[];
+    const aussm_b200_delta_t& p = a.p;
+    const int r = p.HV / p.HK, c = blockIdx.x % a.n, b = blockIdx.x / a.n / p.HK, hk = blockIdx.x / a.n % p.HK;
+    const int t0 = c * C, rows = min(C, p.L - t0), DK = p.DK, DV = p.DV;
+    float *Ep = sm, *E = Ep + C * C, *F = E + C * C, *dQ = F + C * C, *dK = dQ + C * DK, *dG = dK + C * DK, *dB = dG + C, *dGs = dB + C;
+    const Rows<T> q = rows_of<T>(a.in.q, p.q_stride, b, t0, hk, p.L), k = rows_of<T>(a.in.k, p.k_stride, b, t0, hk, p.L);
+    for (int e = threadIdx.x; e < 2 * C * DK; e += NT) dQ[e] = 0.f;
+    for (int h = hk * r; h < hk * r + r; ++h) {
+        const size_t at = ((size_t)b * p.HV + h) * a.n + c;
+        const double* G = a.r.G + at * C;
+        const float *N = a.r.N + at * C * DV, *X = a.X + at * C * DV, *S = a.r.S + at * DK * DV,
+                    *dS = a.dS + at * DK * DV;
+        const Rows<T> go = rows_of<T>(a.go, p.go_stride, b, t0, h, p.L), v = rows_of<T>(a.in.v, p.v_stride, b, t0, h, p.L);
+        const float* beta = a.in.beta + ((long long)b * p.L + t0) * p.HV + h;
+        auto be = [&](int i) { return i < rows ? beta[(long long)i * p.HV] : 0.f; };
+        __syncthreads();
+        for (int e = threadIdx.x; e < 3 * C; e += NT) dG[e] = 0.f;
+        __syncthreads();
+        products(C, C, DV, [&](int i, int j, int x) { return j <= i ? go(i, x) * N[(size_t)j * DV + x] : 0.f; },
+                 [&](int i, int j, float x) { Ep[i * C + j] = j <= i ? p.scale * expf((float)(G[i] - G[j])) * x : 0.f; });
+        products(C, C, DV, [&](int i, int j, int x) { return j < i ? X[(size_t)i * DV + x] * N[(size_t)j * DV + x] : 0.f; },
+                 [&](int i, int j, float x) { E[i * C + j] = j < i ? -expf((float)(G[i] - G[j])) * x : 0.f; });      // beta follows
+        __syncthreads();
+        if (threadIdx.x < C) {
+            const int i = threadIdx.x;
+            float bi = 0.f;
+            for (int j = 0; j < i; ++j) {
+                float qk = 0.f, kk = 0.f;
+                for (int x = 0; x < DK; ++x) {
+                    qk += q(i, x) * k(j, x);
+                    kk += k(i, x) * k(j, x);
+                }
+                F[i * C + j] = Ep[i * C + j] * qk + be(i) * E[i * C + j] * kk;      // gradient of G_i - G_j
+                bi += E[i * C + j] * kk;
+            }
+            for (int x = 0; x < DV; ++x) bi += X[(size_t)i * DV + x] * v(i, x);
+            dB[i] = bi;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < C; i += NT) {            // row i: the terms with states
+            const float since = expf((float)(G[i])), until = expf((float)(G[C - 1] - G[i]));
+            float kz = 0.f, kkt = 0.f, qqt = 0.f;
+            for (int x = 0; x < DK; ++x) {
+                float dqt = 0.f, z = 0.f, dkt = 0.f;
+                for (int y = 0; y < DV; ++y) {
+                    dqt += go(i, y) * S[(size_t)x * DV + y];
+                    z += X[(size_t)i * DV + y] * S[(size_t)x * DV + y];
+                    dkt += N[(size_t)i * DV + y] * dS[(size_t)x * DV + y];
+                }
+                kz += since * z * k(i, x);
+                kkt += until * dkt * k(i, x);
+                qqt += p.scale * since * dqt * q(i, x);
+                float dq = p.scale * since * dqt, dk = until * dkt - be(i) * since * z;
+                for (int j = 0; j < C; ++j) {
+                    dq += Ep[i * C + j] * k(j, x);
+                    dk += Ep[j * C + i] * q(j, x) + (be(i) * E[i * C + j] + be(j) * E[j * C + i]) * k(j, x);
+                }
+                dQ[i * DK + x] += dq;
+                dK[i * DK + x] += dk;
+            }
+            dG[i] = qqt - be(i) * kz;
+            dB[i] -= kz;
+            dGs[i] = kkt;
+        }
+        __syncthreads();
+        // g_t stands in G_i for i >= t, in G_i - G_j for j < t <= i, in G_C - G_i for i < t and in G_C: summed over just
+        // these pairs, since sums over all of which most cancel would lose a strongly decayed head's small gradients
+        if (threadIdx.x < rows) {
+            const int t = threadIdx.x;
+            float ss = 0.f, sum = 0.f;
+            for (int e = 0; e < DK * DV; ++e) ss += dS[e] * S[e];
+            sum = expf((float)(G[C - 1])) * ss;
+            for (int i = 0; i < t; ++i) sum += dGs[i];
+            for (int i = t; i < C; ++i) {
+                sum += dG[i];
+                for (int j = 0; j < t; ++j) sum += F[i * C + j];
+            }
+            const long long o = ((long long)b * p.L + t0 + t) * p.HV + h;
+            a.dg[o] = sum;
+            a.dbeta[o] = dB[t];
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * DK; e += NT) {
+        const long long o = (((long long)b * p.L + t0 + e / DK) * p.HK + hk) * DK + e % DK;
+        static_cast<T*>(a.dq)[o] = from_f32<T>(dQ[e]);
+        static_cast<T*>(a.dk)[o] = from_f32<T>(dK[e]);
+    }
+}
+
+template <typename T>
+cudaError_t forward(const Params& a, cudaStream_t st) {
+    prepare_kernel<T><<<(unsigned)heads_of(a.p), NT, 0, st>>>(a);
+    forward_kernel<T><<<dim3(a.p.B * a.p.HV, (a.p.DV + SLICE - 1) / SLICE), NT, a.p.DK * SLICE * 4, st>>>(a);
+    count_launch(2);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t backward(const Params& a, cudaStream_t st) {
+    backward_kernel<T><<<dim3(a.p.B * a.p.HV, (a.p.DV + SLICE - 1) / SLICE), NT, a.p.DK * SLICE * 4, st>>>(a);
+    const int smem = (3 * C * C + 2 * C * a.p.DK + 3 * C) * 4;
+    cudaError_t e = cudaFuncSetAttribute(gradients_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    gradients_kernel<T><<<(unsigned)(a.p.B * a.p.HK * a.n), NT, smem, st>>>(a);
+    count_launch(2);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t delta_keep_bytes(const aussm_b200_delta_t& p) {
+    return up256(heads_of(p) * (size_t)(2 * C + 2 * C * C + C * p.DK + C * p.DV + p.DK * p.DV) * 4);
+}
+size_t delta_bwd_bytes(const aussm_b200_delta_t& p) {
+    return up256(heads_of(p) * (size_t)(2 * C * p.DV + p.DK * p.DV) * 4);
+}
+
+cudaError_t launch_delta_fwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const float* s0, void* o, float* s1,
+                             void* keep, cudaStream_t st) {
+    Params a = {};
+    a.p = p; a.in = in; a.s0 = s0; a.o = o; a.s1 = s1; a.r = record_at(p, keep); a.n = chunks_of(p);
+    return p.dtype == AUSSM_FLOAT32 ? forward<float>(a, st) : p.dtype == AUSSM_BFLOAT16 ? forward<__nv_bfloat16>(a, st)
+                                                                                       : forward<__half>(a, st);
+}
+
+cudaError_t launch_delta_bwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const void* go, const float* gs1,
+                             const void* keep, void* dq, void* dk, void* dv, float* dg, float* dbeta, float* ds0,
+                             void* ws, cudaStream_t st) {
+    Params a = {};
+    a.p = p; a.in = in; a.go = go; a.gs1 = gs1; a.r = record_at(p, const_cast<void*>(keep)); a.n = chunks_of(p);
+    a.dq = dq; a.dk = dk; a.dv = dv; a.dg = dg; a.dbeta = dbeta; a.ds0 = ds0;
+    const size_t n = heads_of(p);
+    a.X = static_cast<float*>(ws);
+    a.dN = a.X + n * C * p.DV;
+    a.dS = a.dN + n * C * p.DV;
+    return p.dtype == AUSSM_FLOAT32 ? backward<float>(a, st) : p.dtype == AUSSM_BFLOAT16 ? backward<__nv_bfloat16>(a, st)
+                                                                                        : backward<__half>(a, st);
+}
+
+}  // namespace aussm

@@ -1,0 +1,191 @@
+"""The gated delta rule on B200: a sequence mixer with a matrix state.
+
+Per batch entry and value head, with ``a_t = exp(g_t)`` and the state ``S`` (dk, dv)::
+
+    e_t = beta_t (v_t - a_t S_{t-1}^T k_t)        what the state does not yet answer to the key, times the step size
+    S_t = a_t S_{t-1} + k_t e_t^T
+    o_t = scale S_t^T q_t
+
+``gated_delta_rule`` takes whole sequences (a chunk of 64 steps at a time, forward and backward),
+``gated_delta_step`` one or a few new steps of many sequences.  Both agree with the recurrence to float32 accuracy for
+every input type.  CUDA tensors only; all arithmetic runs in libaussm_b200.so.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .ops import _PLAIN, _eager, _ptr, _stream, _workspace
+
+__all__ = ["gated_delta_rule", "gated_delta_step", "MAX_KEY", "MAX_VALUE"]
+
+MAX_KEY, MAX_VALUE = 128, 256            # widths of a head that the kernels take
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _refuse_traced(what: str, *tensors) -> None:
+    """A kernel that writes through raw pointers is invisible to tracers and function transforms: refuse them."""
+    plain = all(t is None or type(t) in _PLAIN for t in tensors)
+    if plain and _eager():
+        return
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    if (not plain or torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0
+            or torch.compiler.is_compiling() or torch._C._is_tracing() or get_proxy_mode() is not None):
+        raise RuntimeError(f"{what} runs eagerly on plain tensors: no function transforms, forward-mode differentiation, "
+                           "tracing or tensor subclasses")
+
+
+def _typed(name: str, t: Tensor, dtype, shape, device) -> Tensor:
+    """``t`` checked, with unit stride along its last axis (a copy only where it has not)."""
+    if not isinstance(t, Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (there is no CPU implementation of this operator)")
+    if t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides(t: Tensor):
+    return (ctypes.c_longlong * 3)(*t.stride()[:3])
+
+
+def _check(q, k, v, g, beta, scale):
+    """The problem, and the inputs as the kernels take them."""
+    if not isinstance(q, Tensor) or not q.is_cuda:
+        raise RuntimeError("q must be a CUDA tensor (there is no CPU implementation of this operator)")
+    if q.dtype not in _DTYPES:
+        raise RuntimeError(f"q must be float32, bfloat16 or float16, got {q.dtype}")
+    if q.dim() != 4 or not isinstance(v, Tensor) or v.dim() != 4:
+        raise RuntimeError("q, k and v must be (batch, length, heads, width)")
+    b, l, hk, dk = q.shape
+    hv, dv = v.shape[2:]
+    if hk == 0 or hv == 0 or hv % hk:
+        raise RuntimeError(f"the {hv} value heads must be a multiple of the {hk} key heads")
+    if not (1 <= dk <= MAX_KEY and 1 <= dv <= MAX_VALUE):
+        raise RuntimeError(f"heads of {dk} keys and {dv} values: 1 to {MAX_KEY} and 1 to {MAX_VALUE} are supported")
+    q = _typed("q", q, q.dtype, (b, l, hk, dk), q.device)
+    k = _typed("k", k, q.dtype, (b, l, hk, dk), q.device)
+    v = _typed("v", v, q.dtype, (b, l, hv, dv), q.device)
+    g = _typed("g", g, torch.float32, (b, l, hv), q.device).contiguous()
+    beta = _typed("beta", beta, torch.float32, (b, l, hv), q.device).contiguous()
+    p = _lib.DeltaProblem(b, l, hk, hv, dk, dv, _DTYPES[q.dtype], dk ** -0.5 if scale is None else float(scale),
+                          _strides(q), _strides(k), _strides(v))
+    return p, q, k, v, g, beta
+
+
+def _state(name: str, s: Tensor, p, device) -> Tensor:
+    return _typed(name, s, torch.float32, (p.B, p.HV, p.DK, p.DV), device).contiguous()
+
+
+class _GatedDelta(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, scale, want_state, keep_for_backward):
+        p, q, k, v, g, beta = _check(q, k, v, g, beta, scale)
+        state = None if state is None else _state("initial_state", state, p, q.device)
+        o = torch.empty(p.B, p.L, p.HV, p.DV, device=q.device, dtype=q.dtype)
+        last = torch.empty(p.B, p.HV, p.DK, p.DV, device=q.device, dtype=torch.float32) if want_state else None
+        ctx.set_materialize_grads(False)
+        ctx.p, ctx.has_state = p, state is not None
+        if o.numel() == 0:
+            if last is not None:
+                last.zero_() if state is None else last.copy_(state)
+            ctx.save_for_backward(q, k, v, g, beta, None)
+            return o, last
+        lib = _lib.load()
+        with torch.cuda.device(q.device):
+            keep = ws = None
+            if keep_for_backward:
+                keep = _workspace(lib.aussm_b200_delta_keep_bytes(p), q.device)
+            else:
+                ws = _workspace(lib.aussm_b200_delta_workspace_bytes(p, 0), q.device)
+            rc = lib.aussm_b200_delta_fwd(p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(o), _ptr(last),
+                                          _ptr(keep), 0 if keep is None else keep.numel(), _ptr(ws),
+                                          0 if ws is None else ws.numel(), _stream(q))
+        _lib.check(rc, "gated_delta_rule")
+        ctx.save_for_backward(q, k, v, g, beta, keep)
+        return o, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go, glast):
+        q, k, v, g, beta, keep = ctx.saved_tensors
+        p = type(ctx.p).from_buffer_copy(ctx.p)         # of this call's own: the gradient's strides go in
+        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+        dg, dbeta = torch.empty_like(g), torch.empty_like(beta)
+        ds0 = None
+        if ctx.has_state and ctx.needs_input_grad[5]:
+            ds0 = torch.empty(p.B, p.HV, p.DK, p.DV, device=q.device, dtype=torch.float32)
+        if glast is not None:
+            glast = glast.contiguous()
+        if keep is None:                                # no steps
+            if ds0 is not None:
+                ds0.zero_() if glast is None else ds0.copy_(glast)
+            return dq, dk, dv, dg, dbeta, ds0, None, None, None
+        go = torch.zeros(v.shape, device=v.device, dtype=v.dtype) if go is None else go
+        go = go if go.stride(-1) == 1 or go.shape[-1] == 1 else go.contiguous()
+        p.go_stride = _strides(go)
+        lib = _lib.load()
+        with torch.cuda.device(q.device):
+            ws = _workspace(lib.aussm_b200_delta_workspace_bytes(p, 1), q.device)
+            rc = lib.aussm_b200_delta_bwd(p, _ptr(go), _ptr(glast), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(keep),
+                                          keep.numel(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dg), _ptr(dbeta), _ptr(ds0),
+                                          _ptr(ws), ws.numel(), _stream(q))
+        _lib.check(rc, "gated_delta_rule backward")
+        return dq, dk, dv, dg, dbeta, ds0, None, None, None
+
+
+def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, scale: Optional[float] = None,
+                     initial_state: Optional[Tensor] = None, return_final_state: bool = False):
+    """The gated delta rule over whole sequences; differentiable once in every tensor.
+
+    ``q, k`` are ``(b, l, hk, dk)`` and ``v`` ``(b, l, hv, dv)``, of one type (float32, bfloat16 or float16) and any
+    strides; ``hv`` is a multiple of ``hk`` and value head ``h`` reads key head ``h // (hv // hk)``.  ``g`` (logarithm of
+    the decay; -inf forgets the state) and ``beta`` (step size) are ``(b, l, hv)`` float32.  Keys are meant to have unit
+    length (``rotary.qk_norm_rotate``) and ``beta`` to lie in 0..2: otherwise the recurrence itself diverges.  A padded
+    step is one with ``g = beta = 0``: it leaves the state as it is.  ``scale`` defaults to ``dk ** -0.5``.
+    ``initial_state`` is ``(b, hv, dk, dv)`` float32 (None: zero).
+
+    Returns ``o`` ``(b, l, hv, dv)`` of the inputs' type, or ``(o, final_state)``."""
+    _refuse_traced("gated_delta_rule", q, k, v, g, beta, initial_state)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
+    o, last = _GatedDelta.apply(q, k, v, g, beta, initial_state, scale, bool(return_final_state), grad)
+    return (o, last) if return_final_state else o
+
+
+def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, state: Tensor, scale: Optional[float] = None,
+                     new_state: Optional[Tensor] = None) -> Tensor:
+    """One or a few new steps of every sequence, for serving: reads each state once and writes it once.
+
+    Tensors as in ``gated_delta_rule`` with ``l`` the number of new steps.  ``state`` ``(b, hv, dk, dv)`` float32
+    contiguous is updated in place, or left alone when ``new_state`` (same shape, no overlap) is given to take the
+    result.  Returns ``o``.  Not differentiable."""
+    _refuse_traced("gated_delta_step", q, k, v, g, beta, state, new_state)
+    tensors = (q, k, v, g, beta, state, new_state)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("gated_delta_step is not differentiable: call it under torch.no_grad(), or use gated_delta_rule")
+    p, q, k, v, g, beta = _check(q, k, v, g, beta, scale)
+    out = state if new_state is None else new_state
+    state = _state("state", state, p, q.device)
+    if not out.is_contiguous() or tuple(out.shape) != tuple(state.shape) or out.dtype != torch.float32 or out.device != q.device:
+        raise RuntimeError(f"the state that takes the result must be contiguous float32 {tuple(state.shape)} on {q.device}")
+    if new_state is not None and state.numel():
+        lo, hi, size = sorted((state.data_ptr(), out.data_ptr())) + [4 * state.numel()]
+        if lo != hi and hi < lo + size:
+            raise RuntimeError("new_state overlaps state in part")
+    o = torch.empty(p.B, p.L, p.HV, p.DV, device=q.device, dtype=q.dtype)
+    if o.numel() == 0:
+        if out.data_ptr() != state.data_ptr():
+            out.copy_(state)
+        return o
+    with torch.cuda.device(q.device):
+        rc = _lib.load().aussm_b200_delta_step(p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(out),
+                                               _ptr(o), _stream(q))
+    _lib.check(rc, "gated_delta_step")
+    return o

@@ -365,6 +365,77 @@ int aussm_b200_rms_norm_bwd(const float* g, const float* extra, /* may be NULL *
                             const float* x, const float* w, const float* rstd, float* dx, float* dw, long long rows,
                             int d, void* workspace, size_t workspace_bytes, aussm_stream_t stream);
 
+/* ---- gated delta rule --------------------------------------------------------
+ * A mixer with a matrix state (no counterpart in the reference).  Per batch entry
+ * and value head, with a_t = exp(g_t) and the state S (dk, dv):
+ *   e_t = beta_t (v_t - a_t S_{t-1}^T k_t),   S_t = a_t S_{t-1} + k_t e_t^T,   o_t = scale S_t^T q_t
+ * q, k: (B, L, HK, DK), v: (B, L, HV, DV), HV a multiple of HK (value head h uses
+ * key head h / (HV / HK)); their type is `dtype`, their last axis has unit stride
+ * and the other strides (batch, step, head; elements) are in the problem.  o and
+ * the gradients of q, k, v are contiguous, of the same type.  g, beta, dg, dbeta:
+ * (B, L, HV) float32 contiguous; states: (B, HV, DK, DV) float32 contiguous.  1 <=
+ * DK <= AUSSM_MAX_DELTA_KEY, 1 <= DV <= AUSSM_MAX_DELTA_VALUE.  All arithmetic has
+ * float32 accuracy whatever `dtype` is; outputs are rounded once.
+ * exp(g) below about 1e-38 counts as zero (g = -inf forgets the state).
+ * `keep` is what the backward call reads of its forward call (aussm_b200_delta_
+ * keep_bytes bytes; NULL when there will be none); the backward call leaves it as it
+ * is.  Deterministic: no atomics.  keep and workspace are 256-byte aligned. */
+#define AUSSM_MAX_DELTA_KEY 128
+#define AUSSM_MAX_DELTA_VALUE 256
+#define AUSSM_FLOAT32 0
+#define AUSSM_BFLOAT16 1
+#define AUSSM_FLOAT16 2
+typedef struct {
+    int B, L, HK, HV, DK, DV;
+    int dtype;
+    float scale;
+    long long q_stride[3], k_stride[3], v_stride[3], go_stride[3];   /* batch, step, head; go: the gradient of o */
+} aussm_b200_delta_t;
+size_t aussm_b200_delta_keep_bytes(const aussm_b200_delta_t* p);
+size_t aussm_b200_delta_workspace_bytes(const aussm_b200_delta_t* p, int backward);
+int aussm_b200_delta_fwd(const aussm_b200_delta_t* p, const void* q, const void* k, const void* v, const float* g,
+                         const float* beta, const float* s0, /* may be NULL (= 0) */
+                         void* o, float* s1, /* may be NULL */
+                         void* keep, size_t keep_bytes, void* workspace, size_t workspace_bytes, aussm_stream_t stream);
+/* gs1 (gradient of the final state) may be NULL (= 0), ds0 NULL (not wanted). */
+int aussm_b200_delta_bwd(const aussm_b200_delta_t* p, const void* go, const float* gs1, const void* q, const void* k,
+                         const void* v, const float* g, const float* beta, const void* keep, size_t keep_bytes,
+                         void* dq, void* dk, void* dv, float* dg, float* dbeta, float* ds0, void* workspace,
+                         size_t workspace_bytes, aussm_stream_t stream);
+/* The recurrence itself, for few steps: reads every state once and writes it once.
+ * new_state may be state. */
+int aussm_b200_delta_step(const aussm_b200_delta_t* p, const void* q, const void* k, const void* v, const float* g,
+                          const float* beta, const float* state, float* new_state, void* o, aussm_stream_t stream);
+
+/* ---- queries and keys: norm over each head and rotation by position --------------
+ * y = R(position) (x r w) over the last axis (d <= AUSSM_MAX_ROTATE_HEAD) of q (B, L, HQ, d) and k (B, L, HK, d):
+ * r = rsqrt(mean(x^2) + eps) (AUSSM_NORM_RMS), rsqrt(sum(x^2) + eps) (AUSSM_NORM_L2) or 1 (AUSSM_NORM_NONE); w a
+ * weight of d floats or NULL; R turns the pairs of the first `rot` elements by position * frequencies[pair] radians
+ * and multiplies them by `magnitude`: pair i is (i, i + rot/2), or (2i, 2i + 1) when interleaved.  frequencies:
+ * rot/2 doubles; positions: 64-bit, step t of entry b at [b * position_stride + t], NULL = t.  q, k and the gradients
+ * gq, gk of the results have unit stride along the last axis and strides (batch, step, head; elements) of their own;
+ * results are contiguous, of the same type.  The weights' gradients (float32, NULL = not wanted) are added in a fixed
+ * order. */
+#define AUSSM_MAX_ROTATE_HEAD 256
+#define AUSSM_NORM_NONE 0
+#define AUSSM_NORM_RMS 1
+#define AUSSM_NORM_L2 2
+typedef struct {
+    int B, L, HQ, HK, d, rot;
+    int dtype, norm, interleaved;
+    float eps, magnitude;
+    long long position_stride;
+    long long q_stride[3], k_stride[3], gq_stride[3], gk_stride[3];
+} aussm_b200_rotate_t;
+int aussm_b200_rotate_fwd(const aussm_b200_rotate_t* p, const void* q, const void* k, const double* frequencies,
+                          const long long* positions, const float* q_weight, const float* k_weight, void* yq, void* yk,
+                          aussm_stream_t stream);
+size_t aussm_b200_rotate_bwd_workspace_bytes(const aussm_b200_rotate_t* p);
+int aussm_b200_rotate_bwd(const aussm_b200_rotate_t* p, const void* gq, const void* gk, const void* q, const void* k,
+                          const double* frequencies, const long long* positions, const float* q_weight,
+                          const float* k_weight, void* dq, void* dk, float* dq_weight, float* dk_weight, void* workspace,
+                          size_t workspace_bytes, aussm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
