@@ -60,12 +60,12 @@ int launched(const char* who, cudaError_t e) {
 extern "C" {
 
 size_t aussm_b200_delta_keep_bytes(const aussm_b200_delta_t* p) {
-    return delta_check("delta_keep_bytes", p) ? 0 : delta_keep_bytes(*p);
+    return delta_check("delta_keep_bytes", p) ? 0 : delta_plan(*p).keep_bytes;
 }
 
 size_t aussm_b200_delta_workspace_bytes(const aussm_b200_delta_t* p, int backward) {
     if (delta_check("delta_workspace_bytes", p)) return 0;
-    return backward ? delta_bwd_bytes(*p) : delta_keep_bytes(*p);
+    return backward ? delta_plan(*p).bwd_bytes : delta_plan(*p).keep_bytes;
 }
 
 int aussm_b200_delta_fwd(const aussm_b200_delta_t* p, const void* q, const void* k, const void* v, const float* g,
@@ -77,7 +77,7 @@ int aussm_b200_delta_fwd(const aussm_b200_delta_t* p, const void* q, const void*
         return AUSSM_EINVAL;
     }
     if (keep) {
-        if (int rc = need("delta_fwd", "keep buffer", keep, keep_bytes, delta_keep_bytes(*p))) return rc;
+        if (int rc = need("delta_fwd", "keep buffer", keep, keep_bytes, delta_plan(*p).keep_bytes)) return rc;
     } else {
         if (int rc = need("delta_fwd", "workspace", workspace, workspace_bytes, aussm_b200_delta_workspace_bytes(p, 0))) return rc;
         keep = workspace;
@@ -94,8 +94,8 @@ int aussm_b200_delta_bwd(const aussm_b200_delta_t* p, const void* go, const floa
         set_error("delta_bwd: null input or output pointer");
         return AUSSM_EINVAL;
     }
-    if (int rc = need("delta_bwd", "keep buffer", keep, keep_bytes, delta_keep_bytes(*p))) return rc;
-    if (int rc = need("delta_bwd", "workspace", workspace, workspace_bytes, delta_bwd_bytes(*p))) return rc;
+    if (int rc = need("delta_bwd", "keep buffer", keep, keep_bytes, delta_plan(*p).keep_bytes)) return rc;
+    if (int rc = need("delta_bwd", "workspace", workspace, workspace_bytes, delta_plan(*p).bwd_bytes)) return rc;
     return launched("delta_bwd", launch_delta_bwd(*p, {q, k, v, g, beta}, go, gs1, keep, dq, dk, dv, dg, dbeta, ds0,
                                                   workspace, (cudaStream_t)stream));
 }

@@ -25,6 +25,56 @@ namespace aussm {
 
 constexpr int kDeltaChunk = 64;
 
+// ---- operand tiles -----------------------------------------------------------------------------------------------
+// Products run on FP16 parts: with S the power of two that brings a tile's largest magnitude to 2^13..2^14,
+// hi = fp16(S a), lo = fp16(S a - hi): 22 significant bits down to 2^-17 of the largest element and an absolute error of
+// 2^-39 of it below; a product is hi hi + hi lo + lo hi.  A tile of 64 rows is stored the way the tensor core reads it
+// from shared memory: panels of 64 columns (64 rows of 128 bytes, 16-byte pieces swizzled by the row), the hi panels
+// and then the lo panels.  Rows of 128 bytes serve as K-major and as MN-major operands alike.
+//
+// Per chunk and value head one record of such tiles (`key` = DK rounded up to 64 or 128):
+struct DeltaRecord {
+    int key;                                            // columns of W, Kt, Q
+    static constexpr int kHead = 1024;                  // bytes of the header
+    static constexpr int kSquare = 16384;               // bytes of a 64 x 64 tile, hi and lo
+    __host__ __device__ int tile() const { return key * 256; }
+    __host__ __device__ int w() const { return kHead; }                             // W = T beta e^G K
+    __host__ __device__ int kt() const { return kHead + tile(); }                   // Kt = e^(G_C - G) K
+    __host__ __device__ int q() const { return kHead + 2 * tile(); }                // Q as it is
+    __host__ __device__ int t() const { return kHead + 3 * tile(); }                // T = (I + A)^-1
+    __host__ __device__ int p() const { return kHead + 3 * tile() + kSquare; }      // P
+    __host__ __device__ int bytes() const { return kHead + 3 * tile() + 2 * kSquare; }
+};
+// header, in floats: what a stored part is to be multiplied with (1 / S) ...
+enum : int { kUnW = 0, kUnKt = 1, kUnQ = 2, kUnT = 3, kUnP = 4, kGamma = 5 /* e^(G_C) */,
+             kSince = 16 /* scale e^(G_i), 64 */, kGHi = 80, kGLo = 144 /* G_i = hi + lo, 64 each */ };
+
+// byte offset of element (row, col) in the hi panels of a tile
+__host__ __device__ __forceinline__ int panel_at(int row, int col) {
+    return (col >> 6) * 8192 + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
+}
+
+__host__ __device__ __forceinline__ float pow2_float(int k) {
+#ifdef __CUDA_ARCH__
+    return __uint_as_float((unsigned)(127 + k) << 23);
+#else
+    return 0.f;
+#endif
+}
+// exponent k of the scale 2^k for a tile whose largest magnitude is m
+__device__ __forceinline__ int part_exponent(float m) {
+    const int e = (int)((__float_as_uint(m) >> 23) & 0xffu) - 127;
+    return max(-100, min(100, 13 - e));
+}
+// hi and lo parts of two values that are scaled already, packed
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
 struct DeltaInputs {
     const void *q, *k, *v;
     const float *g, *beta;
@@ -41,6 +91,18 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return
 // exp(-200) is zero in float32: g of -inf (forget everything) would make differences of its sums NaN
 __device__ __forceinline__ float clamp_log_decay(float g) { return g < -200.f ? -200.f : g; }
 
+// Sizes and buffers of a problem.  keep: [records][V' (chunk heads, 64, DV)][entry states (chunk heads, DK, DV)]
+struct DeltaPlan {
+    int n;                 // chunks of a sequence
+    size_t heads;          // chunk heads: (b * HV + h) * n + chunk
+    DeltaRecord rec;
+    size_t keep_bytes, bwd_bytes;
+    size_t news, states;   // byte offsets in keep
+};
+DeltaPlan delta_plan(const aussm_b200_delta_t& p);
+
+cudaError_t launch_delta_prepare(const aussm_b200_delta_t& p, const DeltaPlan& plan, const DeltaInputs& in, void* records,
+                                 cudaStream_t stream);
 cudaError_t launch_delta_fwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const float* s0, void* o, float* s1,
                              void* keep, cudaStream_t stream);
 cudaError_t launch_delta_bwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const void* go, const float* gs1,
@@ -48,7 +110,5 @@ cudaError_t launch_delta_bwd(const aussm_b200_delta_t& p, const DeltaInputs& in,
                              void* workspace, cudaStream_t stream);
 cudaError_t launch_delta_step(const aussm_b200_delta_t& p, const DeltaInputs& in, const float* state, float* new_state,
                               void* o, cudaStream_t stream);
-size_t delta_keep_bytes(const aussm_b200_delta_t& p);
-size_t delta_bwd_bytes(const aussm_b200_delta_t& p);
 
 }  // namespace aussm

@@ -11,29 +11,38 @@ constexpr int NT = 256;
 constexpr int SLICE = 32;            // value columns of a block of the recurrences
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
-int chunks_of(const aussm_b200_delta_t& p) { return (p.L + C - 1) / C; }
-size_t heads_of(const aussm_b200_delta_t& p) { return (size_t)p.B * p.HV * chunks_of(p); }
 
-// per chunk and value head
-struct Record {
-    double *G;       // (C) sums of g: differences of large sums have to be right to 24 bits
-    float *T, *P;    // (C, C)
-    float *W;        // (C, DK)
-    float *N;        // (C, DV): V'
-    float *S;        // (DK, DV): entry state
+// a stored tile as the numbers it stands for
+struct Tile {
+    const uint8_t* p;
+    int lo;
+    float un;
+    __device__ float operator()(int i, int j) const {
+        const uint8_t* at = p + panel_at(i, j);
+        return (__half2float(*reinterpret_cast<const __half*>(at)) + __half2float(*reinterpret_cast<const __half*>(at + lo))) * un;
+    }
 };
-Record record_at(const aussm_b200_delta_t& p, void* keep) {
-    const size_t n = heads_of(p);
-    Record r;
-    r.G = static_cast<double*>(keep);
-    float* f = reinterpret_cast<float*>(r.G + n * C);
-    r.T = f; f += n * C * C;
-    r.P = f; f += n * C * C;
-    r.W = f; f += n * C * p.DK;
-    r.N = f; f += n * C * p.DV;
-    r.S = f;
-    return r;
-}
+struct Header {
+    const float* f;
+    __device__ float diff(int i, int j) const { return (f[kGHi + i] - f[kGHi + j]) + (f[kGLo + i] - f[kGLo + j]); }
+    __device__ float since(int i) const { return expf(f[kGHi + i] + f[kGLo + i]); }
+    __device__ float until(int i) const { return expf(diff(C - 1, i)); }
+};
+struct Record {
+    Header G;
+    Tile W, Kt, Q, T, P;
+    __device__ Record(const uint8_t* base, const DeltaRecord& r, size_t at) {
+        const uint8_t* p = base + at * r.bytes();
+        const float* f = reinterpret_cast<const float*>(p);
+        const int lo = r.key * 128;
+        G.f = f;
+        W = {p + r.w(), lo, f[kUnW]};
+        Kt = {p + r.kt(), lo, f[kUnKt]};
+        Q = {p + r.q(), lo, f[kUnQ]};
+        T = {p + r.t(), 8192, f[kUnT]};
+        P = {p + r.p(), 8192, f[kUnP]};
+    }
+};
 
 struct Params {
     aussm_b200_delta_t p;
@@ -42,7 +51,9 @@ struct Params {
     const float *s0, *gs1;
     void* o;
     float *s1, *ds0;
-    Record r;
+    const uint8_t* records;
+    DeltaRecord rec;
+    float *N, *S;              // V' and entry states of every chunk and head
     float *X, *dN, *dS;        // backward: (C, DV) twice, (DK, DV) per chunk and head
     void *dq, *dk, *dv;
     float *dg, *dbeta;
@@ -72,45 +83,6 @@ __device__ void products(int M, int N, int K, F term, G store) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT) prepare_kernel(const Params a) {
-    __shared__ float A[C][C + 1], be[C];
-    __shared__ double G[C];
-    const aussm_b200_delta_t& p = a.p;
-    const int c = blockIdx.x % a.n, bh = blockIdx.x / a.n, b = bh / p.HV, h = bh % p.HV, hk = h / (p.HV / p.HK);
-    const int t0 = c * C, rows = min(C, p.L - t0);
-    const Rows<T> q = rows_of<T>(a.in.q, p.q_stride, b, t0, hk, p.L), k = rows_of<T>(a.in.k, p.k_stride, b, t0, hk, p.L);
-    const size_t at = blockIdx.x;
-    float *Tm = a.r.T + at * C * C, *P = a.r.P + at * C * C, *W = a.r.W + at * C * p.DK;
-    if (threadIdx.x == 0) {
-        double s = 0;
-        for (int i = 0; i < C; ++i) {
-            const long long o = ((long long)b * p.L + t0 + i) * p.HV + h;
-            s += i < rows ? clamp_log_decay(a.in.g[o]) : 0.f;
-            G[i] = s;
-            be[i] = i < rows ? a.in.beta[o] : 0.f;
-            a.r.G[at * C + i] = G[i];
-        }
-    }
-    __syncthreads();
-    products(C, C, p.DK, [&](int i, int j, int x) { return j < i ? k(i, x) * k(j, x) : 0.f; },
-             [&](int i, int j, float v) { A[i][j] = j < i ? be[i] * expf((float)(G[i] - G[j])) * v : 0.f; });
-    products(C, C, p.DK, [&](int i, int j, int x) { return j <= i ? q(i, x) * k(j, x) : 0.f; },
-             [&](int i, int j, float v) { P[i * C + j] = j <= i ? p.scale * expf((float)(G[i] - G[j])) * v : 0.f; });
-    __syncthreads();
-    if (threadIdx.x < C) {           // column j of T by forward substitution
-        const int j = threadIdx.x;
-        for (int i = 0; i < C; ++i) {
-            float s = i == j ? 1.f : 0.f;
-            for (int m = j; m < i; ++m) s -= A[i][m] * Tm[m * C + j];
-            Tm[i * C + j] = i < j ? 0.f : s;
-        }
-    }
-    __syncthreads();
-    products(C, p.DK, C, [&](int i, int x, int j) { return j <= i ? Tm[i * C + j] * be[j] * expf((float)(G[j])) * k(j, x) : 0.f; },
-             [&](int i, int x, float v) { W[i * p.DK + x] = v; });
-}
-
-template <typename T>
 __global__ void __launch_bounds__(NT) forward_kernel(const Params a) {
     extern __shared__ float S[];     // (DK, SLICE)
     const aussm_b200_delta_t& p = a.p;
@@ -122,28 +94,27 @@ __global__ void __launch_bounds__(NT) forward_kernel(const Params a) {
     for (int c = 0; c < a.n; ++c) {
         const int t0 = c * C, rows = min(C, p.L - t0);
         const size_t at = (size_t)bh * a.n + c;
-        const double* G = a.r.G + at * C;
-        const float *Tm = a.r.T + at * C * C, *P = a.r.P + at * C * C, *W = a.r.W + at * C * p.DK;
-        float* N = a.r.N + at * C * p.DV + v0;
+        const Record r(a.records, a.rec, at);
+        float* N = a.N + at * C * p.DV + v0;
         const Rows<T> q = rows_of<T>(a.in.q, p.q_stride, b, t0, hk, p.L), k = rows_of<T>(a.in.k, p.k_stride, b, t0, hk, p.L),
                       v = rows_of<T>(a.in.v, p.v_stride, b, t0, h, p.L);
         const float* be = a.in.beta + ((long long)b * p.L + t0) * p.HV + h;
         for (int e = threadIdx.x; e < p.DK * nv; e += NT)
-            a.r.S[(at * p.DK + e / nv) * p.DV + v0 + e % nv] = S[e / nv * SLICE + e % nv];
+            a.S[(at * p.DK + e / nv) * p.DV + v0 + e % nv] = S[e / nv * SLICE + e % nv];
         products(C, nv, C + p.DK, [&](int i, int j, int m) {
-            if (m >= C) return -W[i * p.DK + m - C] * S[(m - C) * SLICE + j];
-            return m <= i && m < rows ? Tm[i * C + m] * be[(long long)m * p.HV] * v(m, v0 + j) : 0.f;
+            if (m >= C) return -r.W(i, m - C) * S[(m - C) * SLICE + j];
+            return m <= i && m < rows ? r.T(i, m) * be[(long long)m * p.HV] * v(m, v0 + j) : 0.f;
         }, [&](int i, int j, float x) { N[(size_t)i * p.DV + j] = x; });
         __syncthreads();
         products(rows, nv, C + p.DK, [&](int i, int j, int m) {
-            if (m >= C) return p.scale * expf((float)(G[i])) * q(i, m - C) * S[(m - C) * SLICE + j];
-            return m <= i ? P[i * C + m] * N[(size_t)m * p.DV + j] : 0.f;
+            if (m >= C) return r.G.f[kSince + i] * r.Q(i, m - C) * S[(m - C) * SLICE + j];
+            return m <= i ? r.P(i, m) * N[(size_t)m * p.DV + j] : 0.f;
         }, [&](int i, int j, float x) {
             static_cast<T*>(a.o)[(((long long)b * p.L + t0 + i) * p.HV + h) * p.DV + v0 + j] = from_f32<T>(x);
         });
         __syncthreads();
-        products(p.DK, nv, C, [&](int x, int j, int i) { return expf((float)(G[C - 1] - G[i])) * k(i, x) * N[(size_t)i * p.DV + j]; },
-                 [&](int x, int j, float s) { S[x * SLICE + j] = expf((float)(G[C - 1])) * S[x * SLICE + j] + s; });
+        products(p.DK, nv, C, [&](int x, int j, int i) { return r.Kt(i, x) * N[(size_t)i * p.DV + j]; },
+                 [&](int x, int j, float s) { S[x * SLICE + j] = r.G.f[kGamma] * S[x * SLICE + j] + s; });
         __syncthreads();
     }
     if (a.s1)
@@ -163,8 +134,7 @@ __global__ void __launch_bounds__(NT) backward_kernel(const Params a) {
     for (int c = a.n - 1; c >= 0; --c) {
         const int t0 = c * C, rows = min(C, p.L - t0);
         const size_t at = (size_t)bh * a.n + c;
-        const double* G = a.r.G + at * C;
-        const float *Tm = a.r.T + at * C * C, *P = a.r.P + at * C * C, *W = a.r.W + at * C * p.DK;
+        const Record r(a.records, a.rec, at);
         float *dN = a.dN + at * C * p.DV + v0, *X = a.X + at * C * p.DV + v0;
         const Rows<T> q = rows_of<T>(a.in.q, p.q_stride, b, t0, hk, p.L), k = rows_of<T>(a.in.k, p.k_stride, b, t0, hk, p.L),
                       go = rows_of<T>(a.go, p.go_stride, b, t0, h, p.L);
@@ -172,11 +142,11 @@ __global__ void __launch_bounds__(NT) backward_kernel(const Params a) {
         for (int e = threadIdx.x; e < p.DK * nv; e += NT)
             a.dS[(at * p.DK + e / nv) * p.DV + v0 + e % nv] = dS[e / nv * SLICE + e % nv];
         products(C, nv, C + p.DK, [&](int i, int j, int m) {
-            if (m >= C) return expf((float)(G[C - 1] - G[i])) * k(i, m - C) * dS[(m - C) * SLICE + j];
-            return m >= i ? P[m * C + i] * go(m, v0 + j) : 0.f;
+            if (m >= C) return r.Kt(i, m - C) * dS[(m - C) * SLICE + j];
+            return m >= i ? r.P(m, i) * go(m, v0 + j) : 0.f;
         }, [&](int i, int j, float x) { dN[(size_t)i * p.DV + j] = x; });
         __syncthreads();
-        products(C, nv, C, [&](int i, int j, int m) { return m >= i ? Tm[m * C + i] * dN[(size_t)m * p.DV + j] : 0.f; },
+        products(C, nv, C, [&](int i, int j, int m) { return m >= i ? r.T(m, i) * dN[(size_t)m * p.DV + j] : 0.f; },
                  [&](int i, int j, float x) {
                      X[(size_t)i * p.DV + j] = x;
                      if (i < rows)
@@ -184,8 +154,8 @@ __global__ void __launch_bounds__(NT) backward_kernel(const Params a) {
                              from_f32<T>(be[(long long)i * p.HV] * x);
                  });
         products(p.DK, nv, C, [&](int x, int j, int i) {
-            return p.scale * expf((float)(G[i])) * q(i, x) * go(i, v0 + j) - W[i * p.DK + x] * dN[(size_t)i * p.DV + j];
-        }, [&](int x, int j, float s) { dS[x * SLICE + j] = expf((float)(G[C - 1])) * dS[x * SLICE + j] + s; });
+            return r.G.f[kSince + i] * r.Q(i, x) * go(i, v0 + j) - r.W(i, x) * dN[(size_t)i * p.DV + j];
+        }, [&](int x, int j, float s) { dS[x * SLICE + j] = r.G.f[kGamma] * dS[x * SLICE + j] + s; });
         __syncthreads();
     }
     if (a.ds0)
@@ -205,8 +175,9 @@ __global__ void __launch_bounds__(NT) gradients_kernel(const Params a) {
     for (int e = threadIdx.x; e < 2 * C * DK; e += NT) dQ[e] = 0.f;
     for (int h = hk * r; h < hk * r + r; ++h) {
         const size_t at = ((size_t)b * p.HV + h) * a.n + c;
-        const double* G = a.r.G + at * C;
-        const float *N = a.r.N + at * C * DV, *X = a.X + at * C * DV, *S = a.r.S + at * DK * DV,
+        const Record rc(a.records, a.rec, at);
+        const Header& G = rc.G;
+        const float *N = a.N + at * C * DV, *X = a.X + at * C * DV, *S = a.S + at * DK * DV,
                     *dS = a.dS + at * DK * DV;
         const Rows<T> go = rows_of<T>(a.go, p.go_stride, b, t0, h, p.L), v = rows_of<T>(a.in.v, p.v_stride, b, t0, h, p.L);
         const float* beta = a.in.beta + ((long long)b * p.L + t0) * p.HV + h;
@@ -215,9 +186,9 @@ __global__ void __launch_bounds__(NT) gradients_kernel(const Params a) {
         for (int e = threadIdx.x; e < 3 * C; e += NT) dG[e] = 0.f;
         __syncthreads();
         products(C, C, DV, [&](int i, int j, int x) { return j <= i ? go(i, x) * N[(size_t)j * DV + x] : 0.f; },
-                 [&](int i, int j, float x) { Ep[i * C + j] = j <= i ? p.scale * expf((float)(G[i] - G[j])) * x : 0.f; });
+                 [&](int i, int j, float x) { Ep[i * C + j] = j <= i ? p.scale * expf(G.diff(i, j)) * x : 0.f; });
         products(C, C, DV, [&](int i, int j, int x) { return j < i ? X[(size_t)i * DV + x] * N[(size_t)j * DV + x] : 0.f; },
-                 [&](int i, int j, float x) { E[i * C + j] = j < i ? -expf((float)(G[i] - G[j])) * x : 0.f; });      // beta follows
+                 [&](int i, int j, float x) { E[i * C + j] = j < i ? -expf(G.diff(i, j)) * x : 0.f; });      // beta follows
         __syncthreads();
         if (threadIdx.x < C) {
             const int i = threadIdx.x;
@@ -236,7 +207,7 @@ __global__ void __launch_bounds__(NT) gradients_kernel(const Params a) {
         }
         __syncthreads();
         for (int i = threadIdx.x; i < C; i += NT) {            // row i: the terms with states
-            const float since = expf((float)(G[i])), until = expf((float)(G[C - 1] - G[i]));
+            const float since = G.since(i), until = G.until(i);
             float kz = 0.f, kkt = 0.f, qqt = 0.f;
             for (int x = 0; x < DK; ++x) {
                 float dqt = 0.f, z = 0.f, dkt = 0.f;
@@ -267,7 +238,7 @@ __global__ void __launch_bounds__(NT) gradients_kernel(const Params a) {
             const int t = threadIdx.x;
             float ss = 0.f, sum = 0.f;
             for (int e = 0; e < DK * DV; ++e) ss += dS[e] * S[e];
-            sum = expf((float)(G[C - 1])) * ss;
+            sum = G.f[kGamma] * ss;
             for (int i = 0; i < t; ++i) sum += dGs[i];
             for (int i = t; i < C; ++i) {
                 sum += dG[i];
@@ -288,9 +259,8 @@ __global__ void __launch_bounds__(NT) gradients_kernel(const Params a) {
 
 template <typename T>
 cudaError_t forward(const Params& a, cudaStream_t st) {
-    prepare_kernel<T><<<(unsigned)heads_of(a.p), NT, 0, st>>>(a);
     forward_kernel<T><<<dim3(a.p.B * a.p.HV, (a.p.DV + SLICE - 1) / SLICE), NT, a.p.DK * SLICE * 4, st>>>(a);
-    count_launch(2);
+    count_launch();
     return cudaGetLastError();
 }
 
@@ -307,17 +277,34 @@ cudaError_t backward(const Params& a, cudaStream_t st) {
 
 }  // namespace
 
-size_t delta_keep_bytes(const aussm_b200_delta_t& p) {
-    return up256(heads_of(p) * (size_t)(2 * C + 2 * C * C + C * p.DK + C * p.DV + p.DK * p.DV) * 4);
+DeltaPlan delta_plan(const aussm_b200_delta_t& p) {
+    DeltaPlan d;
+    d.n = (p.L + C - 1) / C;
+    d.heads = (size_t)p.B * p.HV * d.n;
+    d.rec.key = p.DK <= 64 ? 64 : 128;
+    d.news = d.heads * d.rec.bytes();
+    d.states = d.news + up256(d.heads * C * p.DV * sizeof(float));
+    d.keep_bytes = d.states + up256(d.heads * p.DK * p.DV * sizeof(float));
+    d.bwd_bytes = up256(d.heads * (size_t)(2 * C * p.DV + p.DK * p.DV) * 4);
+    return d;
 }
-size_t delta_bwd_bytes(const aussm_b200_delta_t& p) {
-    return up256(heads_of(p) * (size_t)(2 * C * p.DV + p.DK * p.DV) * 4);
+
+static Params params(const aussm_b200_delta_t& p, const DeltaPlan& plan, const DeltaInputs& in, void* keep) {
+    Params a = {};
+    uint8_t* k = static_cast<uint8_t*>(keep);
+    a.p = p; a.in = in; a.n = plan.n; a.rec = plan.rec; a.records = k;
+    a.N = reinterpret_cast<float*>(k + plan.news);
+    a.S = reinterpret_cast<float*>(k + plan.states);
+    return a;
 }
 
 cudaError_t launch_delta_fwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const float* s0, void* o, float* s1,
                              void* keep, cudaStream_t st) {
-    Params a = {};
-    a.p = p; a.in = in; a.s0 = s0; a.o = o; a.s1 = s1; a.r = record_at(p, keep); a.n = chunks_of(p);
+    const DeltaPlan plan = delta_plan(p);
+    cudaError_t e = launch_delta_prepare(p, plan, in, keep, st);
+    if (e != cudaSuccess) return e;
+    Params a = params(p, plan, in, keep);
+    a.s0 = s0; a.o = o; a.s1 = s1;
     return p.dtype == AUSSM_FLOAT32 ? forward<float>(a, st) : p.dtype == AUSSM_BFLOAT16 ? forward<__nv_bfloat16>(a, st)
                                                                                        : forward<__half>(a, st);
 }
@@ -325,13 +312,13 @@ cudaError_t launch_delta_fwd(const aussm_b200_delta_t& p, const DeltaInputs& in,
 cudaError_t launch_delta_bwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const void* go, const float* gs1,
                              const void* keep, void* dq, void* dk, void* dv, float* dg, float* dbeta, float* ds0,
                              void* ws, cudaStream_t st) {
-    Params a = {};
-    a.p = p; a.in = in; a.go = go; a.gs1 = gs1; a.r = record_at(p, const_cast<void*>(keep)); a.n = chunks_of(p);
+    const DeltaPlan plan = delta_plan(p);
+    Params a = params(p, plan, in, const_cast<void*>(keep));
+    a.go = go; a.gs1 = gs1;
     a.dq = dq; a.dk = dk; a.dv = dv; a.dg = dg; a.dbeta = dbeta; a.ds0 = ds0;
-    const size_t n = heads_of(p);
     a.X = static_cast<float*>(ws);
-    a.dN = a.X + n * C * p.DV;
-    a.dS = a.dN + n * C * p.DV;
+    a.dN = a.X + plan.heads * C * p.DV;
+    a.dS = a.dN + plan.heads * C * p.DV;
     return p.dtype == AUSSM_FLOAT32 ? backward<float>(a, st) : p.dtype == AUSSM_BFLOAT16 ? backward<__nv_bfloat16>(a, st)
                                                                                         : backward<__half>(a, st);
 }

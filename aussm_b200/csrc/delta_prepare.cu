@@ -1,0 +1,487 @@
+// Gated delta rule, what a chunk of 64 steps needs and no state enters: A, T = (I + A)^-1, W, P and the operand tiles
+// of Kt and Q (formulas in delta.cuh), written as the records that the recurrences read.
+//
+// One block per chunk and key head; K K^T and Q K^T serve all value heads of the key head.  All products run on the
+// FP16 parts with mma.sync (two blocks an SM, 8 warps each, warp = 16 rows x half of the columns), skipping the 16 x 16
+// blocks above the diagonal.  Differences of the sums of g are taken from pairs of floats: sums reach thousands, and
+// e^(G_i - G_j) has to be right to 24 bits where G_i - G_j is small.
+#include "common.cuh"
+#include "delta.cuh"
+#include "host_common.cuh"
+
+namespace aussm {
+namespace {
+
+constexpr int C = kDeltaChunk;
+constexpr int NT = 256;
+constexpr int PITCH = 68;                // floats of a row of A / T: rows start on 16 bytes
+
+struct PrepareParams {
+    aussm_b200_delta_t p;
+    DeltaInputs in;
+    uint8_t* records;
+    DeltaRecord rec;
+    int n;
+    int vec_q, vec_k;                    // rows can be read 16 bytes at a time
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// eight consecutive elements of a row, zeros from `cols` on
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int c, int cols, bool vec, float (&f)[8]) {
+    if (vec) {
+        if (c < cols) {
+            constexpr int N = 16 / sizeof(T);
+            struct alignas(16) Raw { T v[N]; };
+#pragma unroll
+            for (int k = 0; k < 8 / N; ++k) {
+                const Raw r = *reinterpret_cast<const Raw*>(row + c + k * N);
+#pragma unroll
+                for (int i = 0; i < N; ++i) f[k * N + i] = to_f32(r.v[i]);
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = c + i < cols ? to_f32(row[c + i]) : 0.f;
+    }
+}
+
+__device__ __forceinline__ void split8(const float (&f)[8], float s, uint4& hi, uint4& lo) {
+    split2(f[0] * s, f[1] * s, hi.x, lo.x);
+    split2(f[2] * s, f[3] * s, hi.y, lo.y);
+    split2(f[4] * s, f[5] * s, hi.z, lo.z);
+    split2(f[6] * s, f[7] * s, hi.w, lo.w);
+}
+
+// maxima of three values over the block; `buf` has 3 * 8 floats and is free again after the next barrier
+__device__ __forceinline__ void block_max3(float& a, float& b, float& c, float* buf) {
+#pragma unroll
+    for (int m = 16; m; m >>= 1) {
+        a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, m));
+        b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, m));
+        c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, m));
+    }
+    const int w = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) { buf[w] = a; buf[8 + w] = b; buf[16 + w] = c; }
+    __syncthreads();
+    a = b = c = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) {
+        a = fmaxf(a, buf[i]);
+        b = fmaxf(b, buf[8 + i]);
+        c = fmaxf(c, buf[16 + i]);
+    }
+}
+
+// 4 x 4 words of a quad of lanes change places: lane t comes to hold word t of lanes 0..3
+__device__ __forceinline__ void quad_transpose(uint32_t (&w)[4], int t) {
+    const bool o = t & 1, u = t & 2;
+    const uint32_t a = __shfl_xor_sync(0xffffffffu, o ? w[0] : w[1], 1), b = __shfl_xor_sync(0xffffffffu, o ? w[2] : w[3], 1);
+    if (o) { w[0] = a; w[2] = b; } else { w[1] = a; w[3] = b; }
+    const uint32_t c = __shfl_xor_sync(0xffffffffu, u ? w[0] : w[2], 2), d = __shfl_xor_sync(0xffffffffu, u ? w[1] : w[3], 2);
+    if (u) { w[0] = c; w[1] = d; } else { w[2] = c; w[3] = d; }
+}
+
+// Accumulator fragments of four neighbouring 8-column tiles (columns col0..col0+31) to a tile in memory: each lane puts
+// together the 16-byte pieces of one of the four.
+__device__ __forceinline__ void store_fragments(uint8_t* tile, int lo_off, int row0, int col0, const float (&c)[4][4], float s) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) split2(c[x][2 * half] * s, c[x][2 * half + 1] * s, hi[x], lo[x]);
+        quad_transpose(hi, t);
+        quad_transpose(lo, t);
+        uint8_t* at = tile + panel_at(row0 + g + 8 * half, col0 + 8 * t);
+        *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(at + lo_off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+
+// T = (I + A)^-1 in place of the strictly lower triangular A (zeros elsewhere): 16 x 16 diagonal blocks by forward
+// substitution, then twice by halves, T21 = -T22 A21 T11.
+__device__ __forceinline__ void invert(float* A, float* tmp) {
+    const int tid = threadIdx.x;
+    if (tid < C) {
+        const int d = (tid >> 4) * 16, j = tid & 15;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float s = i == j ? 1.f : 0.f;
+#pragma unroll
+            for (int m = 0; m < i; ++m) s = fmaf(-A[(d + i) * PITCH + d + m], x[m], s);
+            x[i] = s;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) A[(d + i) * PITCH + d + j] = x[i];
+    }
+    __syncthreads();
+    {   // 32 x 32: two pairs of blocks, 128 threads each, two rows of one column per thread
+        const int e = (tid >> 7) * 32, j = tid & 15, i = (tid & 127) >> 4;
+        float s[2] = {};
+#pragma unroll
+        for (int m = 0; m < 16; ++m) {
+            const float t = A[(e + m) * PITCH + e + j];
+            s[0] = fmaf(A[(e + 16 + i) * PITCH + e + m], t, s[0]);
+            s[1] = fmaf(A[(e + 24 + i) * PITCH + e + m], t, s[1]);
+        }
+        tmp[(e + i) * 33 + j] = s[0];
+        tmp[(e + i + 8) * 33 + j] = s[1];
+        __syncthreads();
+        s[0] = s[1] = 0.f;
+#pragma unroll
+        for (int m = 0; m < 16; ++m) {
+            const float t = tmp[(e + m) * 33 + j];
+            s[0] = fmaf(A[(e + 16 + i) * PITCH + e + 16 + m], t, s[0]);
+            s[1] = fmaf(A[(e + 24 + i) * PITCH + e + 16 + m], t, s[1]);
+        }
+        A[(e + 16 + i) * PITCH + e + j] = -s[0];
+        A[(e + 24 + i) * PITCH + e + j] = -s[1];
+    }
+    __syncthreads();
+    {   // 64 x 64: 2 x 2 elements per thread
+        const int j = (tid & 15) * 2, i = (tid >> 4) * 2;
+        float s[2][2] = {};
+#pragma unroll 8
+        for (int m = 0; m < 32; ++m) {
+            const float2 t = *reinterpret_cast<const float2*>(A + m * PITCH + j);
+            const float a = A[(32 + i) * PITCH + m], b = A[(33 + i) * PITCH + m];
+            s[0][0] = fmaf(a, t.x, s[0][0]); s[0][1] = fmaf(a, t.y, s[0][1]);
+            s[1][0] = fmaf(b, t.x, s[1][0]); s[1][1] = fmaf(b, t.y, s[1][1]);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) { tmp[(i + x) * 34 + j] = s[x][0]; tmp[(i + x) * 34 + j + 1] = s[x][1]; }
+        __syncthreads();
+        s[0][0] = s[0][1] = s[1][0] = s[1][1] = 0.f;
+#pragma unroll 8
+        for (int m = 0; m < 32; ++m) {
+            const float2 t = *reinterpret_cast<const float2*>(tmp + m * 34 + j);
+            const float a = A[(32 + i) * PITCH + 32 + m], b = A[(33 + i) * PITCH + 32 + m];
+            s[0][0] = fmaf(a, t.x, s[0][0]); s[0][1] = fmaf(a, t.y, s[0][1]);
+            s[1][0] = fmaf(b, t.x, s[1][0]); s[1][1] = fmaf(b, t.y, s[1][1]);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) { A[(32 + i + x) * PITCH + j] = -s[x][0]; A[(32 + i + x) * PITCH + j + 1] = -s[x][1]; }
+    }
+    __syncthreads();
+}
+
+template <int KEY>
+struct PrepareSmem {
+    static constexpr int kTile = KEY * 256;
+    static constexpr int kQ = kTile > DeltaRecord::kSquare ? kTile : DeltaRecord::kSquare;    // Q, then T beta e^G
+    static constexpr int kBytes = kTile + kQ + C * PITCH * 4 + 64 * 34 * 4 + 5 * C * 4 + 64 * 4;
+};
+
+template <typename T, int KEY>
+__global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParams a) {
+    using Smem = PrepareSmem<KEY>;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint8_t *kr = sm, *qr = sm + Smem::kTile;
+    float* A = reinterpret_cast<float*>(qr + Smem::kQ);
+    float *tmp = A + C * PITCH, *ghi = tmp + 64 * 34, *glo = ghi + C, *be = glo + C, *until = be + C, *left = until + C, *red = left + C;
+    constexpr int LO = KEY * 128;                                     // lo panels behind the hi panels
+    const aussm_b200_delta_t& p = a.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int r = p.HV / p.HK, c = blockIdx.x % a.n, bk = blockIdx.x / a.n, b = bk / p.HK, hk = bk % p.HK;
+    const int t0 = c * C, rows = min(C, p.L - t0);
+    const T* q = static_cast<const T*>(a.in.q) + b * p.q_stride[0] + t0 * p.q_stride[1] + hk * p.q_stride[2];
+    const T* k = static_cast<const T*>(a.in.k) + b * p.k_stride[0] + t0 * p.k_stride[1] + hk * p.k_stride[2];
+    auto record = [&](int h) { return a.records + (((size_t)b * p.HV + h) * a.n + c) * a.rec.bytes(); };
+
+    // K and Q: 16-byte pieces of a tile, KEY / 32 of each per thread
+    constexpr int PIECES = C * KEY / 8 / NT;
+    int ek, eq;
+    {
+        float fk[PIECES][8], fq[PIECES][8], mk = 0.f, mq = 0.f, none = 0.f;
+#pragma unroll
+        for (int x = 0; x < PIECES; ++x) {
+            const int piece = tid + x * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8;
+            if (row < rows) {
+                load8(k + row * p.k_stride[1], col, p.DK, a.vec_k, fk[x]);
+                load8(q + row * p.q_stride[1], col, p.DK, a.vec_q, fq[x]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) fk[x][i] = fq[x][i] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < PIECES; ++x)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { mk = fmaxf(mk, fabsf(fk[x][i])); mq = fmaxf(mq, fabsf(fq[x][i])); }
+        block_max3(mk, mq, none, red);
+        ek = part_exponent(mk);
+        eq = part_exponent(mq);
+        const float sk = pow2_float(ek), sq = pow2_float(eq);
+#pragma unroll
+        for (int x = 0; x < PIECES; ++x) {
+            const int piece = tid + x * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8, at = panel_at(row, col);
+            uint4 hi, lo;
+            split8(fk[x], sk, hi, lo);
+            *reinterpret_cast<uint4*>(kr + at) = hi;
+            *reinterpret_cast<uint4*>(kr + LO + at) = lo;
+            split8(fq[x], sq, hi, lo);
+            *reinterpret_cast<uint4*>(qr + at) = hi;
+            *reinterpret_cast<uint4*>(qr + LO + at) = lo;
+            for (int h = hk * r; h < hk * r + r; ++h) {
+                uint8_t* dst = record(h) + a.rec.q() + at;
+                *reinterpret_cast<uint4*>(dst) = hi;
+                *reinterpret_cast<uint4*>(dst + LO) = lo;
+            }
+        }
+    }
+    __syncthreads();
+
+    // K K^T and Q K^T on and below the diagonal blocks: warp = rows rb*16.., columns half*32..
+    const int rb = warp & 3, half = warp >> 2;
+    const uint32_t ks = smem_addr(kr), qs = smem_addr(qr);
+    float kk[4][4] = {}, qk[4][4] = {};
+    {
+        const int arow = rb * 16 + (lane & 15), acol = (lane >> 4) * 8;
+        const int brow = (lane & 7) + ((lane >> 4) << 3), bcol = ((lane >> 3) & 1) * 8;
+#pragma unroll
+        for (int k0 = 0; k0 < KEY; k0 += 16) {
+            uint32_t kh[4], kl[4], qh[4], ql[4];
+            const int at = panel_at(arow, k0 + acol);
+            ldmatrix4(kh, ks + at);
+            ldmatrix4(kl, ks + LO + at);
+            ldmatrix4(qh, qs + at);
+            ldmatrix4(ql, qs + LO + at);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int n0 = half * 32 + x * 16;
+                if (n0 > rb * 16) continue;
+                uint32_t bh[4], bl[4];
+                const int bt = panel_at(n0 + brow, k0 + bcol);
+                ldmatrix4(bh, ks + bt);
+                ldmatrix4(bl, ks + LO + bt);
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    mma16816(kk[2 * x + y], kl, bh[2 * y], bh[2 * y + 1]);
+                    mma16816(qk[2 * x + y], ql, bh[2 * y], bh[2 * y + 1]);
+                    mma16816(kk[2 * x + y], kh, bl[2 * y], bl[2 * y + 1]);
+                    mma16816(qk[2 * x + y], qh, bl[2 * y], bl[2 * y + 1]);
+                    mma16816(kk[2 * x + y], kh, bh[2 * y], bh[2 * y + 1]);
+                    mma16816(qk[2 * x + y], qh, bh[2 * y], bh[2 * y + 1]);
+                }
+            }
+        }
+    }
+    const float unk = pow2_float(-ek), unq = pow2_float(-eq);
+
+    for (int h = hk * r; h < hk * r + r; ++h) {
+        uint8_t* rec = record(h);
+        float* head = reinterpret_cast<float*>(rec);
+        __syncthreads();                       // the last value head's T beta e^G and vectors are read
+        if (warp == 0) {
+            const long long o = ((long long)b * p.L + t0) * p.HV + h;
+            const int i0 = 2 * lane, i1 = i0 + 1;
+            const double g0 = i0 < rows ? clamp_log_decay(a.in.g[o + (long long)i0 * p.HV]) : 0.f;
+            const double g1 = i1 < rows ? clamp_log_decay(a.in.g[o + (long long)i1 * p.HV]) : 0.f;
+            be[i0] = i0 < rows ? a.in.beta[o + (long long)i0 * p.HV] : 0.f;
+            be[i1] = i1 < rows ? a.in.beta[o + (long long)i1 * p.HV] : 0.f;
+            double s = g0 + g1;
+#pragma unroll
+            for (int m = 1; m < 32; m *= 2) {
+                const double v = __shfl_up_sync(0xffffffffu, s, m);
+                if (lane >= m) s += v;
+            }
+            const double before = s - g1, all = __shfl_sync(0xffffffffu, s, 31);
+            const float h0 = (float)before, h1 = (float)s;
+            const float u0 = expf((float)(all - before)), u1 = expf((float)(all - s));
+            ghi[i0] = h0; ghi[i1] = h1;
+            glo[i0] = (float)(before - h0); glo[i1] = (float)(s - h1);
+            until[i0] = u0; until[i1] = u1;
+            const float e0 = expf((float)before), e1 = expf((float)s);
+            left[i0] = be[i0] * e0; left[i1] = be[i1] * e1;                 // what T's columns are multiplied with for W
+            head[kSince + i0] = p.scale * e0; head[kSince + i1] = p.scale * e1;
+            head[kGHi + i0] = h0; head[kGHi + i1] = h1;
+            head[kGLo + i0] = glo[i0]; head[kGLo + i1] = glo[i1];
+            if (lane == 31) head[kGamma] = e1;
+            const float u = fmaxf(u0, u1);
+            float um = u;
+#pragma unroll
+            for (int m = 16; m; m >>= 1) um = fmaxf(um, __shfl_xor_sync(0xffffffffu, um, m));
+            if (lane == 0) red[48] = um;
+        }
+        __syncthreads();
+        // A to shared memory, P kept in the fragments
+        float pr[4][4], mp = 0.f;
+        {
+            const int i0 = rb * 16 + (lane >> 2);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int i = i0 + 8 * (y >> 1), j = half * 32 + x * 8 + (lane & 3) * 2 + (y & 1);
+                    const float d = j <= i ? expf((ghi[i] - ghi[j]) + (glo[i] - glo[j])) : 0.f;
+                    A[i * PITCH + j] = j < i ? be[i] * d * (kk[x][y] * unk * unk) : 0.f;
+                    pr[x][y] = j <= i ? p.scale * d * (qk[x][y] * unk * unq) : 0.f;
+                    mp = fmaxf(mp, fabsf(pr[x][y]));
+                }
+        }
+        // Kt from the parts of K
+        const int et = part_exponent(red[48] * pow2_float(14 - ek));     // its largest magnitude is at most this
+        {
+            const float s = unk * pow2_float(et);
+#pragma unroll
+            for (int x = 0; x < PIECES; ++x) {
+                const int piece = tid + x * NT, row = piece / (KEY / 8), at = panel_at(row, piece % (KEY / 8) * 8);
+                const uint4 h4 = *reinterpret_cast<const uint4*>(kr + at), l4 = *reinterpret_cast<const uint4*>(kr + LO + at);
+                const __half2 *hp = reinterpret_cast<const __half2*>(&h4), *lp = reinterpret_cast<const __half2*>(&l4);
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 u = __half22float2(hp[i]), v = __half22float2(lp[i]);
+                    f[2 * i] = (u.x + v.x) * until[row];
+                    f[2 * i + 1] = (u.y + v.y) * until[row];
+                }
+                uint4 hi, lo;
+                split8(f, s, hi, lo);
+                *reinterpret_cast<uint4*>(rec + a.rec.kt() + at) = hi;
+                *reinterpret_cast<uint4*>(rec + a.rec.kt() + LO + at) = lo;
+            }
+        }
+        __syncthreads();
+        invert(A, tmp);
+        // T and T beta e^G: two 16-byte pieces of each per thread
+        float ft[2][8], mt = 0.f, ml = 0.f;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int piece = tid + x * NT, row = piece >> 3, col = (piece & 7) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(A + row * PITCH + col + i);
+                ft[x][i] = v.x; ft[x][i + 1] = v.y; ft[x][i + 2] = v.z; ft[x][i + 3] = v.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                mt = fmaxf(mt, fabsf(ft[x][i]));
+                ml = fmaxf(ml, fabsf(ft[x][i] * left[col + i]));
+            }
+        }
+        block_max3(mp, mt, ml, red);
+        const int ep = part_exponent(mp), ett = part_exponent(mt), el = part_exponent(ml);
+        store_fragments(rec + a.rec.p(), 8192, rb * 16, half * 32, pr, pow2_float(ep));
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int piece = tid + x * NT, row = piece >> 3, col = (piece & 7) * 8, at = panel_at(row, col);
+            uint4 hi, lo;
+            split8(ft[x], pow2_float(ett), hi, lo);
+            *reinterpret_cast<uint4*>(rec + a.rec.t() + at) = hi;
+            *reinterpret_cast<uint4*>(rec + a.rec.t() + 8192 + at) = lo;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ft[x][i] *= left[col + i];
+            split8(ft[x], pow2_float(el), hi, lo);
+            *reinterpret_cast<uint4*>(qr + at) = hi;
+            *reinterpret_cast<uint4*>(qr + 8192 + at) = lo;
+        }
+        __syncthreads();
+        // W = (T beta e^G) K: warp = 16 rows x half of the columns, steps up to the row block
+        constexpr int TILES = KEY / 16;                                    // 8-column tiles of a warp
+        float w[TILES][4] = {};
+        {
+            const int arow = rb * 16 + (lane & 15), acol = (lane >> 4) * 8;
+            const int brow = lane & 15, bcol = (lane >> 4) * 8;
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb) {
+                if (jb > rb) continue;
+                uint32_t th[4], tl[4];
+                const int at = panel_at(arow, jb * 16 + acol);
+                ldmatrix4(th, qs + at);
+                ldmatrix4(tl, qs + 8192 + at);
+#pragma unroll
+                for (int x = 0; x < TILES / 2; ++x) {
+                    uint32_t bh[4], bl[4];
+                    const int bt = panel_at(jb * 16 + brow, half * (KEY / 2) + x * 16 + bcol);
+                    ldmatrix4_trans(bh, ks + bt);
+                    ldmatrix4_trans(bl, ks + LO + bt);
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        mma16816(w[2 * x + y], tl, bh[2 * y], bh[2 * y + 1]);
+                        mma16816(w[2 * x + y], th, bl[2 * y], bl[2 * y + 1]);
+                        mma16816(w[2 * x + y], th, bh[2 * y], bh[2 * y + 1]);
+                    }
+                }
+            }
+        }
+        float mw = 0.f, none1 = 0.f, none2 = 0.f;
+        const float unw = pow2_float(-el) * unk;
+#pragma unroll
+        for (int x = 0; x < TILES; ++x)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                w[x][y] *= unw;
+                mw = fmaxf(mw, fabsf(w[x][y]));
+            }
+        block_max3(mw, none1, none2, red + 24);
+        const int ew = part_exponent(mw);
+#pragma unroll
+        for (int x = 0; x < TILES / 4; ++x) {
+            float f[4][4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int z = 0; z < 4; ++z) f[y][z] = w[4 * x + y][z];
+            store_fragments(rec + a.rec.w(), LO, rb * 16, half * (KEY / 2) + x * 32, f, pow2_float(ew));
+        }
+        if (tid == 0) {
+            head[kUnW] = pow2_float(-ew);
+            head[kUnKt] = pow2_float(-et);
+            head[kUnQ] = unq;
+            head[kUnT] = pow2_float(-ett);
+            head[kUnP] = pow2_float(-ep);
+        }
+    }
+}
+
+template <typename T, int KEY>
+cudaError_t prepare(const PrepareParams& a, cudaStream_t st) {
+    constexpr int smem = PrepareSmem<KEY>::kBytes;
+    cudaError_t e = cudaFuncSetAttribute(delta_prepare_kernel<T, KEY>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    delta_prepare_kernel<T, KEY><<<(unsigned)(a.p.B * a.p.HK * a.n), NT, smem, st>>>(a);
+    count_launch();
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t prepare_typed(PrepareParams& a, cudaStream_t st) {
+    auto vec = [&](const void* base, const long long* s) {
+        return reinterpret_cast<uintptr_t>(base) % 16 == 0 && s[0] * sizeof(T) % 16 == 0 && s[1] * sizeof(T) % 16 == 0 &&
+               s[2] * sizeof(T) % 16 == 0 && a.p.DK % 8 == 0;
+    };
+    a.vec_q = vec(a.in.q, a.p.q_stride);
+    a.vec_k = vec(a.in.k, a.p.k_stride);
+    return a.rec.key == 64 ? prepare<T, 64>(a, st) : prepare<T, 128>(a, st);
+}
+
+}  // namespace
+
+cudaError_t launch_delta_prepare(const aussm_b200_delta_t& p, const DeltaPlan& plan, const DeltaInputs& in, void* records,
+                                 cudaStream_t st) {
+    PrepareParams a = {p, in, static_cast<uint8_t*>(records), plan.rec, plan.n, 0, 0};
+    return p.dtype == AUSSM_FLOAT32 ? prepare_typed<float>(a, st)
+           : p.dtype == AUSSM_BFLOAT16 ? prepare_typed<__nv_bfloat16>(a, st) : prepare_typed<__half>(a, st);
+}
+
+}  // namespace aussm
