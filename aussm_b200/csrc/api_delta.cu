@@ -65,7 +65,7 @@ size_t aussm_b200_delta_keep_bytes(const aussm_b200_delta_t* p) {
 
 size_t aussm_b200_delta_workspace_bytes(const aussm_b200_delta_t* p, int backward) {
     if (delta_check("delta_workspace_bytes", p)) return 0;
-    return backward ? delta_plan(*p).bwd_bytes : delta_plan(*p).keep_bytes;
+    return backward ? delta_plan(*p).bwd_bytes : delta_plan(*p).news;     // without a backward pass only the records
 }
 
 int aussm_b200_delta_fwd(const aussm_b200_delta_t* p, const void* q, const void* k, const void* v, const float* g,
@@ -76,13 +76,14 @@ int aussm_b200_delta_fwd(const aussm_b200_delta_t* p, const void* q, const void*
         set_error("delta_fwd: null input or output pointer");
         return AUSSM_EINVAL;
     }
-    if (keep) {
+    const bool train = keep != nullptr;
+    if (train) {
         if (int rc = need("delta_fwd", "keep buffer", keep, keep_bytes, delta_plan(*p).keep_bytes)) return rc;
     } else {
         if (int rc = need("delta_fwd", "workspace", workspace, workspace_bytes, aussm_b200_delta_workspace_bytes(p, 0))) return rc;
         keep = workspace;
     }
-    return launched("delta_fwd", launch_delta_fwd(*p, {q, k, v, g, beta}, s0, o, s1, keep, (cudaStream_t)stream));
+    return launched("delta_fwd", launch_delta_fwd(*p, {q, k, v, g, beta}, s0, o, s1, keep, train, (cudaStream_t)stream));
 }
 
 int aussm_b200_delta_bwd(const aussm_b200_delta_t* p, const void* go, const float* gs1, const void* q, const void* k,

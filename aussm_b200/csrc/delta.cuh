@@ -40,14 +40,14 @@ struct DeltaRecord {
     __host__ __device__ int tile() const { return key * 256; }
     __host__ __device__ int w() const { return kHead; }                             // W = T beta e^G K
     __host__ __device__ int kt() const { return kHead + tile(); }                   // Kt = e^(G_C - G) K
-    __host__ __device__ int q() const { return kHead + 2 * tile(); }                // Q as it is
+    __host__ __device__ int q() const { return kHead + 2 * tile(); }                // Qt = scale e^G Q
     __host__ __device__ int t() const { return kHead + 3 * tile(); }                // T = (I + A)^-1
     __host__ __device__ int p() const { return kHead + 3 * tile() + kSquare; }      // P
     __host__ __device__ int bytes() const { return kHead + 3 * tile() + 2 * kSquare; }
 };
 // header, in floats: what a stored part is to be multiplied with (1 / S) ...
 enum : int { kUnW = 0, kUnKt = 1, kUnQ = 2, kUnT = 3, kUnP = 4, kGamma = 5 /* e^(G_C) */,
-             kSince = 16 /* scale e^(G_i), 64 */, kGHi = 80, kGLo = 144 /* G_i = hi + lo, 64 each */ };
+             kBeta = 16 /* 64 */, kGHi = 80, kGLo = 144 /* G_i = hi + lo, 64 each */ };
 
 // byte offset of element (row, col) in the hi panels of a tile
 __host__ __device__ __forceinline__ int panel_at(int row, int col) {
@@ -103,8 +103,19 @@ DeltaPlan delta_plan(const aussm_b200_delta_t& p);
 
 cudaError_t launch_delta_prepare(const aussm_b200_delta_t& p, const DeltaPlan& plan, const DeltaInputs& in, void* records,
                                  cudaStream_t stream);
+// the recurrence over chunks, forward or (V -> dO, O -> dV, V' -> X, states -> gradients) backward
+struct DeltaScan {
+    const void* records;
+    const void* v;
+    const float* s0;
+    float* s1;
+    void* out;
+    float *rows, *states;      // V' / X and entry states / gradients of exit states of every chunk; forward: NULL = not kept
+};
+cudaError_t launch_delta_scan(const aussm_b200_delta_t& p, const DeltaPlan& plan, const DeltaScan& io, bool backward,
+                              cudaStream_t stream);
 cudaError_t launch_delta_fwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const float* s0, void* o, float* s1,
-                             void* keep, cudaStream_t stream);
+                             void* keep, bool train, cudaStream_t stream);
 cudaError_t launch_delta_bwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const void* go, const float* gs1,
                              const void* keep, void* dq, void* dk, void* dv, float* dg, float* dbeta, float* ds0,
                              void* workspace, cudaStream_t stream);

@@ -83,46 +83,6 @@ __device__ void products(int M, int N, int K, F term, G store) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT) forward_kernel(const Params a) {
-    extern __shared__ float S[];     // (DK, SLICE)
-    const aussm_b200_delta_t& p = a.p;
-    const int bh = blockIdx.x, b = bh / p.HV, h = bh % p.HV, hk = h / (p.HV / p.HK);
-    const int v0 = blockIdx.y * SLICE, nv = min(SLICE, p.DV - v0);
-    for (int e = threadIdx.x; e < p.DK * nv; e += NT)
-        S[e / nv * SLICE + e % nv] = a.s0 ? a.s0[((size_t)bh * p.DK + e / nv) * p.DV + v0 + e % nv] : 0.f;
-    __syncthreads();
-    for (int c = 0; c < a.n; ++c) {
-        const int t0 = c * C, rows = min(C, p.L - t0);
-        const size_t at = (size_t)bh * a.n + c;
-        const Record r(a.records, a.rec, at);
-        float* N = a.N + at * C * p.DV + v0;
-        const Rows<T> q = rows_of<T>(a.in.q, p.q_stride, b, t0, hk, p.L), k = rows_of<T>(a.in.k, p.k_stride, b, t0, hk, p.L),
-                      v = rows_of<T>(a.in.v, p.v_stride, b, t0, h, p.L);
-        const float* be = a.in.beta + ((long long)b * p.L + t0) * p.HV + h;
-        for (int e = threadIdx.x; e < p.DK * nv; e += NT)
-            a.S[(at * p.DK + e / nv) * p.DV + v0 + e % nv] = S[e / nv * SLICE + e % nv];
-        products(C, nv, C + p.DK, [&](int i, int j, int m) {
-            if (m >= C) return -r.W(i, m - C) * S[(m - C) * SLICE + j];
-            return m <= i && m < rows ? r.T(i, m) * be[(long long)m * p.HV] * v(m, v0 + j) : 0.f;
-        }, [&](int i, int j, float x) { N[(size_t)i * p.DV + j] = x; });
-        __syncthreads();
-        products(rows, nv, C + p.DK, [&](int i, int j, int m) {
-            if (m >= C) return r.G.f[kSince + i] * r.Q(i, m - C) * S[(m - C) * SLICE + j];
-            return m <= i ? r.P(i, m) * N[(size_t)m * p.DV + j] : 0.f;
-        }, [&](int i, int j, float x) {
-            static_cast<T*>(a.o)[(((long long)b * p.L + t0 + i) * p.HV + h) * p.DV + v0 + j] = from_f32<T>(x);
-        });
-        __syncthreads();
-        products(p.DK, nv, C, [&](int x, int j, int i) { return r.Kt(i, x) * N[(size_t)i * p.DV + j]; },
-                 [&](int x, int j, float s) { S[x * SLICE + j] = r.G.f[kGamma] * S[x * SLICE + j] + s; });
-        __syncthreads();
-    }
-    if (a.s1)
-        for (int e = threadIdx.x; e < p.DK * nv; e += NT)
-            a.s1[((size_t)bh * p.DK + e / nv) * p.DV + v0 + e % nv] = S[e / nv * SLICE + e % nv];
-}
-
-template <typename T>
 __global__ void __launch_bounds__(NT) backward_kernel(const Params a) {
     extern __shared__ float dS[];    // (DK, SLICE)
     const aussm_b200_delta_t& p = a.p;
@@ -154,7 +114,7 @@ __global__ void __launch_bounds__(NT) backward_kernel(const Params a) {
                              from_f32<T>(be[(long long)i * p.HV] * x);
                  });
         products(p.DK, nv, C, [&](int x, int j, int i) {
-            return r.G.f[kSince + i] * r.Q(i, x) * go(i, v0 + j) - r.W(i, x) * dN[(size_t)i * p.DV + j];
+            return r.Q(i, x) * go(i, v0 + j) - r.W(i, x) * dN[(size_t)i * p.DV + j];
         }, [&](int x, int j, float s) { dS[x * SLICE + j] = r.G.f[kGamma] * dS[x * SLICE + j] + s; });
         __syncthreads();
     }
@@ -258,13 +218,6 @@ __global__ void __launch_bounds__(NT) gradients_kernel(const Params a) {
 }
 
 template <typename T>
-cudaError_t forward(const Params& a, cudaStream_t st) {
-    forward_kernel<T><<<dim3(a.p.B * a.p.HV, (a.p.DV + SLICE - 1) / SLICE), NT, a.p.DK * SLICE * 4, st>>>(a);
-    count_launch();
-    return cudaGetLastError();
-}
-
-template <typename T>
 cudaError_t backward(const Params& a, cudaStream_t st) {
     backward_kernel<T><<<dim3(a.p.B * a.p.HV, (a.p.DV + SLICE - 1) / SLICE), NT, a.p.DK * SLICE * 4, st>>>(a);
     const int smem = (3 * C * C + 2 * C * a.p.DK + 3 * C) * 4;
@@ -299,14 +252,13 @@ static Params params(const aussm_b200_delta_t& p, const DeltaPlan& plan, const D
 }
 
 cudaError_t launch_delta_fwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const float* s0, void* o, float* s1,
-                             void* keep, cudaStream_t st) {
+                             void* keep, bool train, cudaStream_t st) {
     const DeltaPlan plan = delta_plan(p);
     cudaError_t e = launch_delta_prepare(p, plan, in, keep, st);
     if (e != cudaSuccess) return e;
-    Params a = params(p, plan, in, keep);
-    a.s0 = s0; a.o = o; a.s1 = s1;
-    return p.dtype == AUSSM_FLOAT32 ? forward<float>(a, st) : p.dtype == AUSSM_BFLOAT16 ? forward<__nv_bfloat16>(a, st)
-                                                                                       : forward<__half>(a, st);
+    uint8_t* k = static_cast<uint8_t*>(keep);
+    float *news = train ? reinterpret_cast<float*>(k + plan.news) : nullptr, *states = train ? reinterpret_cast<float*>(k + plan.states) : nullptr;
+    return launch_delta_scan(p, plan, {keep, in.v, s0, s1, o, news, states}, false, st);
 }
 
 cudaError_t launch_delta_bwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const void* go, const float* gs1,

@@ -63,6 +63,18 @@ __device__ __forceinline__ void load8(const T* row, int c, int cols, bool vec, f
     }
 }
 
+// what eight stored hi and lo parts stand for, times f
+__device__ __forceinline__ void join8(const uint8_t* hi, const uint8_t* lo, float f, float (&v)[8]) {
+    const uint4 h4 = *reinterpret_cast<const uint4*>(hi), l4 = *reinterpret_cast<const uint4*>(lo);
+    const __half2 *hp = reinterpret_cast<const __half2*>(&h4), *lp = reinterpret_cast<const __half2*>(&l4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = __half22float2(hp[i]), b = __half22float2(lp[i]);
+        v[2 * i] = (a.x + b.x) * f;
+        v[2 * i + 1] = (a.y + b.y) * f;
+    }
+}
+
 __device__ __forceinline__ void split8(const float (&f)[8], float s, uint4& hi, uint4& lo) {
     split2(f[0] * s, f[1] * s, hi.x, lo.x);
     split2(f[2] * s, f[3] * s, hi.y, lo.y);
@@ -188,8 +200,7 @@ __device__ __forceinline__ void invert(float* A, float* tmp) {
 template <int KEY>
 struct PrepareSmem {
     static constexpr int kTile = KEY * 256;
-    static constexpr int kQ = kTile > DeltaRecord::kSquare ? kTile : DeltaRecord::kSquare;    // Q, then T beta e^G
-    static constexpr int kBytes = kTile + kQ + C * PITCH * 4 + 64 * 34 * 4 + 5 * C * 4 + 64 * 4;
+    static constexpr int kBytes = 2 * kTile + DeltaRecord::kSquare + C * PITCH * 4 + 64 * 34 * 4 + 6 * C * 4 + 64 * 4;
 };
 
 template <typename T, int KEY>
@@ -197,8 +208,9 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
     using Smem = PrepareSmem<KEY>;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t *kr = sm, *qr = sm + Smem::kTile;
-    float* A = reinterpret_cast<float*>(qr + Smem::kQ);
-    float *tmp = A + C * PITCH, *ghi = tmp + 64 * 34, *glo = ghi + C, *be = glo + C, *until = be + C, *left = until + C, *red = left + C;
+    uint8_t* tr = qr + Smem::kTile;                                   // T beta e^G
+    float* A = reinterpret_cast<float*>(tr + DeltaRecord::kSquare);
+    float *tmp = A + C * PITCH, *ghi = tmp + 64 * 34, *glo = ghi + C, *be = glo + C, *until = be + C, *left = until + C, *since = left + C, *red = since + C;
     constexpr int LO = KEY * 128;                                     // lo panels behind the hi panels
     const aussm_b200_delta_t& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -242,18 +254,13 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             split8(fq[x], sq, hi, lo);
             *reinterpret_cast<uint4*>(qr + at) = hi;
             *reinterpret_cast<uint4*>(qr + LO + at) = lo;
-            for (int h = hk * r; h < hk * r + r; ++h) {
-                uint8_t* dst = record(h) + a.rec.q() + at;
-                *reinterpret_cast<uint4*>(dst) = hi;
-                *reinterpret_cast<uint4*>(dst + LO) = lo;
-            }
         }
     }
     __syncthreads();
 
     // K K^T and Q K^T on and below the diagonal blocks: warp = rows rb*16.., columns half*32..
     const int rb = warp & 3, half = warp >> 2;
-    const uint32_t ks = smem_addr(kr), qs = smem_addr(qr);
+    const uint32_t ks = smem_addr(kr), qs = smem_addr(qr), ts = smem_addr(tr);
     float kk[4][4] = {}, qk[4][4] = {};
     {
         const int arow = rb * 16 + (lane & 15), acol = (lane >> 4) * 8;
@@ -313,15 +320,18 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             until[i0] = u0; until[i1] = u1;
             const float e0 = expf((float)before), e1 = expf((float)s);
             left[i0] = be[i0] * e0; left[i1] = be[i1] * e1;                 // what T's columns are multiplied with for W
-            head[kSince + i0] = p.scale * e0; head[kSince + i1] = p.scale * e1;
+            since[i0] = p.scale * e0; since[i1] = p.scale * e1;
+            head[kBeta + i0] = be[i0]; head[kBeta + i1] = be[i1];
             head[kGHi + i0] = h0; head[kGHi + i1] = h1;
             head[kGLo + i0] = glo[i0]; head[kGLo + i1] = glo[i1];
             if (lane == 31) head[kGamma] = e1;
-            const float u = fmaxf(u0, u1);
-            float um = u;
+            float um = fmaxf(u0, u1), em = fabsf(p.scale) * fmaxf(e0, e1);
 #pragma unroll
-            for (int m = 16; m; m >>= 1) um = fmaxf(um, __shfl_xor_sync(0xffffffffu, um, m));
-            if (lane == 0) red[48] = um;
+            for (int m = 16; m; m >>= 1) {
+                um = fmaxf(um, __shfl_xor_sync(0xffffffffu, um, m));
+                em = fmaxf(em, __shfl_xor_sync(0xffffffffu, em, m));
+            }
+            if (lane == 0) { red[48] = um; red[49] = em; }
         }
         __syncthreads();
         // A to shared memory, P kept in the fragments
@@ -339,26 +349,23 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                     mp = fmaxf(mp, fabsf(pr[x][y]));
                 }
         }
-        // Kt from the parts of K
-        const int et = part_exponent(red[48] * pow2_float(14 - ek));     // its largest magnitude is at most this
+        // Kt and Qt from the parts of K and Q; their largest magnitudes are at most these
+        const int et = part_exponent(red[48] * pow2_float(14 - ek)), eqt = part_exponent(red[49] * pow2_float(14 - eq));
         {
-            const float s = unk * pow2_float(et);
+            const float s = unk * pow2_float(et), sq = unq * pow2_float(eqt);
 #pragma unroll
             for (int x = 0; x < PIECES; ++x) {
                 const int piece = tid + x * NT, row = piece / (KEY / 8), at = panel_at(row, piece % (KEY / 8) * 8);
-                const uint4 h4 = *reinterpret_cast<const uint4*>(kr + at), l4 = *reinterpret_cast<const uint4*>(kr + LO + at);
-                const __half2 *hp = reinterpret_cast<const __half2*>(&h4), *lp = reinterpret_cast<const __half2*>(&l4);
                 float f[8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 u = __half22float2(hp[i]), v = __half22float2(lp[i]);
-                    f[2 * i] = (u.x + v.x) * until[row];
-                    f[2 * i + 1] = (u.y + v.y) * until[row];
-                }
                 uint4 hi, lo;
+                join8(kr + at, kr + LO + at, until[row], f);
                 split8(f, s, hi, lo);
                 *reinterpret_cast<uint4*>(rec + a.rec.kt() + at) = hi;
                 *reinterpret_cast<uint4*>(rec + a.rec.kt() + LO + at) = lo;
+                join8(qr + at, qr + LO + at, since[row], f);
+                split8(f, sq, hi, lo);
+                *reinterpret_cast<uint4*>(rec + a.rec.q() + at) = hi;
+                *reinterpret_cast<uint4*>(rec + a.rec.q() + LO + at) = lo;
             }
         }
         __syncthreads();
@@ -392,8 +399,8 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
 #pragma unroll
             for (int i = 0; i < 8; ++i) ft[x][i] *= left[col + i];
             split8(ft[x], pow2_float(el), hi, lo);
-            *reinterpret_cast<uint4*>(qr + at) = hi;
-            *reinterpret_cast<uint4*>(qr + 8192 + at) = lo;
+            *reinterpret_cast<uint4*>(tr + at) = hi;
+            *reinterpret_cast<uint4*>(tr + 8192 + at) = lo;
         }
         __syncthreads();
         // W = (T beta e^G) K: warp = 16 rows x half of the columns, steps up to the row block
@@ -407,8 +414,8 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 if (jb > rb) continue;
                 uint32_t th[4], tl[4];
                 const int at = panel_at(arow, jb * 16 + acol);
-                ldmatrix4(th, qs + at);
-                ldmatrix4(tl, qs + 8192 + at);
+                ldmatrix4(th, ts + at);
+                ldmatrix4(tl, ts + 8192 + at);
 #pragma unroll
                 for (int x = 0; x < TILES / 2; ++x) {
                     uint32_t bh[4], bl[4];
@@ -447,7 +454,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
         if (tid == 0) {
             head[kUnW] = pow2_float(-ew);
             head[kUnKt] = pow2_float(-et);
-            head[kUnQ] = unq;
+            head[kUnQ] = pow2_float(-eqt);
             head[kUnT] = pow2_float(-ett);
             head[kUnP] = pow2_float(-ep);
         }
