@@ -98,6 +98,7 @@ struct DeltaPlan {
     DeltaRecord rec;
     size_t keep_bytes, bwd_bytes;
     size_t news, states;   // byte offsets in keep
+    size_t dstates;        // byte offset in the backward workspace: [X (chunk heads, 64, DV)][gradients of exit states]
 };
 DeltaPlan delta_plan(const aussm_b200_delta_t& p);
 
@@ -114,6 +115,14 @@ struct DeltaScan {
 };
 cudaError_t launch_delta_scan(const aussm_b200_delta_t& p, const DeltaPlan& plan, const DeltaScan& io, bool backward,
                               cudaStream_t stream);
+struct DeltaGrads {
+    const void *records, *go;
+    const float *news, *x, *states, *dstates;
+    void *dq, *dk;
+    float *dg, *dbeta;
+};
+cudaError_t launch_delta_grads(const aussm_b200_delta_t& p, const DeltaPlan& plan, const DeltaInputs& in, const DeltaGrads& io,
+                               cudaStream_t stream);
 cudaError_t launch_delta_fwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const float* s0, void* o, float* s1,
                              void* keep, bool train, cudaStream_t stream);
 cudaError_t launch_delta_bwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const void* go, const float* gs1,

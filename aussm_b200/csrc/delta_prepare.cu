@@ -5,8 +5,7 @@
 // FP16 parts with mma.sync (two blocks an SM, 8 warps each, warp = 16 rows x half of the columns), skipping the 16 x 16
 // blocks above the diagonal.  Differences of the sums of g are taken from pairs of floats: sums reach thousands, and
 // e^(G_i - G_j) has to be right to 24 bits where G_i - G_j is small.
-#include "common.cuh"
-#include "delta.cuh"
+#include "delta_tiles.cuh"
 #include "host_common.cuh"
 
 namespace aussm {
@@ -24,83 +23,6 @@ struct PrepareParams {
     int n;
     int vec_q, vec_k;                    // rows can be read 16 bytes at a time
 };
-
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// eight consecutive elements of a row, zeros from `cols` on
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int c, int cols, bool vec, float (&f)[8]) {
-    if (vec) {
-        if (c < cols) {
-            constexpr int N = 16 / sizeof(T);
-            struct alignas(16) Raw { T v[N]; };
-#pragma unroll
-            for (int k = 0; k < 8 / N; ++k) {
-                const Raw r = *reinterpret_cast<const Raw*>(row + c + k * N);
-#pragma unroll
-                for (int i = 0; i < N; ++i) f[k * N + i] = to_f32(r.v[i]);
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = 0.f;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = c + i < cols ? to_f32(row[c + i]) : 0.f;
-    }
-}
-
-// what eight stored hi and lo parts stand for, times f
-__device__ __forceinline__ void join8(const uint8_t* hi, const uint8_t* lo, float f, float (&v)[8]) {
-    const uint4 h4 = *reinterpret_cast<const uint4*>(hi), l4 = *reinterpret_cast<const uint4*>(lo);
-    const __half2 *hp = reinterpret_cast<const __half2*>(&h4), *lp = reinterpret_cast<const __half2*>(&l4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 a = __half22float2(hp[i]), b = __half22float2(lp[i]);
-        v[2 * i] = (a.x + b.x) * f;
-        v[2 * i + 1] = (a.y + b.y) * f;
-    }
-}
-
-__device__ __forceinline__ void split8(const float (&f)[8], float s, uint4& hi, uint4& lo) {
-    split2(f[0] * s, f[1] * s, hi.x, lo.x);
-    split2(f[2] * s, f[3] * s, hi.y, lo.y);
-    split2(f[4] * s, f[5] * s, hi.z, lo.z);
-    split2(f[6] * s, f[7] * s, hi.w, lo.w);
-}
-
-// maxima of three values over the block; `buf` has 3 * 8 floats and is free again after the next barrier
-__device__ __forceinline__ void block_max3(float& a, float& b, float& c, float* buf) {
-#pragma unroll
-    for (int m = 16; m; m >>= 1) {
-        a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, m));
-        b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, m));
-        c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, m));
-    }
-    const int w = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) { buf[w] = a; buf[8 + w] = b; buf[16 + w] = c; }
-    __syncthreads();
-    a = b = c = 0.f;
-#pragma unroll
-    for (int i = 0; i < NT / 32; ++i) {
-        a = fmaxf(a, buf[i]);
-        b = fmaxf(b, buf[8 + i]);
-        c = fmaxf(c, buf[16 + i]);
-    }
-}
 
 // 4 x 4 words of a quad of lanes change places: lane t comes to hold word t of lanes 0..3
 __device__ __forceinline__ void quad_transpose(uint32_t (&w)[4], int t) {
@@ -224,7 +146,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
     constexpr int PIECES = C * KEY / 8 / NT;
     int ek, eq;
     {
-        float fk[PIECES][8], fq[PIECES][8], mk = 0.f, mq = 0.f, none = 0.f;
+        float fk[PIECES][8], fq[PIECES][8], m[2] = {};
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
             const int piece = tid + x * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8;
@@ -232,28 +154,21 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 load8(k + row * p.k_stride[1], col, p.DK, a.vec_k, fk[x]);
                 load8(q + row * p.q_stride[1], col, p.DK, a.vec_q, fq[x]);
             } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) fk[x][i] = fq[x][i] = 0.f;
+                zero8(fk[x]);
+                zero8(fq[x]);
             }
         }
 #pragma unroll
-        for (int x = 0; x < PIECES; ++x)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { mk = fmaxf(mk, fabsf(fk[x][i])); mq = fmaxf(mq, fabsf(fq[x][i])); }
-        block_max3(mk, mq, none, red);
-        ek = part_exponent(mk);
-        eq = part_exponent(mq);
+        for (int x = 0; x < PIECES; ++x) { m[0] = max8(fk[x], m[0]); m[1] = max8(fq[x], m[1]); }
+        block_max<8>(m, red);
+        ek = part_exponent(m[0]);
+        eq = part_exponent(m[1]);
         const float sk = pow2_float(ek), sq = pow2_float(eq);
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
             const int piece = tid + x * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8, at = panel_at(row, col);
-            uint4 hi, lo;
-            split8(fk[x], sk, hi, lo);
-            *reinterpret_cast<uint4*>(kr + at) = hi;
-            *reinterpret_cast<uint4*>(kr + LO + at) = lo;
-            split8(fq[x], sq, hi, lo);
-            *reinterpret_cast<uint4*>(qr + at) = hi;
-            *reinterpret_cast<uint4*>(qr + LO + at) = lo;
+            put8(kr + at, LO, fk[x], sk);
+            put8(qr + at, LO, fq[x], sq);
         }
     }
     __syncthreads();
@@ -263,12 +178,10 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
     const uint32_t ks = smem_addr(kr), qs = smem_addr(qr), ts = smem_addr(tr);
     float kk[4][4] = {}, qk[4][4] = {};
     {
-        const int arow = rb * 16 + (lane & 15), acol = (lane >> 4) * 8;
-        const int brow = (lane & 7) + ((lane >> 4) << 3), bcol = ((lane >> 3) & 1) * 8;
 #pragma unroll
         for (int k0 = 0; k0 < KEY; k0 += 16) {
             uint32_t kh[4], kl[4], qh[4], ql[4];
-            const int at = panel_at(arow, k0 + acol);
+            const int at = frag_a(rb * 16, k0);
             ldmatrix4(kh, ks + at);
             ldmatrix4(kl, ks + LO + at);
             ldmatrix4(qh, qs + at);
@@ -278,7 +191,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 const int n0 = half * 32 + x * 16;
                 if (n0 > rb * 16) continue;
                 uint32_t bh[4], bl[4];
-                const int bt = panel_at(n0 + brow, k0 + bcol);
+                const int bt = frag_b(n0, k0);
                 ldmatrix4(bh, ks + bt);
                 ldmatrix4(bl, ks + LO + bt);
 #pragma unroll
@@ -335,7 +248,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
         }
         __syncthreads();
         // A to shared memory, P kept in the fragments
-        float pr[4][4], mp = 0.f;
+        float pr[4][4], m[3] = {};
         {
             const int i0 = rb * 16 + (lane >> 2);
 #pragma unroll
@@ -346,7 +259,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                     const float d = j <= i ? expf((ghi[i] - ghi[j]) + (glo[i] - glo[j])) : 0.f;
                     A[i * PITCH + j] = j < i ? be[i] * d * (kk[x][y] * unk * unk) : 0.f;
                     pr[x][y] = j <= i ? p.scale * d * (qk[x][y] * unk * unq) : 0.f;
-                    mp = fmaxf(mp, fabsf(pr[x][y]));
+                    m[0] = fmaxf(m[0], fabsf(pr[x][y]));
                 }
         }
         // Kt and Qt from the parts of K and Q; their largest magnitudes are at most these
@@ -357,21 +270,16 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             for (int x = 0; x < PIECES; ++x) {
                 const int piece = tid + x * NT, row = piece / (KEY / 8), at = panel_at(row, piece % (KEY / 8) * 8);
                 float f[8];
-                uint4 hi, lo;
                 join8(kr + at, kr + LO + at, until[row], f);
-                split8(f, s, hi, lo);
-                *reinterpret_cast<uint4*>(rec + a.rec.kt() + at) = hi;
-                *reinterpret_cast<uint4*>(rec + a.rec.kt() + LO + at) = lo;
+                put8(rec + a.rec.kt() + at, LO, f, s);
                 join8(qr + at, qr + LO + at, since[row], f);
-                split8(f, sq, hi, lo);
-                *reinterpret_cast<uint4*>(rec + a.rec.q() + at) = hi;
-                *reinterpret_cast<uint4*>(rec + a.rec.q() + LO + at) = lo;
+                put8(rec + a.rec.q() + at, LO, f, sq);
             }
         }
         __syncthreads();
         invert(A, tmp);
         // T and T beta e^G: two 16-byte pieces of each per thread
-        float ft[2][8], mt = 0.f, ml = 0.f;
+        float ft[2][8];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int piece = tid + x * NT, row = piece >> 3, col = (piece & 7) * 8;
@@ -382,44 +290,37 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                mt = fmaxf(mt, fabsf(ft[x][i]));
-                ml = fmaxf(ml, fabsf(ft[x][i] * left[col + i]));
+                m[1] = fmaxf(m[1], fabsf(ft[x][i]));
+                m[2] = fmaxf(m[2], fabsf(ft[x][i] * left[col + i]));
             }
         }
-        block_max3(mp, mt, ml, red);
-        const int ep = part_exponent(mp), ett = part_exponent(mt), el = part_exponent(ml);
+        block_max<8>(m, red);
+        const int ep = part_exponent(m[0]), ett = part_exponent(m[1]), el = part_exponent(m[2]);
         store_fragments(rec + a.rec.p(), 8192, rb * 16, half * 32, pr, pow2_float(ep));
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int piece = tid + x * NT, row = piece >> 3, col = (piece & 7) * 8, at = panel_at(row, col);
-            uint4 hi, lo;
-            split8(ft[x], pow2_float(ett), hi, lo);
-            *reinterpret_cast<uint4*>(rec + a.rec.t() + at) = hi;
-            *reinterpret_cast<uint4*>(rec + a.rec.t() + 8192 + at) = lo;
+            put8(rec + a.rec.t() + at, 8192, ft[x], pow2_float(ett));
 #pragma unroll
             for (int i = 0; i < 8; ++i) ft[x][i] *= left[col + i];
-            split8(ft[x], pow2_float(el), hi, lo);
-            *reinterpret_cast<uint4*>(tr + at) = hi;
-            *reinterpret_cast<uint4*>(tr + 8192 + at) = lo;
+            put8(tr + at, 8192, ft[x], pow2_float(el));
         }
         __syncthreads();
         // W = (T beta e^G) K: warp = 16 rows x half of the columns, steps up to the row block
         constexpr int TILES = KEY / 16;                                    // 8-column tiles of a warp
         float w[TILES][4] = {};
         {
-            const int arow = rb * 16 + (lane & 15), acol = (lane >> 4) * 8;
-            const int brow = lane & 15, bcol = (lane >> 4) * 8;
 #pragma unroll
             for (int jb = 0; jb < 4; ++jb) {
                 if (jb > rb) continue;
                 uint32_t th[4], tl[4];
-                const int at = panel_at(arow, jb * 16 + acol);
+                const int at = frag_a(rb * 16, jb * 16);
                 ldmatrix4(th, ts + at);
                 ldmatrix4(tl, ts + 8192 + at);
 #pragma unroll
                 for (int x = 0; x < TILES / 2; ++x) {
                     uint32_t bh[4], bl[4];
-                    const int bt = panel_at(jb * 16 + brow, half * (KEY / 2) + x * 16 + bcol);
+                    const int bt = frag_bt(jb * 16, half * (KEY / 2) + x * 16);
                     ldmatrix4_trans(bh, ks + bt);
                     ldmatrix4_trans(bl, ks + LO + bt);
 #pragma unroll
@@ -431,17 +332,17 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 }
             }
         }
-        float mw = 0.f, none1 = 0.f, none2 = 0.f;
+        float mw[1] = {};
         const float unw = pow2_float(-el) * unk;
 #pragma unroll
         for (int x = 0; x < TILES; ++x)
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
                 w[x][y] *= unw;
-                mw = fmaxf(mw, fabsf(w[x][y]));
+                mw[0] = fmaxf(mw[0], fabsf(w[x][y]));
             }
-        block_max3(mw, none1, none2, red + 24);
-        const int ew = part_exponent(mw);
+        block_max<8>(mw, red + 24);
+        const int ew = part_exponent(mw[0]);
 #pragma unroll
         for (int x = 0; x < TILES / 4; ++x) {
             float f[4][4];

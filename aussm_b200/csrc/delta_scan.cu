@@ -22,7 +22,7 @@ namespace {
 
 constexpr int C = kDeltaChunk;
 constexpr int THREADS = 384;             // three warpgroups; launched with 168 registers a thread, 504 for one of each
-constexpr int MAIN_REGS = 240, SIDE_REGS = 216, REST_REGS = 40;
+constexpr int MAIN_REGS = 240, SIDE_REGS = 208, REST_REGS = 56;
 static_assert(MAIN_REGS + SIDE_REGS + REST_REGS <= 3 * 168, "more registers than the block is launched with");
 constexpr int SQUARE = DeltaRecord::kSquare;
 // tensor memory columns
