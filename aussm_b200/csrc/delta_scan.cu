@@ -8,11 +8,15 @@
 // product is converted by the thread that owns the row and goes back as the next product's A without leaving the lane.
 // A row's FP16 parts are scaled by a power of two of the row's own: no reduction between threads.
 //
-// Warps 0-3 own the state (the chain: convert S, product, convert V', product, add), warps 4-7 bring V (dO) in and
-// O (X) out, warp 8 copies the records' tiles (bulk copies), warp 9 issues the MMAs
+// Warps 0-3 own the state (the chain: convert S, product, convert V', product, add), warps 4-7 bring V (dO) in (a chunk
+// ahead, through shared memory) and everything out (O or X; the states and V' that a backward pass wants, rebuilt from
+// the parts in tensor memory), warp 8 copies the records' tiles (bulk copies), warp 9 issues the MMAs
 // (10 and 11 fill their warpgroup, which hands its registers to the other two).  Tensor memory, 512 columns:
 // [X | Y] take turns as the parts of S and as the product that updates it, two accumulators of 64 columns, the parts of
 // V' and of V.  Every wait is bounded: one that runs out sets the status word and the block ends.
+//
+// The three roles walk different code, chunk after chunk, out of one instruction cache: with every loop unrolled the issue
+// of 36 MMAs took 4700 cycles instead of 1700.  Only what must be (registers that are indexed) is unrolled.
 #include "common.cuh"
 #include "delta.cuh"
 #include "host_common.cuh"
@@ -22,7 +26,7 @@ namespace {
 
 constexpr int C = kDeltaChunk;
 constexpr int THREADS = 384;             // three warpgroups; launched with 168 registers a thread, 504 for one of each
-constexpr int MAIN_REGS = 240, SIDE_REGS = 208, REST_REGS = 56;
+constexpr int MAIN_REGS = 240, SIDE_REGS = 168, REST_REGS = 96;
 static_assert(MAIN_REGS + SIDE_REGS + REST_REGS <= 3 * 168, "more registers than the block is launched with");
 constexpr int SQUARE = DeltaRecord::kSquare;
 // tensor memory columns
@@ -40,6 +44,7 @@ struct ScanParams {
     void* out;                           // forward: O; backward: dV
     float* rows;                         // forward: V' of every chunk (NULL = not kept); backward: X
     float* states;                       // forward: entry states (NULL); backward: gradients of the exit states
+    int vec_v;                           // rows of v can be copied 16 bytes at a time
     int* status;
 };
 
@@ -80,6 +85,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
                  "%15, %16};" ::"r"(t), W4(r, 0), W4(r, 4), W4(r, 8), W4(r, 12) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t t, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+                 "[%16];" : R4(r, 0), R4(r, 4), R4(r, 8), R4(r, 12) : "r"(t) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(t), W4(r, 0), W4(r, 4) : "memory");
+}
 #undef R4
 #undef W4
 
@@ -98,39 +111,50 @@ template <int N, int STEPS, bool MN>
 __device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, int b_lo) {
     constexpr uint32_t id = idesc(N, MN);
     constexpr uint32_t A_LO = STEPS * 8;
-#pragma unroll
+    const uint64_t first = row_desc(b, MN ? 8192 : 16);
+    const uint32_t lo = (uint32_t)b_lo >> 4;
+#pragma unroll 1
     for (int k = 0; k < STEPS; ++k) {
-        const uint32_t at = MN ? b + k * 2048 : b + (k >> 2) * 8192 + (k & 3) * 32;
-        const uint64_t bh = row_desc(at, MN ? 8192 : 16), bl = row_desc(at + b_lo, MN ? 8192 : 16);
+        const uint64_t bh = first + (uint32_t)((MN ? k * 2048 : (k >> 2) * 8192 + (k & 3) * 32) >> 4), bl = bh + lo;
         mma_ts(d, a + A_LO + k * 8, bh, id, k > 0);
         mma_ts(d, a + k * 8, bl, id, 1);
         mma_ts(d, a + k * 8, bh, id, 1);
     }
 }
 
-// COUNT values of this thread's row, scaled by s, as hi parts (COUNT / 2 columns) and lo parts behind them
+// COUNT values of this thread's row, scaled by f, as hi parts (COUNT / 2 columns) and lo parts behind them
 template <int COUNT>
-__device__ __forceinline__ void store_parts(uint32_t t, const float (&x)[COUNT], float s) {
+__device__ __forceinline__ void store_parts(uint32_t t, const float2 (&x)[COUNT / 2], float f) {
+    const float2 f2 = make_float2(f, f), minus = make_float2(-1.f, -1.f);
 #pragma unroll
-    for (int i = 0; i < COUNT; i += 32) {
+    for (int i = 0; i < COUNT / 2; i += 16) {
         uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) split2(x[i + 2 * j] * s, x[i + 2 * j + 1] * s, hi[j], lo[j]);
-        tmem_st16(t + i / 2, hi);
-        tmem_st16(t + COUNT / 2 + i / 2, lo);
+        for (int j = 0; j < 16; ++j) {
+            const float2 v = __fmul2_rn(x[i + j], f2);
+            const __half2 h = __float22half2_rn(v);
+            const __half2 l = __float22half2_rn(__ffma2_rn(__half22float2(h), minus, v));
+            hi[j] = *reinterpret_cast<const uint32_t*>(&h);
+            lo[j] = *reinterpret_cast<const uint32_t*>(&l);
+        }
+        tmem_st16(t + i, hi);
+        tmem_st16(t + COUNT / 2 + i, lo);
     }
 }
 template <int COUNT>
-__device__ __forceinline__ int row_exponent(const float (&x)[COUNT]) {
-    float m0 = 0.f, m1 = 0.f, m2 = 0.f, m3 = 0.f;
+__device__ __forceinline__ int row_exponent(const float2 (&x)[COUNT]) {
+    float m0 = 0.f, m1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < COUNT; i += 4) {
-        m0 = fmaxf(m0, fabsf(x[i]));
-        m1 = fmaxf(m1, fabsf(x[i + 1]));
-        m2 = fmaxf(m2, fabsf(x[i + 2]));
-        m3 = fmaxf(m3, fabsf(x[i + 3]));
+    for (int i = 0; i < COUNT; ++i) {
+        m0 = fmaxf(m0, fabsf(x[i].x));
+        m1 = fmaxf(m1, fabsf(x[i].y));
     }
-    return part_exponent(fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)));
+    return part_exponent(fmaxf(m0, m1));
+}
+// two values from a word of hi parts and one of lo parts
+__device__ __forceinline__ float2 join2(uint32_t hi, uint32_t lo, float f) {
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi)), l = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+    return make_float2((h.x + l.x) * f, (h.y + l.y) * f);
 }
 
 // the same answer in all lanes: what follows is executed by whole warps
@@ -138,20 +162,21 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* s
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, status));
 }
 
-template <int KEY>
+template <typename T, int KEY>
 struct ScanSmem {
     static constexpr int kTile = KEY * 256;
-    // phase 1 operands twice (tile, square), then the two tiles and the square of the later phases
-    static constexpr int kA = 0, kB = 2 * (kTile + SQUARE), kC = kB + kTile, kE = kC + kTile, kBytes = kE + SQUARE + 1024;
+    // phase 1 operands twice (tile, square), then the two tiles and the square of the later phases, then V (dO)
+    static constexpr int kA = 0, kB = 2 * (kTile + SQUARE), kC = kB + kTile, kE = kC + kTile, kV = kE + SQUARE,
+                         kBytes = kV + C * 128 * (int)sizeof(T) + 1024;
 };
 
 template <typename T, int KEY, bool BWD>
 __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams a) {
-    using Smem = ScanSmem<KEY>;
+    using Smem = ScanSmem<T, KEY>;
     constexpr int TILE = Smem::kTile, LO = KEY * 128, SQ_LO = 8192;
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full_a[2], full_b, full_c, full_e, empty_a[2], empty_b, empty_c, empty_e;
-    __shared__ uint64_t s_ready, v_ready, v_done, n_ready, a_done, y_free, d_done, o_done, o_free;
+    __shared__ uint64_t s_ready, v_ready, v_done, n_ready, a_done, y_free, d_done, o_done, o_free, x_free, v_loaded, v_read;
     __shared__ uint32_t holder;
     __shared__ float un_s[2][128], un_v[128], un_n[128];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -168,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         for (uint64_t* x : {&full_a[0], &full_a[1], &full_b, &full_c, &full_e, &empty_a[0], &empty_a[1], &empty_b, &empty_c,
                             &empty_e, &v_done, &a_done, &d_done, &o_done})
             mbar_init(x, 1);
-        for (uint64_t* x : {&s_ready, &v_ready, &n_ready, &y_free, &o_free}) mbar_init(x, 128);
+        for (uint64_t* x : {&s_ready, &v_ready, &n_ready, &y_free, &o_free, &x_free, &v_loaded, &v_read}) mbar_init(x, 128);
         fence_mbar_init();
         fence_proxy_async();
     }
@@ -181,123 +206,157 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     if (warp < 4) {
         // ---- the state -----------------------------------------------------------------------------------------
         more_registers<MAIN_REGS>();
-        float s[KEY];
+        float2 s[KEY / 2];
 #pragma unroll
-        for (int x = 0; x < KEY; ++x) s[x] = a.s0 && mine && x < p.DK ? a.s0[((size_t)bh * p.DK + x) * p.DV + v] : 0.f;
+        for (int x = 0; x < KEY / 2; ++x) {
+            const float* src = a.s0 + ((size_t)bh * p.DK + 2 * x) * p.DV + v;
+            s[x] = make_float2(a.s0 && mine && 2 * x < p.DK ? src[0] : 0.f, a.s0 && mine && 2 * x + 1 < p.DK ? src[p.DV] : 0.f);
+        }
+        // s = s * keep + r * f over all columns of a product
+        auto add = [&](uint32_t t, float keep, float f) {
+            const float2 k2 = make_float2(keep, keep), f2 = make_float2(f, f);
+#pragma unroll
+            for (int x = 0; x < KEY; x += 32) {
+                uint32_t r[32];
+                tmem_ld32(t + x, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int y = 0; y < 16; ++y)
+                    s[x / 2 + y] = __ffma2_rn(make_float2(__uint_as_float(r[2 * y]), __uint_as_float(r[2 * y + 1])), f2,
+                                              __fmul2_rn(s[x / 2 + y], k2));
+            }
+        };
         for (int i = 0; i < count; ++i) {
             const uint32_t ph = i & 1, X = lanes + (ph ? kY : kX), Y = lanes + (ph ? kX : kY);
             const float* head = reinterpret_cast<const float*>(record(i));
+            const float un1 = head[BWD ? kUnKt : kUnW], un2 = head[BWD ? kUnP : kUnT], un3 = head[BWD ? kUnW : kUnKt],
+                        unq = head[kUnQ], gamma = head[kGamma];
             const int es = row_exponent(s);
             const float uns = pow2_float(-es);
-            store_parts(X, s, pow2_float(es));
+            store_parts<KEY>(X, s, pow2_float(es));
             un_s[ph][threadIdx.x] = uns;
             tc_wait_st();
             tc_before();
             arrive(&s_ready);
-            const float un1 = head[BWD ? kUnKt : kUnW], un2 = head[BWD ? kUnP : kUnT], un3 = head[BWD ? kUnW : kUnKt],
-                        unq = head[kUnQ], gamma = head[kGamma];
-            if (a.states && mine) {
-                float* dst = a.states + ((size_t)bh * a.n + chunk_at(i)) * p.DK * p.DV + v;
-#pragma unroll
-                for (int x = 0; x < KEY; ++x)
-                    if (x < p.DK) dst[(size_t)x * p.DV] = s[x];
-            }
             // V' (dV')
             if (!warp_wait(&v_done, ph, a.status) || !warp_wait(&v_ready, ph, a.status)) break;
             tc_after();
-            const float f1 = (BWD ? uns : -uns) * un1, f2 = un_v[threadIdx.x] * un2;
-            float w[C];
+            const float unv = un_v[threadIdx.x], f1 = (BWD ? uns : -uns) * un1, f2 = unv * un2;
+            float2 w[C / 2];
 #pragma unroll
-            for (int x = 0; x < C; x += 32) {
-                uint32_t r1[32], r2[32];
-                tmem_ld32(lanes + kAcc + x, r1);
-                tmem_ld32(lanes + kAcc2 + x, r2);
+            for (int x = 0; x < C; x += 16) {
+                uint32_t r1[16], r2[16];
+                tmem_ld16(lanes + kAcc + x, r1);
+                tmem_ld16(lanes + kAcc2 + x, r2);
                 tc_wait_ld();
 #pragma unroll
-                for (int y = 0; y < 32; ++y) w[x + y] = fmaf(__uint_as_float(r1[y]), f1, __uint_as_float(r2[y]) * f2);
+                for (int y = 0; y < 8; ++y)
+                    w[x / 2 + y] = __ffma2_rn(make_float2(__uint_as_float(r1[2 * y]), __uint_as_float(r1[2 * y + 1])), make_float2(f1, f1),
+                                              __fmul2_rn(make_float2(__uint_as_float(r2[2 * y]), __uint_as_float(r2[2 * y + 1])), make_float2(f2, f2)));
             }
             const int en = row_exponent(w);
             const float unn = pow2_float(-en);
-            store_parts(lanes + kNew, w, pow2_float(en));
+            if (i && !warp_wait(&x_free, ph ^ 1, a.status)) break;      // the last V' has been taken out
+            store_parts<C>(lanes + kNew, w, pow2_float(en));
             un_n[threadIdx.x] = unn;
             tc_wait_st();
             tc_before();
             arrive(&n_ready);
-            if (!BWD && a.rows && mine) {
-                float* dst = a.rows + ((size_t)bh * a.n + chunk_at(i)) * C * p.DV + v;
-#pragma unroll
-                for (int x = 0; x < C; ++x) dst[(size_t)x * p.DV] = w[x];
-            }
             if (BWD) {
                 if (!warp_wait(&a_done, ph, a.status)) break;
                 tc_after();
-                const float f = un_v[threadIdx.x] * unq;
-#pragma unroll
-                for (int x = 0; x < KEY; x += 32) {
-                    uint32_t r[32];
-                    tmem_ld32(Y + x, r);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int y = 0; y < 32; ++y) s[x + y] = fmaf(gamma, s[x + y], __uint_as_float(r[y]) * f);
-                }
+                add(Y, gamma, unv * unq);
                 tc_before();
                 arrive(&y_free);
             }
             if (!warp_wait(&d_done, ph, a.status)) break;
             tc_after();
-            const float f = (BWD ? -unn : unn) * un3;
-#pragma unroll
-            for (int x = 0; x < KEY; x += 32) {
-                uint32_t r[32];
-                tmem_ld32(Y + x, r);
-                tc_wait_ld();
-#pragma unroll
-                for (int y = 0; y < 32; ++y) s[x + y] = fmaf(__uint_as_float(r[y]), f, BWD ? s[x + y] : gamma * s[x + y]);
-            }
+            add(Y, BWD ? 1.f : gamma, (BWD ? -unn : unn) * un3);
         }
         if (a.s1 && mine) {
 #pragma unroll
-            for (int x = 0; x < KEY; ++x)
-                if (x < p.DK) a.s1[((size_t)bh * p.DK + x) * p.DV + v] = s[x];
+            for (int x = 0; x < KEY / 2; ++x) {
+                float* dst = a.s1 + ((size_t)bh * p.DK + 2 * x) * p.DV + v;
+                if (2 * x < p.DK) dst[0] = s[x].x;
+                if (2 * x + 1 < p.DK) dst[p.DV] = s[x].y;
+            }
         }
     } else if (warp < 8) {
-        // ---- V (dO) in, O (X) out --------------------------------------------------------------------------------
+        // ---- V (dO) in; O (X), states and V' out -----------------------------------------------------------------
         more_registers<SIDE_REGS>();
         const int me = threadIdx.x & 127;
-        const T* src = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + v;
+        const T* src = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + blockIdx.y * 128;
         T* dst = static_cast<T*>(a.out) + ((long long)b * p.L * p.HV + h) * p.DV + v;
-        auto fetch = [&](int i, float (&x)[C]) {
+        T* tile = reinterpret_cast<T*>(sm + Smem::kV);
+        const int width = min(128, p.DV - (int)blockIdx.y * 128);
+        // rows of chunk i to shared memory, [64][128]: 16-byte pieces in flight, or each lane its own column
+        auto fetch = [&](int i) {
             const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
-#pragma unroll
-            for (int t = 0; t < C; ++t) x[t] = mine && t < rows ? to_f32(src[(long long)(t0 + t) * a.v_stride[1]]) : 0.f;
-        };
-        auto hand_over = [&](int i, float (&x)[C]) {
-            if (!BWD) {
-                const float4* be = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(record(i)) + kBeta);
-#pragma unroll
-                for (int t = 0; t < C / 4; ++t) {
-                    const float4 f = be[t];
-                    x[4 * t] *= f.x; x[4 * t + 1] *= f.y; x[4 * t + 2] *= f.z; x[4 * t + 3] *= f.w;
+            const T* from = src + (long long)t0 * a.v_stride[1];
+            if (a.vec_v) {
+                constexpr int E = 16 / (int)sizeof(T), PIECES = 128 / E;
+#pragma unroll 1
+                for (int x = me; x < C * PIECES; x += 128) {
+                    const int row = x / PIECES, col = x % PIECES * E;
+                    if (row < rows && col < width) cp_async16(tile + row * 128 + col, from + row * a.v_stride[1] + col);
                 }
+            } else if (mine) {
+#pragma unroll 8
+                for (int row = 0; row < rows; ++row) tile[row * 128 + me] = from[row * a.v_stride[1] + me];
             }
-            const int e = row_exponent(x);
-            store_parts(lanes + kVal, x, pow2_float(e));
+            cp_async_commit();
+        };
+        // chunk i's row of this lane from shared memory to the parts in tensor memory; false: a wait ran out
+        auto hand_over = [&](int i) {
+            const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
+            const float* be = reinterpret_cast<const float*>(record(i)) + kBeta;
+            cp_async_wait<0>();
+            arrive(&v_loaded);
+            if (!warp_wait(&v_loaded, i & 1, a.status)) return false;
+            float m = 0.f;
+#pragma unroll 1
+            for (int x = 0; x < C; x += 16)
+#pragma unroll
+                for (int y = 0; y < 16; ++y)
+                    if (x + y < rows) m = fmaxf(m, fabsf(to_f32(tile[(x + y) * 128 + me]) * (BWD ? 1.f : be[x + y])));
+            const int e = part_exponent(mine ? m : 0.f);
+            const float f = mine ? pow2_float(e) : 0.f;
+#pragma unroll 1
+            for (int x = 0; x < C; x += 16) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                    const int t = x + 2 * y;
+                    const float v0 = mine && t < rows ? to_f32(tile[t * 128 + me]) * (BWD ? f : be[t] * f) : 0.f;
+                    const float v1 = mine && t + 1 < rows ? to_f32(tile[(t + 1) * 128 + me]) * (BWD ? f : be[t + 1] * f) : 0.f;
+                    split2(v0, v1, hi[y], lo[y]);
+                }
+                tmem_st8(lanes + kVal + x / 2, hi);
+                tmem_st8(lanes + kVal + C / 2 + x / 2, lo);
+            }
             un_v[me] = pow2_float(-e);
             tc_wait_st();
             tc_before();
             arrive(&v_ready);
+            arrive(&v_read);
+            return true;
         };
-        float x[C];
-        fetch(0, x);
-        hand_over(0, x);
-        for (int i = 0; i < count; ++i) {
+        // the tile is free when all lanes have read chunk i from it
+        auto fetch_next = [&](int i) {
+            if (!warp_wait(&v_read, (i - 1) & 1, a.status)) return false;
+            fetch(i);
+            return true;
+        };
+        fetch(0);
+        bool ok = hand_over(0) && (count < 2 || fetch_next(1));
+        for (int i = 0; ok && i < count; ++i) {
             const uint32_t ph = i & 1;
             const float* head = reinterpret_cast<const float*>(record(i));
             const float unq = head[kUnQ], un2 = head[BWD ? kUnT : kUnP];
-            if (i + 1 < count) fetch(i + 1, x);
+            const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
             if (!warp_wait(&n_ready, ph, a.status) || !warp_wait(&o_done, ph, a.status)) break;
             tc_after();
-            const float f1 = un_s[ph][me] * unq, f2 = un_n[me] * un2;
+            const float f0 = un_s[ph][me], f1 = f0 * unq, unn = un_n[me], f2 = unn * un2;
             float y[C];
 #pragma unroll
             for (int t = 0; t < C; t += 32) {
@@ -311,21 +370,63 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             }
             tc_before();
             arrive(&o_free);
-            if (i + 1 < count) hand_over(i + 1, x);
+            if (i + 1 < count && !hand_over(i + 1)) break;
+            const size_t at = (size_t)bh * a.n + chunk_at(i);
+            if (a.states) {
+                const uint32_t X = lanes + (ph ? kY : kX);
+                float* to = a.states + at * p.DK * p.DV + v;
+#pragma unroll 1
+                for (int x = 0; x < KEY; x += 32) {
+                    uint32_t hi[16], lo[16];
+                    tmem_ld16(X + x / 2, hi);
+                    tmem_ld16(X + KEY / 2 + x / 2, lo);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int z = 0; z < 16; ++z) {
+                        const float2 w = join2(hi[z], lo[z], f0);
+                        if (mine && x + 2 * z < p.DK) to[0] = w.x;
+                        to += p.DV;
+                        if (mine && x + 2 * z + 1 < p.DK) to[0] = w.y;
+                        to += p.DV;
+                    }
+                }
+            }
+            if (!BWD && a.rows) {
+                float* to = a.rows + at * C * p.DV + v;
+#pragma unroll 1
+                for (int x = 0; x < C; x += 32) {
+                    uint32_t hi[16], lo[16];
+                    tmem_ld16(lanes + kNew + x / 2, hi);
+                    tmem_ld16(lanes + kNew + C / 2 + x / 2, lo);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int z = 0; z < 16; ++z) {
+                        const float2 w = join2(hi[z], lo[z], unn);
+                        if (mine) { to[0] = w.x; to[p.DV] = w.y; }
+                        to += 2 * p.DV;
+                    }
+                }
+            }
+            tc_before();
+            arrive(&x_free);
             if (mine) {
-                const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
                 if (BWD) {
-                    float* keep = a.rows + ((size_t)bh * a.n + chunk_at(i)) * C * p.DV + v;
+                    float* keep = a.rows + at * C * p.DV + v;
 #pragma unroll
                     for (int t = 0; t < C; ++t) {
-                        keep[(size_t)t * p.DV] = y[t];
+                        *keep = y[t];
+                        keep += p.DV;
                         y[t] *= head[kBeta + t];
                     }
                 }
+                T* to = dst + (long long)t0 * p.HV * p.DV;
 #pragma unroll
-                for (int t = 0; t < C; ++t)
-                    if (t < rows) dst[(long long)(t0 + t) * p.HV * p.DV] = from_f32<T>(y[t]);
+                for (int t = 0; t < C; ++t) {
+                    if (t < rows) *to = from_f32<T>(y[t]);
+                    to += (long long)p.HV * p.DV;
+                }
             }
+            if (i + 2 < count) ok = fetch_next(i + 2);
         }
     } else {
         fewer_registers<REST_REGS>();
@@ -375,13 +476,14 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 commit(&v_done);
                 commit(&empty_a[ph]);
                 if (BWD) {
-                    if (!wait(&full_c, ph)) break;
+                    if (!wait(&full_c, ph) || (i && !wait(&x_free, ph ^ 1))) break;
                     product<KEY, C / 16, true>(Y, tm + kVal, base + Smem::kC, LO);
                     commit(&a_done);
                     commit(&empty_c);
                     if (!wait(&y_free, ph)) break;
                 }
-                if (!wait(&full_b, ph) || !wait(&n_ready, ph)) break;
+                // Y held the parts of the state before this one: they have been taken out
+                if (!wait(&full_b, ph) || !wait(&n_ready, ph) || (i && !wait(&x_free, ph ^ 1))) break;
                 tc_after();
                 product<KEY, C / 16, true>(Y, tm + kNew, base + Smem::kB, LO);
                 commit(&d_done);
@@ -406,7 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
 
 template <typename T, int KEY, bool BWD>
 cudaError_t scan(const ScanParams& a, cudaStream_t st) {
-    constexpr int smem = ScanSmem<KEY>::kBytes;
+    constexpr int smem = ScanSmem<T, KEY>::kBytes;
     cudaError_t e = cudaFuncSetAttribute(delta_scan_kernel<T, KEY, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     delta_scan_kernel<T, KEY, BWD><<<dim3(a.p.B * a.p.HV, (a.p.DV + 127) / 128), THREADS, smem, st>>>(a);
@@ -414,11 +516,14 @@ cudaError_t scan(const ScanParams& a, cudaStream_t st) {
     return cudaGetLastError();
 }
 template <typename T, bool BWD>
-cudaError_t scan_key(const ScanParams& a, cudaStream_t st) {
+cudaError_t scan_key(ScanParams& a, cudaStream_t st) {
+    const long long* vs = a.v_stride;
+    a.vec_v = reinterpret_cast<uintptr_t>(a.v) % 16 == 0 && vs[0] * sizeof(T) % 16 == 0 && vs[1] * sizeof(T) % 16 == 0 &&
+              vs[2] * sizeof(T) % 16 == 0 && a.p.DV * sizeof(T) % 16 == 0;
     return a.rec.key == 64 ? scan<T, 64, BWD>(a, st) : scan<T, 128, BWD>(a, st);
 }
 template <bool BWD>
-cudaError_t scan_typed(const ScanParams& a, cudaStream_t st) {
+cudaError_t scan_typed(ScanParams& a, cudaStream_t st) {
     return a.p.dtype == AUSSM_FLOAT32 ? scan_key<float, BWD>(a, st)
            : a.p.dtype == AUSSM_BFLOAT16 ? scan_key<__nv_bfloat16, BWD>(a, st) : scan_key<__half, BWD>(a, st);
 }
