@@ -91,14 +91,23 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return
 // exp(-200) is zero in float32: g of -inf (forget everything) would make differences of its sums NaN
 __device__ __forceinline__ float clamp_log_decay(float g) { return g < -200.f ? -200.f : g; }
 
-// Sizes and buffers of a problem.  keep: [records][V' (chunk heads, 64, DV)][entry states (chunk heads, DK, DV)]
+// What the recurrences leave for the gradients, per chunk, value head and slice of 128 value columns, as it lies in tensor
+// memory: 16 bytes of a lane (value column) after the other, [words / 4][128 lanes].  A state: `key` words a lane (8 keys in
+// 4 words of hi parts, then the lo parts), V': 64 words (8 steps in 4 words), and behind them the lanes' float32 factors.
+// X: 64 float32 words a lane.
+//
+// Sizes and buffers of a problem.  keep: [records][V'][entry states], backward workspace: [X][gradients of exit states]
 struct DeltaPlan {
     int n;                 // chunks of a sequence
+    int slices;            // of 128 value columns
+    __host__ __device__ static size_t state_bytes(int key) { return (size_t)key * 512 + 512; }
+    __host__ __device__ static size_t news_bytes() { return 64 * 512 + 512; }
+    __host__ __device__ static size_t x_bytes() { return 64 * 512; }
     size_t heads;          // chunk heads: (b * HV + h) * n + chunk
     DeltaRecord rec;
     size_t keep_bytes, bwd_bytes;
     size_t news, states;   // byte offsets in keep
-    size_t dstates;        // byte offset in the backward workspace: [X (chunk heads, 64, DV)][gradients of exit states]
+    size_t dstates;        // byte offset in the backward workspace
 };
 DeltaPlan delta_plan(const aussm_b200_delta_t& p);
 
@@ -111,13 +120,13 @@ struct DeltaScan {
     const float* s0;
     float* s1;
     void* out;
-    float *rows, *states;      // V' / X and entry states / gradients of exit states of every chunk; forward: NULL = not kept
+    void *rows, *states;       // V' / X and entry states / gradients of exit states; forward: NULL = not kept
 };
 cudaError_t launch_delta_scan(const aussm_b200_delta_t& p, const DeltaPlan& plan, const DeltaScan& io, bool backward,
                               cudaStream_t stream);
 struct DeltaGrads {
     const void *records, *go;
-    const float *news, *x, *states, *dstates;
+    const void *news, *x, *states, *dstates;
     void *dq, *dk;
     float *dg, *dbeta;
 };

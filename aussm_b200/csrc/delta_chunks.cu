@@ -14,11 +14,13 @@ DeltaPlan delta_plan(const aussm_b200_delta_t& p) {
     d.n = (p.L + C - 1) / C;
     d.heads = (size_t)p.B * p.HV * d.n;
     d.rec.key = p.DK <= 64 ? 64 : 128;
+    d.slices = (p.DV + 127) / 128;
+    const size_t pieces = d.heads * d.slices;
     d.news = d.heads * d.rec.bytes();
-    d.states = d.news + up256(d.heads * C * p.DV * sizeof(float));
-    d.keep_bytes = d.states + up256(d.heads * p.DK * p.DV * sizeof(float));
-    d.dstates = up256(d.heads * C * p.DV * sizeof(float));
-    d.bwd_bytes = d.dstates + up256(d.heads * p.DK * p.DV * sizeof(float));
+    d.states = d.news + up256(pieces * DeltaPlan::news_bytes());
+    d.keep_bytes = d.states + up256(pieces * DeltaPlan::state_bytes(d.rec.key));
+    d.dstates = up256(pieces * DeltaPlan::x_bytes());
+    d.bwd_bytes = d.dstates + up256(pieces * DeltaPlan::state_bytes(d.rec.key));
     return d;
 }
 
@@ -28,7 +30,7 @@ cudaError_t launch_delta_fwd(const aussm_b200_delta_t& p, const DeltaInputs& in,
     cudaError_t e = launch_delta_prepare(p, plan, in, keep, st);
     if (e != cudaSuccess) return e;
     uint8_t* k = static_cast<uint8_t*>(keep);
-    float *news = train ? reinterpret_cast<float*>(k + plan.news) : nullptr, *states = train ? reinterpret_cast<float*>(k + plan.states) : nullptr;
+    void *news = train ? k + plan.news : nullptr, *states = train ? k + plan.states : nullptr;
     return launch_delta_scan(p, plan, {keep, in.v, s0, s1, o, news, states}, false, st);
 }
 
@@ -38,11 +40,9 @@ cudaError_t launch_delta_bwd(const aussm_b200_delta_t& p, const DeltaInputs& in,
     const DeltaPlan plan = delta_plan(p);
     const uint8_t* k = static_cast<const uint8_t*>(keep);
     uint8_t* w = static_cast<uint8_t*>(workspace);
-    float *x = reinterpret_cast<float*>(w), *dstates = reinterpret_cast<float*>(w + plan.dstates);
-    cudaError_t e = launch_delta_scan(p, plan, {keep, go, gs1, ds0, dv, x, dstates}, true, st);
+    cudaError_t e = launch_delta_scan(p, plan, {keep, go, gs1, ds0, dv, w, w + plan.dstates}, true, st);
     if (e != cudaSuccess) return e;
-    return launch_delta_grads(p, plan, in, {keep, go, reinterpret_cast<const float*>(k + plan.news), x,
-                                            reinterpret_cast<const float*>(k + plan.states), dstates, dq, dk, dg, dbeta}, st);
+    return launch_delta_grads(p, plan, in, {keep, go, k + plan.news, w, k + plan.states, w + plan.dstates, dq, dk, dg, dbeta}, st);
 }
 
 }  // namespace aussm

@@ -3,7 +3,8 @@
 //
 // One block per chunk and key head, 16 warps; the value heads of the key head follow each other and add up in shared
 // memory (no atomics: a fixed order).  The products with a contraction over the value columns (dO V'^T, X V'^T, dO S^T,
-// X S^T, V' dS^T) take them 64 at a time: the operands come in with wide loads, their FP16 parts go to shared memory under
+// X S^T, V' dS^T) take them 64 at a time: the operands come in as the recurrences left them (a value column's 8 keys or
+// steps in 16 bytes, so V', X and the states lie transposed and are read with transposing fragment loads), their FP16 parts go to shared memory under
 // one power of two per tile (it only shrinks from slice to slice, so the sums stay in one unit) and mma.sync runs the
 // three products of parts.  Then K K^T, and dO V'^T and X V'^T, masked and decayed, meet Q and K.
 // The gradient of g_t is summed over just the pairs and states it stands for (see the end): sums over all pairs of which
@@ -26,7 +27,8 @@ struct GradParams {
     const uint8_t* records;
     DeltaRecord rec;
     int n;
-    const float *news, *x, *states, *dstates;      // V', X, S, dS of every chunk and head
+    const uint8_t *news, *x, *states, *dstates;    // V', X, S, dS
+    int slices;
     void *dq, *dk;
     float *dg, *dbeta;
     int vec_q, vec_k, vec_v, vec_go, vec_out;      // rows can be taken 16 bytes at a time
@@ -52,13 +54,12 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
     float* vec = reinterpret_cast<float*>(sm + Smem::kVec);
     float *ghi = vec, *glo = vec + 64, *be = vec + 128, *rowa = vec + 192 /* (4, 64) */, *rowk = vec + 448 /* (4, 64) */,
           *rowz = vec + 704 /* (4, 64) */;
-    __shared__ float red[6 * WARPS], xv[C], ssum[WARPS], am[C], kkt[C];
+    __shared__ float red[6 * WARPS], xv[8][C], ssum[WARPS], am[C], kkt[C];
     const aussm_b200_delta_t& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int rb = warp & 3, cq = warp >> 2;             // 16 rows, a quarter of the columns
     const int r = p.HV / p.HK, c = blockIdx.x % a.n, bk = blockIdx.x / a.n, b = bk / p.HK, hk = bk % p.HK;
     const int t0 = c * C, rows = min(C, p.L - t0), DV = p.DV;
-    const bool vecf = DV % 8 == 0;
     const uint32_t base = smem_addr(sm);
 
     for (int e = tid; e < 2 * C * KEY; e += NT) accq[e] = 0.f;
@@ -68,8 +69,6 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         const float* head = reinterpret_cast<const float*>(a.records + at * a.rec.bytes());
         const T* go = static_cast<const T*>(a.go) + b * p.go_stride[0] + t0 * p.go_stride[1] + h * p.go_stride[2];
         const T* v = static_cast<const T*>(a.in.v) + b * p.v_stride[0] + t0 * p.v_stride[1] + h * p.v_stride[2];
-        const float *news = a.news + at * C * DV, *xs = a.x + at * C * DV;
-        const float *st = a.states + at * p.DK * DV, *ds = a.dstates + at * p.DK * DV;
         __syncthreads();                                 // the last head is done with shared memory
         if (tid < C) { ghi[tid] = head[kGHi + tid]; glo[tid] = head[kGLo + tid]; be[tid] = head[kBeta + tid]; }
 
@@ -78,17 +77,32 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         int e[5] = {100, 100, 100, 100, 100};            // exponents of dO, X, V', S, dS
         float dotv = 0.f, dots = 0.f;
         for (int v0 = 0; v0 < DV; v0 += VS) {
-            const int row = tid >> 3, col = (tid & 7) * 8, cols = DV - v0;
+            const int cols = DV - v0;
+            // dO by rows; V', X and the states by value column `dv` and groups of 8 steps or keys
+            const int row = tid >> 3, col = (tid & 7) * 8, dv = tid & 63, grp = tid >> 6, l = (v0 & 64) + dv;
+            const size_t piece = at * a.slices + (v0 >> 7);
+            const bool there = dv < cols;
             float f[3][8], s[KEY / 64][8], d[KEY / 64][8], m[5] = {};
             if (row < rows) load8(go + row * p.go_stride[1] + v0, col, cols, a.vec_go, f[0]); else zero8(f[0]);
-            load8(xs + (size_t)row * DV + v0, col, cols, vecf, f[1]);
-            load8(news + (size_t)row * DV + v0, col, cols, vecf, f[2]);
+            auto parts = [&](const uint8_t* base, int groups, int g8, float (&o)[8]) {
+                const uint8_t* x = base + ((size_t)g8 * 128 + l) * 16;
+                join8(x, x + (size_t)groups * 2048, reinterpret_cast<const float*>(base + (size_t)groups * 4096)[l], o);
+            };
+            if (there) {
+                const float4* x4 = reinterpret_cast<const float4*>(a.x + piece * DeltaPlan::x_bytes()) + l;
+                const float4 x0 = x4[2 * grp * 128], x1 = x4[(2 * grp + 1) * 128];
+                f[1][0] = x0.x; f[1][1] = x0.y; f[1][2] = x0.z; f[1][3] = x0.w;
+                f[1][4] = x1.x; f[1][5] = x1.y; f[1][6] = x1.z; f[1][7] = x1.w;
+                parts(a.news + piece * DeltaPlan::news_bytes(), C / 8, grp, f[2]);
+            } else {
+                zero8(f[1]);
+                zero8(f[2]);
+            }
 #pragma unroll
             for (int y = 0; y < KEY / 64; ++y) {
-                const int x = row + 64 * y;
-                if (x < p.DK) {
-                    load8(st + (size_t)x * DV + v0, col, cols, vecf, s[y]);
-                    load8(ds + (size_t)x * DV + v0, col, cols, vecf, d[y]);
+                if (there) {
+                    parts(a.states + piece * DeltaPlan::state_bytes(KEY), KEY / 8, grp + 8 * y, s[y]);
+                    parts(a.dstates + piece * DeltaPlan::state_bytes(KEY), KEY / 8, grp + 8 * y, d[y]);
                 } else {
                     zero8(s[y]);
                     zero8(d[y]);
@@ -100,12 +114,6 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             }
 #pragma unroll
             for (int y = 0; y < 3; ++y) m[y] = max8(f[y], 0.f);
-            if (row < rows) {
-                float w[8];
-                load8(v + row * p.v_stride[1] + v0, col, cols, a.vec_v, w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) dotv = fmaf(f[1][i], w[i], dotv);
-            }
             block_max<WARPS>(m, red);
             float shrink[5];
 #pragma unroll
@@ -114,13 +122,13 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                 shrink[y] = v0 ? pow2_float(max(-126, now - e[y])) : 0.f;
                 e[y] = now;
             }
-            const int pa = panel_at(row, col);
-            put8(sm + Smem::kGo + pa, SQ_LO, f[0], pow2_float(e[0]));
-            put8(sm + Smem::kX + pa, SQ_LO, f[1], pow2_float(e[1]));
-            put8(sm + Smem::kNew + pa, SQ_LO, f[2], pow2_float(e[2]));
+            const int pt = panel_at(dv, 8 * grp);
+            put8(sm + Smem::kGo + panel_at(row, col), SQ_LO, f[0], pow2_float(e[0]));
+            put8(sm + Smem::kX + pt, SQ_LO, f[1], pow2_float(e[1]));
+            put8(sm + Smem::kNew + pt, SQ_LO, f[2], pow2_float(e[2]));
 #pragma unroll
             for (int y = 0; y < KEY / 64; ++y) {
-                const int ps = panel_at(row + 64 * y, col);
+                const int ps = panel_at(dv, 8 * grp + 64 * y);
                 put8(sm + Smem::kS + ps, ST_LO, s[y], pow2_float(e[3]));
                 put8(sm + Smem::kDs + ps, ST_LO, d[y], pow2_float(e[4]));
             }
@@ -139,6 +147,16 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                     }
             }
             __syncthreads();
+            if (dv < rows) {                             // X.V of step dv over the columns of group grp
+                float w[8], sum = 0.f;
+                load8(v + dv * p.v_stride[1] + v0, 8 * grp, cols, a.vec_v, w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint8_t* x = sm + Smem::kX + panel_at(8 * grp + i, dv);
+                    sum = fmaf(__half2float(*reinterpret_cast<const __half*>(x)) + __half2float(*reinterpret_cast<const __half*>(x + SQ_LO)), w[i], sum);
+                }
+                dotv = fmaf(sum, pow2_float(-e[1]), dotv);
+            }
 #pragma unroll
             for (int k0 = 0; k0 < VS; k0 += 16) {
                 if (k0 >= cols) break;
@@ -146,12 +164,13 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                 const int fa = frag_a(rb * 16, k0);
                 ldmatrix4(gh, base + Smem::kGo + fa);
                 ldmatrix4(gl, base + Smem::kGo + SQ_LO + fa);
-                ldmatrix4(xh, base + Smem::kX + fa);
-                ldmatrix4(xl, base + Smem::kX + SQ_LO + fa);
+                const int fx = frag_at(k0, rb * 16);
+                ldmatrix4_trans(xh, base + Smem::kX + fx);
+                ldmatrix4_trans(xl, base + Smem::kX + SQ_LO + fx);
                 if (cq <= rb) {                          // on and below the diagonal
-                    const int fb = frag_b(cq * 16, k0);
-                    ldmatrix4(bh, base + Smem::kNew + fb);
-                    ldmatrix4(bl, base + Smem::kNew + SQ_LO + fb);
+                    const int fb = frag_bt(k0, cq * 16);
+                    ldmatrix4_trans(bh, base + Smem::kNew + fb);
+                    ldmatrix4_trans(bl, base + Smem::kNew + SQ_LO + fb);
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         mma16816(dp[y], gl, bh[2 * y], bh[2 * y + 1]);
@@ -164,9 +183,9 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                 }
 #pragma unroll
                 for (int x = 0; x < NW / 2; ++x) {
-                    const int fb = frag_b(cq * (KEY / 4) + x * 16, k0);
-                    ldmatrix4(bh, base + Smem::kS + fb);
-                    ldmatrix4(bl, base + Smem::kS + ST_LO + fb);
+                    const int fb = frag_bt(k0, cq * (KEY / 4) + x * 16);
+                    ldmatrix4_trans(bh, base + Smem::kS + fb);
+                    ldmatrix4_trans(bl, base + Smem::kS + ST_LO + fb);
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         mma16816(dqt[2 * x + y], gl, bh[2 * y], bh[2 * y + 1]);
@@ -177,13 +196,13 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                         mma16816(zz[2 * x + y], xh, bh[2 * y], bh[2 * y + 1]);
                     }
                 }
-                ldmatrix4(gh, base + Smem::kNew + fa);
-                ldmatrix4(gl, base + Smem::kNew + SQ_LO + fa);
+                ldmatrix4_trans(gh, base + Smem::kNew + fx);
+                ldmatrix4_trans(gl, base + Smem::kNew + SQ_LO + fx);
 #pragma unroll
                 for (int x = 0; x < NW / 2; ++x) {
-                    const int fb = frag_b(cq * (KEY / 4) + x * 16, k0);
-                    ldmatrix4(bh, base + Smem::kDs + fb);
-                    ldmatrix4(bl, base + Smem::kDs + ST_LO + fb);
+                    const int fb = frag_bt(k0, cq * (KEY / 4) + x * 16);
+                    ldmatrix4_trans(bh, base + Smem::kDs + fb);
+                    ldmatrix4_trans(bl, base + Smem::kDs + ST_LO + fb);
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         mma16816(dkt[2 * x + y], gl, bh[2 * y], bh[2 * y + 1]);
@@ -194,10 +213,8 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             }
             __syncthreads();
         }
-        // X.V of a row (8 threads each), the product of the states
-#pragma unroll
-        for (int m = 1; m < 8; m *= 2) dotv += __shfl_xor_sync(0xffffffffu, dotv, m);
-        if ((tid & 7) == 0) xv[tid >> 3] = dotv;
+        // X.V of a step (a thread for every 8 columns), the product of the states
+        xv[tid >> 6][tid & 63] = dotv;
 #pragma unroll
         for (int m = 16; m; m >>= 1) dots += __shfl_xor_sync(0xffffffffu, dots, m);
         if (lane == 0) ssum[warp] = dots;
@@ -409,8 +426,11 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         if (tid < C) {
             am[tid] = (rowa[tid] + rowa[64 + tid]) + (rowa[128 + tid] + rowa[192 + tid]);
             kkt[tid] = (rowk[tid] + rowk[64 + tid]) + (rowk[128 + tid] + rowk[192 + tid]);
+            float dotx = 0.f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) dotx += xv[w][tid];
             if (tid < rows)
-                a.dbeta[o + (long long)tid * p.HV] = xv[tid] + ((rowz[tid] + rowz[64 + tid]) + (rowz[128 + tid] + rowz[192 + tid]));
+                a.dbeta[o + (long long)tid * p.HV] = dotx + ((rowz[tid] + rowz[64 + tid]) + (rowz[128 + tid] + rowz[192 + tid]));
         }
         const int i = tid >> 3, seg = tid & 7;           // eight threads a row: sums of F up to and with each column
         {
@@ -501,7 +521,8 @@ cudaError_t launch_delta_grads(const aussm_b200_delta_t& p, const DeltaPlan& pla
                                cudaStream_t st) {
     GradParams a = {};
     a.p = p; a.in = in; a.go = io.go; a.records = static_cast<const uint8_t*>(io.records); a.rec = plan.rec; a.n = plan.n;
-    a.news = io.news; a.x = io.x; a.states = io.states; a.dstates = io.dstates;
+    a.news = static_cast<const uint8_t*>(io.news); a.x = static_cast<const uint8_t*>(io.x); a.slices = plan.slices;
+    a.states = static_cast<const uint8_t*>(io.states); a.dstates = static_cast<const uint8_t*>(io.dstates);
     a.dq = io.dq; a.dk = io.dk; a.dg = io.dg; a.dbeta = io.dbeta;
     return p.dtype == AUSSM_FLOAT32 ? grads_typed<float>(a, st)
            : p.dtype == AUSSM_BFLOAT16 ? grads_typed<__nv_bfloat16>(a, st) : grads_typed<__half>(a, st);

@@ -8,15 +8,16 @@
 // product is converted by the thread that owns the row and goes back as the next product's A without leaving the lane.
 // A row's FP16 parts are scaled by a power of two of the row's own: no reduction between threads.
 //
-// Warps 0-3 own the state (the chain: convert S, product, convert V', product, add), warps 4-7 bring V (dO) in (a chunk
-// ahead, through shared memory) and everything out (O or X; the states and V' that a backward pass wants, rebuilt from
-// the parts in tensor memory), warp 8 copies the records' tiles (bulk copies), warp 9 issues the MMAs
-// (10 and 11 fill their warpgroup, which hands its registers to the other two).  Tensor memory, 512 columns:
-// [X | Y] take turns as the parts of S and as the product that updates it, two accumulators of 64 columns, the parts of
-// V' and of V.  Every wait is bounded: one that runs out sets the status word and the block ends.
+// Warps 0-7 own the state, two threads a row, each half of its columns (the chain: convert S, product, convert V',
+// product, add); warps 8-11 bring V (dO) in (a chunk ahead, through shared memory) and everything out (O or X; the parts of
+// S and V' that a backward pass reads, as they lie in tensor memory); warp 12 copies the records' tiles (bulk copies),
+// warp 13 issues the MMAs (14 and 15 fill their warpgroup, which hands its registers to the others).  Tensor memory, 512
+// columns: [X | Y] take turns as the parts of S and as the product that updates it, two accumulators of 64 columns, the
+// parts of V' and of V.  Every wait is bounded: one that runs out sets the status word and the block ends.
 //
-// The three roles walk different code, chunk after chunk, out of one instruction cache: with every loop unrolled the issue
-// of 36 MMAs took 4700 cycles instead of 1700.  Only what must be (registers that are indexed) is unrolled.
+// The roles walk different code, chunk after chunk, out of one instruction cache: with every loop unrolled the issue of 36
+// MMAs took 4700 cycles instead of 1700.  Only what must be (registers that are indexed) is unrolled, and the state's
+// conversions, the longest straight line, are cut in two halves that run side by side.
 #include "common.cuh"
 #include "delta.cuh"
 #include "host_common.cuh"
@@ -25,9 +26,9 @@ namespace aussm {
 namespace {
 
 constexpr int C = kDeltaChunk;
-constexpr int THREADS = 384;             // three warpgroups; launched with 168 registers a thread, 504 for one of each
-constexpr int MAIN_REGS = 240, SIDE_REGS = 168, REST_REGS = 96;
-static_assert(MAIN_REGS + SIDE_REGS + REST_REGS <= 3 * 168, "more registers than the block is launched with");
+constexpr int THREADS = 512;             // four warpgroups; launched with 128 registers a thread, 512 for one of each
+constexpr int MAIN_REGS = 152, SIDE_REGS = 136, REST_REGS = 72;
+static_assert(2 * MAIN_REGS + SIDE_REGS + REST_REGS <= 4 * 128, "more registers than the block is launched with");
 constexpr int SQUARE = DeltaRecord::kSquare;
 // tensor memory columns
 constexpr uint32_t kX = 0, kY = 128, kAcc = 256, kAcc2 = 320, kNew = 384, kVal = 448;
@@ -42,8 +43,8 @@ struct ScanParams {
     const float* s0;                     // forward: initial state, backward: gradient of the final state (NULL = 0)
     float* s1;                           // forward: final state, backward: gradient of the initial state (NULL)
     void* out;                           // forward: O; backward: dV
-    float* rows;                         // forward: V' of every chunk (NULL = not kept); backward: X
-    float* states;                       // forward: entry states (NULL); backward: gradients of the exit states
+    uint4* rows;                         // forward: V' of every chunk (NULL = not kept); backward: X
+    uint4* states;                       // forward: entry states (NULL); backward: gradients of the exit states
     int vec_v;                           // rows of v can be copied 16 bytes at a time
     int* status;
 };
@@ -122,9 +123,9 @@ __device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, int 
     }
 }
 
-// COUNT values of this thread's row, scaled by f, as hi parts (COUNT / 2 columns) and lo parts behind them
+// COUNT values of a row, scaled by f, as hi parts (COUNT / 2 columns at t) and lo parts (`lo` columns behind them)
 template <int COUNT>
-__device__ __forceinline__ void store_parts(uint32_t t, const float2 (&x)[COUNT / 2], float f) {
+__device__ __forceinline__ void store_parts(uint32_t t, uint32_t lo_cols, const float2 (&x)[COUNT / 2], float f) {
     const float2 f2 = make_float2(f, f), minus = make_float2(-1.f, -1.f);
 #pragma unroll
     for (int i = 0; i < COUNT / 2; i += 16) {
@@ -138,23 +139,18 @@ __device__ __forceinline__ void store_parts(uint32_t t, const float2 (&x)[COUNT 
             lo[j] = *reinterpret_cast<const uint32_t*>(&l);
         }
         tmem_st16(t + i, hi);
-        tmem_st16(t + COUNT / 2 + i, lo);
+        tmem_st16(t + lo_cols + i, lo);
     }
 }
 template <int COUNT>
-__device__ __forceinline__ int row_exponent(const float2 (&x)[COUNT]) {
+__device__ __forceinline__ float row_max(const float2 (&x)[COUNT]) {
     float m0 = 0.f, m1 = 0.f;
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
         m0 = fmaxf(m0, fabsf(x[i].x));
         m1 = fmaxf(m1, fabsf(x[i].y));
     }
-    return part_exponent(fmaxf(m0, m1));
-}
-// two values from a word of hi parts and one of lo parts
-__device__ __forceinline__ float2 join2(uint32_t hi, uint32_t lo, float f) {
-    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi)), l = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-    return make_float2((h.x + l.x) * f, (h.y + l.y) * f);
+    return fmaxf(m0, m1);
 }
 
 // the same answer in all lanes: what follows is executed by whole warps
@@ -177,13 +173,15 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full_a[2], full_b, full_c, full_e, empty_a[2], empty_b, empty_c, empty_e;
     __shared__ uint64_t s_ready, v_ready, v_done, n_ready, a_done, y_free, d_done, o_done, o_free, x_free, v_loaded, v_read;
+    __shared__ uint64_t pair_s[4], pair_n[4];
     __shared__ uint32_t holder;
-    __shared__ float un_s[2][128], un_v[128], un_n[128];
+    __shared__ float un_s[2][128], un_v[128], un_n[128], max_s[2][128], max_n[2][128];
+    __shared__ __align__(16) float betas[C];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const aussm_b200_delta_t& p = a.p;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int bh = blockIdx.x, b = bh / p.HV, h = bh % p.HV;
-    const int v = blockIdx.y * 128 + (threadIdx.x & 127);             // value column of warps 0-3 and of warps 4-7
+    const int me = threadIdx.x & 127, v = blockIdx.y * 128 + me;      // row (value column) of the threads of warps 0-11
     const bool mine = v < p.DV;
     const int count = a.n;                                            // chunks this block walks
     auto chunk_at = [&](int i) { return BWD ? a.n - 1 - i : i; };
@@ -193,32 +191,41 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         for (uint64_t* x : {&full_a[0], &full_a[1], &full_b, &full_c, &full_e, &empty_a[0], &empty_a[1], &empty_b, &empty_c,
                             &empty_e, &v_done, &a_done, &d_done, &o_done})
             mbar_init(x, 1);
-        for (uint64_t* x : {&s_ready, &v_ready, &n_ready, &y_free, &o_free, &x_free, &v_loaded, &v_read}) mbar_init(x, 128);
+        for (uint64_t* x : {&s_ready, &n_ready, &y_free}) mbar_init(x, 256);
+        for (uint64_t* x : {&v_ready, &o_free, &x_free, &v_loaded, &v_read}) mbar_init(x, 128);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&pair_s[i], 64);
+            mbar_init(&pair_n[i], 64);
+        }
         fence_mbar_init();
         fence_proxy_async();
     }
-    if (warp == 9) tmem_alloc512(&holder);
+    if (warp == 13) tmem_alloc512(&holder);
     tc_before();
     __syncthreads();
     tc_after();
     const uint32_t tm = holder, lanes = tm + ((uint32_t)((warp & 3) * 32) << 16);
 
-    if (warp < 4) {
-        // ---- the state -----------------------------------------------------------------------------------------
+    if (warp < 8) {
+        // ---- the state: columns [half * HALF, half * HALF + HALF) of row `me` ------------------------------------------
         more_registers<MAIN_REGS>();
-        float2 s[KEY / 2];
+        constexpr int HALF = KEY / 2;
+        const int half = warp >> 2;
+        const uint32_t sc = half * HALF;                              // first column in a float32 row
+        float2 s[HALF / 2];
 #pragma unroll
-        for (int x = 0; x < KEY / 2; ++x) {
-            const float* src = a.s0 + ((size_t)bh * p.DK + 2 * x) * p.DV + v;
-            s[x] = make_float2(a.s0 && mine && 2 * x < p.DK ? src[0] : 0.f, a.s0 && mine && 2 * x + 1 < p.DK ? src[p.DV] : 0.f);
+        for (int x = 0; x < HALF / 2; ++x) {
+            const int k0 = sc + 2 * x;
+            const float* src = a.s0 + ((size_t)bh * p.DK + k0) * p.DV + v;
+            s[x] = make_float2(a.s0 && mine && k0 < p.DK ? src[0] : 0.f, a.s0 && mine && k0 + 1 < p.DK ? src[p.DV] : 0.f);
         }
-        // s = s * keep + r * f over all columns of a product
+        // s = s * keep + r * f over the columns of a product
         auto add = [&](uint32_t t, float keep, float f) {
             const float2 k2 = make_float2(keep, keep), f2 = make_float2(f, f);
 #pragma unroll
-            for (int x = 0; x < KEY; x += 32) {
+            for (int x = 0; x < HALF; x += 32) {
                 uint32_t r[32];
-                tmem_ld32(t + x, r);
+                tmem_ld32(t + sc + x, r);
                 tc_wait_ld();
 #pragma unroll
                 for (int y = 0; y < 16; ++y)
@@ -231,34 +238,40 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             const float* head = reinterpret_cast<const float*>(record(i));
             const float un1 = head[BWD ? kUnKt : kUnW], un2 = head[BWD ? kUnP : kUnT], un3 = head[BWD ? kUnW : kUnKt],
                         unq = head[kUnQ], gamma = head[kGamma];
-            const int es = row_exponent(s);
+            // one power of two for the whole row: the halves tell each other their maxima
+            max_s[half][me] = row_max(s);
+            arrive(&pair_s[warp & 3]);
+            if (!warp_wait(&pair_s[warp & 3], ph, a.status)) break;
+            const int es = part_exponent(fmaxf(max_s[0][me], max_s[1][me]));
             const float uns = pow2_float(-es);
-            store_parts<KEY>(X, s, pow2_float(es));
-            un_s[ph][threadIdx.x] = uns;
+            store_parts<HALF>(X + half * (HALF / 2), KEY / 2, s, pow2_float(es));
+            if (half == 0) un_s[ph][me] = uns;
             tc_wait_st();
             tc_before();
             arrive(&s_ready);
-            // V' (dV')
+            // V' (dV'), columns [32 half, 32 half + 32)
             if (!warp_wait(&v_done, ph, a.status) || !warp_wait(&v_ready, ph, a.status)) break;
             tc_after();
-            const float unv = un_v[threadIdx.x], f1 = (BWD ? uns : -uns) * un1, f2 = unv * un2;
-            float2 w[C / 2];
-#pragma unroll
-            for (int x = 0; x < C; x += 16) {
-                uint32_t r1[16], r2[16];
-                tmem_ld16(lanes + kAcc + x, r1);
-                tmem_ld16(lanes + kAcc2 + x, r2);
+            const float unv = un_v[me], f1 = (BWD ? uns : -uns) * un1, f2 = unv * un2;
+            float2 w[16];
+            {
+                uint32_t r1[32], r2[32];
+                tmem_ld32(lanes + kAcc + half * 32, r1);
+                tmem_ld32(lanes + kAcc2 + half * 32, r2);
                 tc_wait_ld();
 #pragma unroll
-                for (int y = 0; y < 8; ++y)
-                    w[x / 2 + y] = __ffma2_rn(make_float2(__uint_as_float(r1[2 * y]), __uint_as_float(r1[2 * y + 1])), make_float2(f1, f1),
-                                              __fmul2_rn(make_float2(__uint_as_float(r2[2 * y]), __uint_as_float(r2[2 * y + 1])), make_float2(f2, f2)));
+                for (int y = 0; y < 16; ++y)
+                    w[y] = __ffma2_rn(make_float2(__uint_as_float(r1[2 * y]), __uint_as_float(r1[2 * y + 1])), make_float2(f1, f1),
+                                      __fmul2_rn(make_float2(__uint_as_float(r2[2 * y]), __uint_as_float(r2[2 * y + 1])), make_float2(f2, f2)));
             }
-            const int en = row_exponent(w);
+            max_n[half][me] = row_max(w);
+            arrive(&pair_n[warp & 3]);
+            if (!warp_wait(&pair_n[warp & 3], ph, a.status)) break;
+            const int en = part_exponent(fmaxf(max_n[0][me], max_n[1][me]));
             const float unn = pow2_float(-en);
             if (i && !warp_wait(&x_free, ph ^ 1, a.status)) break;      // the last V' has been taken out
-            store_parts<C>(lanes + kNew, w, pow2_float(en));
-            un_n[threadIdx.x] = unn;
+            store_parts<32>(lanes + kNew + half * 16, C / 2, w, pow2_float(en));
+            if (half == 0) un_n[me] = unn;
             tc_wait_st();
             tc_before();
             arrive(&n_ready);
@@ -275,16 +288,16 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         }
         if (a.s1 && mine) {
 #pragma unroll
-            for (int x = 0; x < KEY / 2; ++x) {
-                float* dst = a.s1 + ((size_t)bh * p.DK + 2 * x) * p.DV + v;
-                if (2 * x < p.DK) dst[0] = s[x].x;
-                if (2 * x + 1 < p.DK) dst[p.DV] = s[x].y;
+            for (int x = 0; x < HALF / 2; ++x) {
+                const int k0 = sc + 2 * x;
+                float* dst = a.s1 + ((size_t)bh * p.DK + k0) * p.DV + v;
+                if (k0 < p.DK) dst[0] = s[x].x;
+                if (k0 + 1 < p.DK) dst[p.DV] = s[x].y;
             }
         }
-    } else if (warp < 8) {
+    } else if (warp < 12) {
         // ---- V (dO) in; O (X), states and V' out -----------------------------------------------------------------
         more_registers<SIDE_REGS>();
-        const int me = threadIdx.x & 127;
         const T* src = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + blockIdx.y * 128;
         T* dst = static_cast<T*>(a.out) + ((long long)b * p.L * p.HV + h) * p.DV + v;
         T* tile = reinterpret_cast<T*>(sm + Smem::kV);
@@ -293,6 +306,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         auto fetch = [&](int i) {
             const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
             const T* from = src + (long long)t0 * a.v_stride[1];
+            if (me < C / 4) cp_async16(betas + 4 * me, reinterpret_cast<const float*>(record(i)) + kBeta + 4 * me);
             if (a.vec_v) {
                 constexpr int E = 16 / (int)sizeof(T), PIECES = 128 / E;
 #pragma unroll 1
@@ -308,8 +322,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         };
         // chunk i's row of this lane from shared memory to the parts in tensor memory; false: a wait ran out
         auto hand_over = [&](int i) {
-            const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
-            const float* be = reinterpret_cast<const float*>(record(i)) + kBeta;
+            const int rows = mine ? min(C, p.L - chunk_at(i) * C) : 0;
             cp_async_wait<0>();
             arrive(&v_loaded);
             if (!warp_wait(&v_loaded, i & 1, a.status)) return false;
@@ -317,19 +330,25 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
 #pragma unroll 1
             for (int x = 0; x < C; x += 16)
 #pragma unroll
-                for (int y = 0; y < 16; ++y)
-                    if (x + y < rows) m = fmaxf(m, fabsf(to_f32(tile[(x + y) * 128 + me]) * (BWD ? 1.f : be[x + y])));
-            const int e = part_exponent(mine ? m : 0.f);
-            const float f = mine ? pow2_float(e) : 0.f;
+                for (int y = 0; y < 16; ++y) {
+                    const float f = to_f32(tile[(x + y) * 128 + me]) * (BWD ? 1.f : betas[x + y]);
+                    m = fmaxf(m, x + y < rows ? fabsf(f) : 0.f);
+                }
+            const int e = part_exponent(m);
+            const float scale = pow2_float(e);
 #pragma unroll 1
             for (int x = 0; x < C; x += 16) {
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int y = 0; y < 8; ++y) {
-                    const int t = x + 2 * y;
-                    const float v0 = mine && t < rows ? to_f32(tile[t * 128 + me]) * (BWD ? f : be[t] * f) : 0.f;
-                    const float v1 = mine && t + 1 < rows ? to_f32(tile[(t + 1) * 128 + me]) * (BWD ? f : be[t + 1] * f) : 0.f;
-                    split2(v0, v1, hi[y], lo[y]);
+                    float f[2];
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const int t = x + 2 * y + z;
+                        const float g = to_f32(tile[t * 128 + me]) * (BWD ? 1.f : betas[t]);
+                        f[z] = t < rows ? g * scale : 0.f;
+                    }
+                    split2(f[0], f[1], hi[y], lo[y]);
                 }
                 tmem_st8(lanes + kVal + x / 2, hi);
                 tmem_st8(lanes + kVal + C / 2 + x / 2, lo);
@@ -338,14 +357,27 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             tc_wait_st();
             tc_before();
             arrive(&v_ready);
-            arrive(&v_read);
             return true;
         };
-        // the tile is free when all lanes have read chunk i from it
+        // the tile is free when all lanes have read chunk i - 1 from it
         auto fetch_next = [&](int i) {
+            arrive(&v_read);
             if (!warp_wait(&v_read, (i - 1) & 1, a.status)) return false;
             fetch(i);
             return true;
+        };
+        // `words` columns of tensor memory, 16 bytes a lane and store: [words / 4][128 lanes]
+        auto dump = [&](uint32_t t, int words, uint4* to) {
+            to += me;
+#pragma unroll 1
+            for (int x = 0; x < words; x += 16) {
+                uint32_t r[16];
+                tmem_ld16(t + x, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int z = 0; z < 4; ++z)
+                    if (mine) to[(x / 4 + z) * 128] = make_uint4(r[4 * z], r[4 * z + 1], r[4 * z + 2], r[4 * z + 3]);
+            }
         };
         fetch(0);
         bool ok = hand_over(0) && (count < 2 || fetch_next(1));
@@ -354,83 +386,67 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             const float* head = reinterpret_cast<const float*>(record(i));
             const float unq = head[kUnQ], un2 = head[BWD ? kUnT : kUnP];
             const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
+            const size_t at = ((size_t)bh * a.n + chunk_at(i)) * gridDim.y + blockIdx.y;
+            // the products with this chunk's V are done: the next one's parts go in
+            if (i + 1 < count) {
+                if (!warp_wait(BWD ? &a_done : &v_done, ph, a.status) || !warp_wait(&n_ready, ph, a.status)) break;
+                tc_after();
+                if (!hand_over(i + 1)) break;
+            }
             if (!warp_wait(&n_ready, ph, a.status) || !warp_wait(&o_done, ph, a.status)) break;
             tc_after();
-            const float f0 = un_s[ph][me], f1 = f0 * unq, unn = un_n[me], f2 = unn * un2;
+            const float uns = un_s[ph][me], f1 = uns * unq, unn = un_n[me], f2 = unn * un2;
             float y[C];
 #pragma unroll
-            for (int t = 0; t < C; t += 32) {
-                uint32_t r1[32], r2[32];
-                if (!BWD) tmem_ld32(lanes + kAcc + t, r1);
-                tmem_ld32(lanes + kAcc2 + t, r2);
+            for (int t = 0; t < C; t += 16) {
+                uint32_t r1[16], r2[16];
+                if (!BWD) tmem_ld16(lanes + kAcc + t, r1);
+                tmem_ld16(lanes + kAcc2 + t, r2);
                 tc_wait_ld();
 #pragma unroll
-                for (int u = 0; u < 32; ++u)
+                for (int u = 0; u < 16; ++u)
                     y[t + u] = BWD ? __uint_as_float(r2[u]) * f2 : fmaf(__uint_as_float(r1[u]), f1, __uint_as_float(r2[u]) * f2);
             }
             tc_before();
             arrive(&o_free);
-            if (i + 1 < count && !hand_over(i + 1)) break;
-            const size_t at = (size_t)bh * a.n + chunk_at(i);
             if (a.states) {
-                const uint32_t X = lanes + (ph ? kY : kX);
-                float* to = a.states + at * p.DK * p.DV + v;
-#pragma unroll 1
-                for (int x = 0; x < KEY; x += 32) {
-                    uint32_t hi[16], lo[16];
-                    tmem_ld16(X + x / 2, hi);
-                    tmem_ld16(X + KEY / 2 + x / 2, lo);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int z = 0; z < 16; ++z) {
-                        const float2 w = join2(hi[z], lo[z], f0);
-                        if (mine && x + 2 * z < p.DK) to[0] = w.x;
-                        to += p.DV;
-                        if (mine && x + 2 * z + 1 < p.DK) to[0] = w.y;
-                        to += p.DV;
-                    }
-                }
+                uint4* to = a.states + at * (KEY / 4 * 128 + 32);
+                dump(lanes + (ph ? kY : kX), KEY, to);
+                reinterpret_cast<float*>(to + KEY / 4 * 128)[me] = uns;
             }
             if (!BWD && a.rows) {
-                float* to = a.rows + at * C * p.DV + v;
-#pragma unroll 1
-                for (int x = 0; x < C; x += 32) {
-                    uint32_t hi[16], lo[16];
-                    tmem_ld16(lanes + kNew + x / 2, hi);
-                    tmem_ld16(lanes + kNew + C / 2 + x / 2, lo);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int z = 0; z < 16; ++z) {
-                        const float2 w = join2(hi[z], lo[z], unn);
-                        if (mine) { to[0] = w.x; to[p.DV] = w.y; }
-                        to += 2 * p.DV;
-                    }
-                }
+                uint4* to = a.rows + at * (C / 4 * 128 + 32);
+                dump(lanes + kNew, C, to);
+                reinterpret_cast<float*>(to + C / 4 * 128)[me] = unn;
             }
             tc_before();
             arrive(&x_free);
             if (mine) {
                 if (BWD) {
-                    float* keep = a.rows + at * C * p.DV + v;
+                    float4* to = reinterpret_cast<float4*>(a.rows) + at * (C / 4 * 128) + me;
 #pragma unroll
-                    for (int t = 0; t < C; ++t) {
-                        *keep = y[t];
-                        keep += p.DV;
-                        y[t] *= head[kBeta + t];
+                    for (int t = 0; t < C; t += 4) {
+                        to[t / 4 * 128] = make_float4(y[t], y[t + 1], y[t + 2], y[t + 3]);
+                        const float4 be = *reinterpret_cast<const float4*>(head + kBeta + t);
+                        y[t] *= be.x; y[t + 1] *= be.y; y[t + 2] *= be.z; y[t + 3] *= be.w;
                     }
                 }
                 T* to = dst + (long long)t0 * p.HV * p.DV;
+                const long long step = (long long)p.HV * p.DV;
+                if (rows == C) {
 #pragma unroll
-                for (int t = 0; t < C; ++t) {
-                    if (t < rows) *to = from_f32<T>(y[t]);
-                    to += (long long)p.HV * p.DV;
+                    for (int t = 0; t < C; ++t, to += step) *to = from_f32<T>(y[t]);
+                } else {
+#pragma unroll
+                    for (int t = 0; t < C; ++t, to += step)
+                        if (t < rows) *to = from_f32<T>(y[t]);
                 }
             }
             if (i + 2 < count) ok = fetch_next(i + 2);
         }
     } else {
         fewer_registers<REST_REGS>();
-        if (warp == 8 && lane == 0) {
+        if (warp == 12 && lane == 0) {
             // ---- copies ------------------------------------------------------------------------------------------
             const int tile_a = BWD ? a.rec.kt() : a.rec.w(), square_a = BWD ? a.rec.p() : a.rec.t();
             const int tile_b = BWD ? a.rec.w() : a.rec.kt(), square_e = BWD ? a.rec.t() : a.rec.p();
@@ -462,17 +478,19 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 mbar_wait_bounded(&full_c, (done_b - 1) & 1, a.status);
                 mbar_wait_bounded(&full_e, (done_b - 1) & 1, a.status);
             }
-        } else if (warp == 9 && lane == 0) {
+        } else if (warp == 13 && lane == 0) {
             // ---- MMAs --------------------------------------------------------------------------------------------
             const uint32_t base = smem_addr(sm);
             auto wait = [&](uint64_t* bar, uint32_t ph) { return mbar_wait_bounded(bar, ph, a.status); };
             for (int i = 0; i < count; ++i) {
                 const uint32_t ph = i & 1, X = tm + (ph ? kY : kX), Y = tm + (ph ? kX : kY);
                 const uint32_t ta = base + Smem::kA + ph * (TILE + SQUARE);
-                if (!wait(&full_a[ph], (i >> 1) & 1) || !wait(&v_ready, ph) || (i && !wait(&o_free, ph ^ 1)) || !wait(&s_ready, ph)) break;
+                if (!wait(&full_a[ph], (i >> 1) & 1) || !wait(&v_ready, ph) || (i && !wait(&o_free, ph ^ 1))) break;
+                tc_after();
+                product<C, C / 16, BWD>(tm + kAcc2, tm + kVal, ta + TILE, SQ_LO);       // no state in it
+                if (!wait(&s_ready, ph)) break;
                 tc_after();
                 product<C, KEY / 16, false>(tm + kAcc, X, ta, LO);
-                product<C, C / 16, BWD>(tm + kAcc2, tm + kVal, ta + TILE, SQ_LO);
                 commit(&v_done);
                 commit(&empty_a[ph]);
                 if (BWD) {
@@ -503,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == 9) tmem_dealloc512(tm);
+    if (warp == 13) tmem_dealloc512(tm);
 }
 
 template <typename T, int KEY, bool BWD>
@@ -534,7 +552,7 @@ cudaError_t launch_delta_scan(const aussm_b200_delta_t& p, const DeltaPlan& plan
                               cudaStream_t st) {
     ScanParams a = {};
     a.p = p; a.records = static_cast<const uint8_t*>(io.records); a.rec = plan.rec; a.n = plan.n;
-    a.v = io.v; a.s0 = io.s0; a.s1 = io.s1; a.out = io.out; a.rows = io.rows; a.states = io.states;
+    a.v = io.v; a.s0 = io.s0; a.s1 = io.s1; a.out = io.out; a.rows = static_cast<uint4*>(io.rows); a.states = static_cast<uint4*>(io.states);
     for (int i = 0; i < 3; ++i) a.v_stride[i] = backward ? p.go_stride[i] : p.v_stride[i];
     a.status = device_status_ptr();
     if (!a.status) return cudaErrorUnknown;
