@@ -64,14 +64,24 @@ __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-__device__ __forceinline__ void commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+// The issuing warp runs as one, so that addresses and descriptors stay in uniform registers; `one` is set in the lane that
+// issues.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t one) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 ::"r"(smem_addr(bar)), "r"(one) : "memory");
 }
 // A from tensor memory, B from shared memory
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+template <bool ACCUMULATE>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t one) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "n"(ACCUMULATE ? 1 : 0), "r"(one) : "memory");
 }
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -109,17 +119,17 @@ __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn) {
 // MN: B's rows (64 of 128 bytes a panel) are the contraction and N runs along them, in panels of 64; otherwise the rows
 // are N and the contraction runs along them.
 template <int N, int STEPS, bool MN>
-__device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, int b_lo) {
+__device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, int b_lo, uint32_t one) {
     constexpr uint32_t id = idesc(N, MN);
     constexpr uint32_t A_LO = STEPS * 8;
     const uint64_t first = row_desc(b, MN ? 8192 : 16);
-    const uint32_t lo = (uint32_t)b_lo >> 4;
-#pragma unroll 1
+#pragma unroll
     for (int k = 0; k < STEPS; ++k) {
-        const uint64_t bh = first + (uint32_t)((MN ? k * 2048 : (k >> 2) * 8192 + (k & 3) * 32) >> 4), bl = bh + lo;
-        mma_ts(d, a + A_LO + k * 8, bh, id, k > 0);
-        mma_ts(d, a + k * 8, bl, id, 1);
-        mma_ts(d, a + k * 8, bh, id, 1);
+        const uint64_t bh = first + (uint32_t)((MN ? k * 2048 : (k >> 2) * 8192 + (k & 3) * 32) >> 4), bl = bh + (uint32_t)(b_lo >> 4);
+        if (k == 0) mma_ts<false>(d, a + A_LO, bh, id, one);
+        else mma_ts<true>(d, a + A_LO + k * 8, bh, id, one);
+        mma_ts<true>(d, a + k * 8, bl, id, one);
+        mma_ts<true>(d, a + k * 8, bh, id, one);
     }
 }
 
@@ -153,9 +163,17 @@ __device__ __forceinline__ float row_max(const float2 (&x)[COUNT]) {
     return fmaxf(m0, m1);
 }
 
+// mbar_wait_bounded as a loop of one poll (25 unrolled ones were 65 KB of the kernel's code)
+__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity, int* status) {
+#pragma unroll 1
+    for (uint32_t it = 0; it < (1u << 22); ++it)
+        if (mbar_try_wait(bar, parity)) return true;
+    atomicExch(status, kStatusBarrierTimeout);
+    return false;
+}
 // the same answer in all lanes: what follows is executed by whole warps
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status) {
-    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, status));
+    return __all_sync(0xffffffffu, poll(bar, parity, status));
 }
 
 template <typename T, int KEY>
@@ -302,6 +320,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         T* dst = static_cast<T*>(a.out) + ((long long)b * p.L * p.HV + h) * p.DV + v;
         T* tile = reinterpret_cast<T*>(sm + Smem::kV);
         const int width = min(128, p.DV - (int)blockIdx.y * 128);
+        const long long out_step = (long long)p.HV * p.DV;
         // rows of chunk i to shared memory, [64][128]: 16-byte pieces in flight, or each lane its own column
         auto fetch = [&](int i) {
             const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
@@ -359,13 +378,6 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             arrive(&v_ready);
             return true;
         };
-        // the tile is free when all lanes have read chunk i - 1 from it
-        auto fetch_next = [&](int i) {
-            arrive(&v_read);
-            if (!warp_wait(&v_read, (i - 1) & 1, a.status)) return false;
-            fetch(i);
-            return true;
-        };
         // `words` columns of tensor memory, 16 bytes a lane and store: [words / 4][128 lanes]
         auto dump = [&](uint32_t t, int words, uint4* to) {
             to += me;
@@ -380,69 +392,67 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             }
         };
         fetch(0);
-        bool ok = hand_over(0) && (count < 2 || fetch_next(1));
-        for (int i = 0; ok && i < count; ++i) {
+        for (int i = -1; i < count; ++i) {
             const uint32_t ph = i & 1;
+            // chunk i's products with V are done: the next chunk's parts go in, and the one's after it on their way
+            if (i + 1 < count) {
+                if (i >= 0) {
+                    if (!warp_wait(BWD ? &a_done : &v_done, ph, a.status) || !warp_wait(&n_ready, ph, a.status)) break;
+                    tc_after();
+                }
+                if (!hand_over(i + 1)) break;
+                if (i + 2 < count) {
+                    arrive(&v_read);
+                    if (!warp_wait(&v_read, ph ^ 1, a.status)) break;        // all lanes have read their rows
+                    fetch(i + 2);
+                }
+            }
+            if (i < 0) continue;
             const float* head = reinterpret_cast<const float*>(record(i));
             const float unq = head[kUnQ], un2 = head[BWD ? kUnT : kUnP];
-            const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
+            const int t0 = chunk_at(i) * C, rows = mine ? min(C, p.L - t0) : 0;
             const size_t at = ((size_t)bh * a.n + chunk_at(i)) * gridDim.y + blockIdx.y;
-            // the products with this chunk's V are done: the next one's parts go in
-            if (i + 1 < count) {
-                if (!warp_wait(BWD ? &a_done : &v_done, ph, a.status) || !warp_wait(&n_ready, ph, a.status)) break;
-                tc_after();
-                if (!hand_over(i + 1)) break;
-            }
             if (!warp_wait(&n_ready, ph, a.status) || !warp_wait(&o_done, ph, a.status)) break;
             tc_after();
             const float uns = un_s[ph][me], f1 = uns * unq, unn = un_n[me], f2 = unn * un2;
-            float y[C];
-#pragma unroll
+            T* to = dst + (long long)t0 * p.HV * p.DV;
+#pragma unroll 1
             for (int t = 0; t < C; t += 16) {
                 uint32_t r1[16], r2[16];
+                float y[16];
                 if (!BWD) tmem_ld16(lanes + kAcc + t, r1);
                 tmem_ld16(lanes + kAcc2 + t, r2);
                 tc_wait_ld();
 #pragma unroll
                 for (int u = 0; u < 16; ++u)
-                    y[t + u] = BWD ? __uint_as_float(r2[u]) * f2 : fmaf(__uint_as_float(r1[u]), f1, __uint_as_float(r2[u]) * f2);
+                    y[u] = BWD ? __uint_as_float(r2[u]) * f2 : fmaf(__uint_as_float(r1[u]), f1, __uint_as_float(r2[u]) * f2);
+                if (BWD) {
+                    float4* keep = reinterpret_cast<float4*>(a.rows) + at * (C / 4 * 128) + t / 4 * 128 + me;
+#pragma unroll
+                    for (int u = 0; u < 16; u += 4) {
+                        if (mine) keep[u / 4 * 128] = make_float4(y[u], y[u + 1], y[u + 2], y[u + 3]);
+                        const float4 be = *reinterpret_cast<const float4*>(head + kBeta + t + u);
+                        y[u] *= be.x; y[u + 1] *= be.y; y[u + 2] *= be.z; y[u + 3] *= be.w;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 16; ++u, to += out_step)
+                    if (t + u < rows) *to = from_f32<T>(y[u]);
             }
             tc_before();
             arrive(&o_free);
             if (a.states) {
-                uint4* to = a.states + at * (KEY / 4 * 128 + 32);
-                dump(lanes + (ph ? kY : kX), KEY, to);
-                reinterpret_cast<float*>(to + KEY / 4 * 128)[me] = uns;
+                uint4* st = a.states + at * (KEY / 4 * 128 + 32);
+                dump(lanes + (ph ? kY : kX), KEY, st);
+                reinterpret_cast<float*>(st + KEY / 4 * 128)[me] = uns;
             }
             if (!BWD && a.rows) {
-                uint4* to = a.rows + at * (C / 4 * 128 + 32);
-                dump(lanes + kNew, C, to);
-                reinterpret_cast<float*>(to + C / 4 * 128)[me] = unn;
+                uint4* st = a.rows + at * (C / 4 * 128 + 32);
+                dump(lanes + kNew, C, st);
+                reinterpret_cast<float*>(st + C / 4 * 128)[me] = unn;
             }
             tc_before();
             arrive(&x_free);
-            if (mine) {
-                if (BWD) {
-                    float4* to = reinterpret_cast<float4*>(a.rows) + at * (C / 4 * 128) + me;
-#pragma unroll
-                    for (int t = 0; t < C; t += 4) {
-                        to[t / 4 * 128] = make_float4(y[t], y[t + 1], y[t + 2], y[t + 3]);
-                        const float4 be = *reinterpret_cast<const float4*>(head + kBeta + t);
-                        y[t] *= be.x; y[t + 1] *= be.y; y[t + 2] *= be.z; y[t + 3] *= be.w;
-                    }
-                }
-                T* to = dst + (long long)t0 * p.HV * p.DV;
-                const long long step = (long long)p.HV * p.DV;
-                if (rows == C) {
-#pragma unroll
-                    for (int t = 0; t < C; ++t, to += step) *to = from_f32<T>(y[t]);
-                } else {
-#pragma unroll
-                    for (int t = 0; t < C; ++t, to += step)
-                        if (t < rows) *to = from_f32<T>(y[t]);
-                }
-            }
-            if (i + 2 < count) ok = fetch_next(i + 2);
         }
     } else {
         fewer_registers<REST_REGS>();
@@ -454,14 +464,14 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             for (int i = 0; i < count; ++i) {
                 const uint8_t* rec = record(i);
                 const int st = i & 1;
-                if (i >= 2 && !mbar_wait_bounded(&empty_a[st], ((i >> 1) - 1) & 1, a.status)) break;
+                if (i >= 2 && !poll(&empty_a[st], ((i >> 1) - 1) & 1, a.status)) break;
                 uint8_t* to = sm + Smem::kA + st * (TILE + SQUARE);
                 mbar_arrive_expect_tx(&full_a[st], TILE + SQUARE);
                 bulk_g2s(to, rec + tile_a, TILE, &full_a[st]);
                 bulk_g2s(to + TILE, rec + square_a, SQUARE, &full_a[st]);
                 done_a = i + 1;
-                if (i >= 1 && (!mbar_wait_bounded(&empty_b, (i - 1) & 1, a.status) || !mbar_wait_bounded(&empty_c, (i - 1) & 1, a.status) ||
-                               !mbar_wait_bounded(&empty_e, (i - 1) & 1, a.status)))
+                if (i >= 1 && (!poll(&empty_b, (i - 1) & 1, a.status) || !poll(&empty_c, (i - 1) & 1, a.status) ||
+                               !poll(&empty_e, (i - 1) & 1, a.status)))
                     break;
                 mbar_arrive_expect_tx(&full_b, TILE);
                 bulk_g2s(sm + Smem::kB, rec + tile_b, TILE, &full_b);
@@ -472,49 +482,49 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 done_b = i + 1;
             }
             // no copy may be in flight when the block ends, also not when a wait ran out
-            for (int i = max(0, done_a - 2); i < done_a; ++i) mbar_wait_bounded(&full_a[i & 1], (i >> 1) & 1, a.status);
+            for (int i = max(0, done_a - 2); i < done_a; ++i) poll(&full_a[i & 1], (i >> 1) & 1, a.status);
             if (done_b) {
-                mbar_wait_bounded(&full_b, (done_b - 1) & 1, a.status);
-                mbar_wait_bounded(&full_c, (done_b - 1) & 1, a.status);
-                mbar_wait_bounded(&full_e, (done_b - 1) & 1, a.status);
+                poll(&full_b, (done_b - 1) & 1, a.status);
+                poll(&full_c, (done_b - 1) & 1, a.status);
+                poll(&full_e, (done_b - 1) & 1, a.status);
             }
-        } else if (warp == 13 && lane == 0) {
+        } else if (warp == 13) {
             // ---- MMAs --------------------------------------------------------------------------------------------
-            const uint32_t base = smem_addr(sm);
-            auto wait = [&](uint64_t* bar, uint32_t ph) { return mbar_wait_bounded(bar, ph, a.status); };
+            const uint32_t base = smem_addr(sm), one = elect_one(), tm = __shfl_sync(0xffffffffu, holder, 0);
+            auto wait = [&](uint64_t* bar, uint32_t ph) { return warp_wait(bar, ph, a.status); };
             for (int i = 0; i < count; ++i) {
                 const uint32_t ph = i & 1, X = tm + (ph ? kY : kX), Y = tm + (ph ? kX : kY);
                 const uint32_t ta = base + Smem::kA + ph * (TILE + SQUARE);
                 if (!wait(&full_a[ph], (i >> 1) & 1) || !wait(&v_ready, ph) || (i && !wait(&o_free, ph ^ 1))) break;
                 tc_after();
-                product<C, C / 16, BWD>(tm + kAcc2, tm + kVal, ta + TILE, SQ_LO);       // no state in it
+                product<C, C / 16, BWD>(tm + kAcc2, tm + kVal, ta + TILE, SQ_LO, one);       // no state in it
                 if (!wait(&s_ready, ph)) break;
                 tc_after();
-                product<C, KEY / 16, false>(tm + kAcc, X, ta, LO);
-                commit(&v_done);
-                commit(&empty_a[ph]);
+                product<C, KEY / 16, false>(tm + kAcc, X, ta, LO, one);
+                commit(&v_done, one);
+                commit(&empty_a[ph], one);
                 if (BWD) {
                     if (!wait(&full_c, ph) || (i && !wait(&x_free, ph ^ 1))) break;
-                    product<KEY, C / 16, true>(Y, tm + kVal, base + Smem::kC, LO);
-                    commit(&a_done);
-                    commit(&empty_c);
+                    product<KEY, C / 16, true>(Y, tm + kVal, base + Smem::kC, LO, one);
+                    commit(&a_done, one);
+                    commit(&empty_c, one);
                     if (!wait(&y_free, ph)) break;
                 }
                 // Y held the parts of the state before this one: they have been taken out
                 if (!wait(&full_b, ph) || !wait(&n_ready, ph) || (i && !wait(&x_free, ph ^ 1))) break;
                 tc_after();
-                product<KEY, C / 16, true>(Y, tm + kNew, base + Smem::kB, LO);
-                commit(&d_done);
-                commit(&empty_b);
+                product<KEY, C / 16, true>(Y, tm + kNew, base + Smem::kB, LO, one);
+                commit(&d_done, one);
+                commit(&empty_b, one);
                 if (!BWD) {
                     if (!wait(&full_c, ph)) break;
-                    product<C, KEY / 16, false>(tm + kAcc, X, base + Smem::kC, LO);
-                    commit(&empty_c);
+                    product<C, KEY / 16, false>(tm + kAcc, X, base + Smem::kC, LO, one);
+                    commit(&empty_c, one);
                 }
                 if (!wait(&full_e, ph)) break;
-                product<C, C / 16, BWD>(tm + kAcc2, tm + kNew, base + Smem::kE, SQ_LO);
-                commit(&o_done);
-                commit(&empty_e);
+                product<C, C / 16, BWD>(tm + kAcc2, tm + kNew, base + Smem::kE, SQ_LO, one);
+                commit(&o_done, one);
+                commit(&empty_e, one);
             }
         }
     }
