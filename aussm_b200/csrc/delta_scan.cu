@@ -9,9 +9,9 @@
 // A row's FP16 parts are scaled by a power of two of the row's own: no reduction between threads.
 //
 // Warps 0-7 own the state, two threads a row, each half of its columns (the chain: convert S, product, convert V',
-// product, add); warps 8-11 bring V (dO) in (a chunk ahead, through shared memory) and everything out (O or X; the parts of
-// S and V' that a backward pass reads, as they lie in tensor memory); warp 12 copies the records' tiles (bulk copies),
-// warp 13 issues the MMAs (14 and 15 fill their warpgroup, which hands its registers to the others).  Tensor memory, 512
+// product, add); warps 8-11 bring V (dO) in, a chunk ahead, through shared memory; warps 12-15 take everything out (O or X;
+// the parts of S and V' that a backward pass reads, as they lie in tensor memory); warp 16 copies the records' tiles (bulk
+// copies), warp 17 issues the MMAs (18 and 19 fill their warpgroup, which hands its registers to the others).  Tensor memory, 512
 // columns: [X | Y] take turns as the parts of S and as the product that updates it, two accumulators of 64 columns, the
 // parts of V' and of V.  Every wait is bounded: one that runs out sets the status word and the block ends.
 //
@@ -26,9 +26,9 @@ namespace aussm {
 namespace {
 
 constexpr int C = kDeltaChunk;
-constexpr int THREADS = 512;             // four warpgroups; launched with 128 registers a thread, 512 for one of each
-constexpr int MAIN_REGS = 152, SIDE_REGS = 136, REST_REGS = 72;
-static_assert(2 * MAIN_REGS + SIDE_REGS + REST_REGS <= 4 * 128, "more registers than the block is launched with");
+constexpr int THREADS = 640;             // five warpgroups; launched with 96 registers a thread, 480 for one of each
+constexpr int MAIN_REGS = 136, IN_REGS = 64, OUT_REGS = 104, REST_REGS = 40;
+static_assert(2 * MAIN_REGS + IN_REGS + OUT_REGS + REST_REGS <= 5 * 96, "more registers than the block is launched with");
 constexpr int SQUARE = DeltaRecord::kSquare;
 // tensor memory columns
 constexpr uint32_t kX = 0, kY = 128, kAcc = 256, kAcc2 = 320, kNew = 384, kVal = 448;
@@ -154,13 +154,15 @@ __device__ __forceinline__ void store_parts(uint32_t t, uint32_t lo_cols, const 
 }
 template <int COUNT>
 __device__ __forceinline__ float row_max(const float2 (&x)[COUNT]) {
-    float m0 = 0.f, m1 = 0.f;
+    float m[4] = {};
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) {
-        m0 = fmaxf(m0, fabsf(x[i].x));
-        m1 = fmaxf(m1, fabsf(x[i].y));
+    for (int i = 0; i < COUNT; i += 2) {
+        m[0] = fmaxf(m[0], fabsf(x[i].x));
+        m[1] = fmaxf(m[1], fabsf(x[i].y));
+        m[2] = fmaxf(m[2], fabsf(x[i + 1].x));
+        m[3] = fmaxf(m[3], fabsf(x[i + 1].y));
     }
-    return fmaxf(m0, m1);
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
 // mbar_wait_bounded as a loop of one poll (25 unrolled ones were 65 KB of the kernel's code)
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     const aussm_b200_delta_t& p = a.p;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int bh = blockIdx.x, b = bh / p.HV, h = bh % p.HV;
-    const int me = threadIdx.x & 127, v = blockIdx.y * 128 + me;      // row (value column) of the threads of warps 0-11
+    const int me = threadIdx.x & 127, v = blockIdx.y * 128 + me;      // row (value column) of the threads of warps 0-15
     const bool mine = v < p.DV;
     const int count = a.n;                                            // chunks this block walks
     auto chunk_at = [&](int i) { return BWD ? a.n - 1 - i : i; };
@@ -218,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         fence_mbar_init();
         fence_proxy_async();
     }
-    if (warp == 13) tmem_alloc512(&holder);
+    if (warp == 17) tmem_alloc512(&holder);
     tc_before();
     __syncthreads();
     tc_after();
@@ -314,27 +316,30 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             }
         }
     } else if (warp < 12) {
-        // ---- V (dO) in; O (X), states and V' out -----------------------------------------------------------------
-        more_registers<SIDE_REGS>();
+        // ---- V (dO) in -------------------------------------------------------------------------------------------
+        fewer_registers<IN_REGS>();
         const T* src = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + blockIdx.y * 128;
-        T* dst = static_cast<T*>(a.out) + ((long long)b * p.L * p.HV + h) * p.DV + v;
         T* tile = reinterpret_cast<T*>(sm + Smem::kV);
         const int width = min(128, p.DV - (int)blockIdx.y * 128);
-        const long long out_step = (long long)p.HV * p.DV;
         // rows of chunk i to shared memory, [64][128]: 16-byte pieces in flight, or each lane its own column
         auto fetch = [&](int i) {
             const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
             const T* from = src + (long long)t0 * a.v_stride[1];
             if (me < C / 4) cp_async16(betas + 4 * me, reinterpret_cast<const float*>(record(i)) + kBeta + 4 * me);
             if (a.vec_v) {
-                constexpr int E = 16 / (int)sizeof(T), PIECES = 128 / E;
-#pragma unroll 1
-                for (int x = me; x < C * PIECES; x += 128) {
-                    const int row = x / PIECES, col = x % PIECES * E;
-                    if (row < rows && col < width) cp_async16(tile + row * 128 + col, from + row * a.v_stride[1] + col);
+                constexpr int E = 16 / (int)sizeof(T), PIECES = 128 / E, ROWS = 128 / PIECES;      // rows an instruction
+                int row = me / PIECES;
+                const int col = me % PIECES * E;
+                const T* at = from + row * a.v_stride[1] + col;
+                uint32_t to = smem_addr(tile + row * 128 + col);
+#pragma unroll 2
+                for (; row < rows && col < width; row += ROWS) {
+                    cp_async16_s(to, at);
+                    at += ROWS * a.v_stride[1];
+                    to += ROWS * 128 * (uint32_t)sizeof(T);
                 }
             } else if (mine) {
-#pragma unroll 8
+#pragma unroll 4
                 for (int row = 0; row < rows; ++row) tile[row * 128 + me] = from[row * a.v_stride[1] + me];
             }
             cp_async_commit();
@@ -378,6 +383,27 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             arrive(&v_ready);
             return true;
         };
+        fetch(0);
+        for (int i = 0; i < count; ++i) {
+            // the products with chunk i - 1 are done: this one's parts go in, and the next rows are on their way
+            if (i) {
+                const uint32_t ph = (i - 1) & 1;
+                if (!warp_wait(BWD ? &a_done : &v_done, ph, a.status) || !warp_wait(&n_ready, ph, a.status)) break;
+                tc_after();
+            }
+            if (!hand_over(i)) break;
+            if (i + 1 < count) {
+                arrive(&v_read);
+                if (!warp_wait(&v_read, i & 1, a.status)) break;             // all lanes have read their rows
+                fetch(i + 1);
+            }
+        }
+        cp_async_wait<0>();
+    } else if (warp < 16) {
+        // ---- O (X), states and V' out ------------------------------------------------------------------------------
+        more_registers<OUT_REGS>();
+        T* dst = static_cast<T*>(a.out) + ((long long)b * p.L * p.HV + h) * p.DV + v;
+        const long long out_step = (long long)p.HV * p.DV;
         // `words` columns of tensor memory, 16 bytes a lane and store: [words / 4][128 lanes]
         auto dump = [&](uint32_t t, int words, uint4* to) {
             to += me;
@@ -391,23 +417,8 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                     if (mine) to[(x / 4 + z) * 128] = make_uint4(r[4 * z], r[4 * z + 1], r[4 * z + 2], r[4 * z + 3]);
             }
         };
-        fetch(0);
-        for (int i = -1; i < count; ++i) {
+        for (int i = 0; i < count; ++i) {
             const uint32_t ph = i & 1;
-            // chunk i's products with V are done: the next chunk's parts go in, and the one's after it on their way
-            if (i + 1 < count) {
-                if (i >= 0) {
-                    if (!warp_wait(BWD ? &a_done : &v_done, ph, a.status) || !warp_wait(&n_ready, ph, a.status)) break;
-                    tc_after();
-                }
-                if (!hand_over(i + 1)) break;
-                if (i + 2 < count) {
-                    arrive(&v_read);
-                    if (!warp_wait(&v_read, ph ^ 1, a.status)) break;        // all lanes have read their rows
-                    fetch(i + 2);
-                }
-            }
-            if (i < 0) continue;
             const float* head = reinterpret_cast<const float*>(record(i));
             const float unq = head[kUnQ], un2 = head[BWD ? kUnT : kUnP];
             const int t0 = chunk_at(i) * C, rows = mine ? min(C, p.L - t0) : 0;
@@ -415,32 +426,34 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             if (!warp_wait(&n_ready, ph, a.status) || !warp_wait(&o_done, ph, a.status)) break;
             tc_after();
             const float uns = un_s[ph][me], f1 = uns * unq, unn = un_n[me], f2 = unn * un2;
-            T* to = dst + (long long)t0 * p.HV * p.DV;
-#pragma unroll 1
+            // all of it to registers first: the accumulators are wanted back
+            float y[C];
+#pragma unroll
             for (int t = 0; t < C; t += 16) {
                 uint32_t r1[16], r2[16];
-                float y[16];
                 if (!BWD) tmem_ld16(lanes + kAcc + t, r1);
                 tmem_ld16(lanes + kAcc2 + t, r2);
                 tc_wait_ld();
 #pragma unroll
                 for (int u = 0; u < 16; ++u)
-                    y[u] = BWD ? __uint_as_float(r2[u]) * f2 : fmaf(__uint_as_float(r1[u]), f1, __uint_as_float(r2[u]) * f2);
-                if (BWD) {
-                    float4* keep = reinterpret_cast<float4*>(a.rows) + at * (C / 4 * 128) + t / 4 * 128 + me;
-#pragma unroll
-                    for (int u = 0; u < 16; u += 4) {
-                        if (mine) keep[u / 4 * 128] = make_float4(y[u], y[u + 1], y[u + 2], y[u + 3]);
-                        const float4 be = *reinterpret_cast<const float4*>(head + kBeta + t + u);
-                        y[u] *= be.x; y[u + 1] *= be.y; y[u + 2] *= be.z; y[u + 3] *= be.w;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < 16; ++u, to += out_step)
-                    if (t + u < rows) *to = from_f32<T>(y[u]);
+                    y[t + u] = BWD ? __uint_as_float(r2[u]) * f2 : fmaf(__uint_as_float(r1[u]), f1, __uint_as_float(r2[u]) * f2);
             }
             tc_before();
             arrive(&o_free);
+            T* to = dst + (long long)t0 * p.HV * p.DV;
+            if (BWD && mine) {
+                float4* keep = reinterpret_cast<float4*>(a.rows) + at * (C / 4 * 128) + me;
+                const float4* be = reinterpret_cast<const float4*>(head + kBeta);
+#pragma unroll
+                for (int t = 0; t < C; t += 4) {
+                    keep[t / 4 * 128] = make_float4(y[t], y[t + 1], y[t + 2], y[t + 3]);
+                    const float4 f = be[t / 4];
+                    y[t] *= f.x; y[t + 1] *= f.y; y[t + 2] *= f.z; y[t + 3] *= f.w;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < C; ++t, to += out_step)
+                if (t < rows) *to = from_f32<T>(y[t]);
             if (a.states) {
                 uint4* st = a.states + at * (KEY / 4 * 128 + 32);
                 dump(lanes + (ph ? kY : kX), KEY, st);
@@ -456,7 +469,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         }
     } else {
         fewer_registers<REST_REGS>();
-        if (warp == 12 && lane == 0) {
+        if (warp == 16 && lane == 0) {
             // ---- copies ------------------------------------------------------------------------------------------
             const int tile_a = BWD ? a.rec.kt() : a.rec.w(), square_a = BWD ? a.rec.p() : a.rec.t();
             const int tile_b = BWD ? a.rec.w() : a.rec.kt(), square_e = BWD ? a.rec.t() : a.rec.p();
@@ -488,7 +501,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 poll(&full_c, (done_b - 1) & 1, a.status);
                 poll(&full_e, (done_b - 1) & 1, a.status);
             }
-        } else if (warp == 13) {
+        } else if (warp == 17) {
             // ---- MMAs --------------------------------------------------------------------------------------------
             const uint32_t base = smem_addr(sm), one = elect_one(), tm = __shfl_sync(0xffffffffu, holder, 0);
             auto wait = [&](uint64_t* bar, uint32_t ph) { return warp_wait(bar, ph, a.status); };
@@ -510,18 +523,18 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                     commit(&empty_c, one);
                     if (!wait(&y_free, ph)) break;
                 }
-                // Y held the parts of the state before this one: they have been taken out
-                if (!wait(&full_b, ph) || !wait(&n_ready, ph) || (i && !wait(&x_free, ph ^ 1))) break;
+                // Y held the parts of the state before this one: they have been taken out.  V' comes last.
+                if (!wait(&full_b, ph) || !wait(&full_e, ph) || (!BWD && !wait(&full_c, ph)) || (i && !wait(&x_free, ph ^ 1)) ||
+                    !wait(&n_ready, ph))
+                    break;
                 tc_after();
                 product<KEY, C / 16, true>(Y, tm + kNew, base + Smem::kB, LO, one);
                 commit(&d_done, one);
                 commit(&empty_b, one);
                 if (!BWD) {
-                    if (!wait(&full_c, ph)) break;
                     product<C, KEY / 16, false>(tm + kAcc, X, base + Smem::kC, LO, one);
                     commit(&empty_c, one);
                 }
-                if (!wait(&full_e, ph)) break;
                 product<C, C / 16, BWD>(tm + kAcc2, tm + kNew, base + Smem::kE, SQ_LO, one);
                 commit(&o_done, one);
                 commit(&empty_e, one);
@@ -531,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == 13) tmem_dealloc512(tm);
+    if (warp == 17) tmem_dealloc512(tm);
 }
 
 template <typename T, int KEY, bool BWD>
