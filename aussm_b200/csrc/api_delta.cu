@@ -65,7 +65,7 @@ size_t aussm_b200_delta_keep_bytes(const aussm_b200_delta_t* p) {
 
 size_t aussm_b200_delta_workspace_bytes(const aussm_b200_delta_t* p, int backward) {
     if (delta_check("delta_workspace_bytes", p)) return 0;
-    return backward ? delta_plan(*p).bwd_bytes : delta_plan(*p).news;     // without a backward pass only the records
+    return backward ? delta_plan(*p).bwd_bytes : delta_plan(*p).fwd_bytes;
 }
 
 int aussm_b200_delta_fwd(const aussm_b200_delta_t* p, const void* q, const void* k, const void* v, const float* g,

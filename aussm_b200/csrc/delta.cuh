@@ -96,18 +96,25 @@ __device__ __forceinline__ float clamp_log_decay(float g) { return g < -200.f ? 
 // 4 words of hi parts, then the lo parts), V': 64 words (8 steps in 4 words), and behind them the lanes' float32 factors.
 // X: 64 float32 words a lane.
 //
-// Sizes and buffers of a problem.  keep: [records][V'][entry states], backward workspace: [X][gradients of exit states]
+// Sizes and buffers of a problem.  keep: [records][transitions][ends][V'][entry states] (the first three are the workspace
+// of a forward call without a backward one), backward workspace: [X][gradients of exit states][ends].
+//
+// Few heads leave most of the GPU idle: the chunks are then cut into `segs` segments of `span` that run side by side.  A pass
+// gives what a segment makes of a zero state and one what it does to a state (its transition, DK x DK; the backward pass
+// uses the transposed ones of the forward pass), a chain over the segments the states at their boundaries, and the pass
+// with all outputs starts every segment from its own.
 struct DeltaPlan {
     int n;                 // chunks of a sequence
     int slices;            // of 128 value columns
+    int segs, span;        // segments of the recurrences, chunks of one
     __host__ __device__ static size_t state_bytes(int key) { return (size_t)key * 512 + 512; }
     __host__ __device__ static size_t news_bytes() { return 64 * 512 + 512; }
     __host__ __device__ static size_t x_bytes() { return 64 * 512; }
     size_t heads;          // chunk heads: (b * HV + h) * n + chunk
     DeltaRecord rec;
-    size_t keep_bytes, bwd_bytes;
-    size_t news, states;   // byte offsets in keep
-    size_t dstates;        // byte offset in the backward workspace
+    size_t keep_bytes, fwd_bytes, bwd_bytes;
+    size_t transitions, ends, news, states;   // byte offsets in keep
+    size_t dstates, bwd_ends;                 // byte offsets in the backward workspace
 };
 DeltaPlan delta_plan(const aussm_b200_delta_t& p);
 
@@ -121,6 +128,7 @@ struct DeltaScan {
     float* s1;
     void* out;
     void *rows, *states;       // V' / X and entry states / gradients of exit states; forward: NULL = not kept
+    void *transitions, *ends;  // of the segments (forward writes the transitions, backward reads them)
 };
 cudaError_t launch_delta_scan(const aussm_b200_delta_t& p, const DeltaPlan& plan, const DeltaScan& io, bool backward,
                               cudaStream_t stream);

@@ -16,11 +16,25 @@ DeltaPlan delta_plan(const aussm_b200_delta_t& p) {
     d.rec.key = p.DK <= 64 ? 64 : 128;
     d.slices = (p.DV + 127) / 128;
     const size_t pieces = d.heads * d.slices;
-    d.news = d.heads * d.rec.bytes();
+    // A block of the recurrences takes an SM.
+    const long long blocks = (long long)p.B * p.HV * d.slices;
+    long long segs = 1;
+    if (blocks * 3 <= 148) {
+        segs = 148 / blocks;
+        if (segs > d.n / 4) segs = d.n / 4;
+        if (segs < 3) segs = 1;
+    }
+    d.span = (int)((d.n + segs - 1) / segs);
+    d.segs = (d.n + d.span - 1) / d.span;
+    const size_t bh = (size_t)p.B * p.HV, ends = d.segs > 1 ? up256((d.segs - 1) * bh * p.DK * p.DV * sizeof(float)) : 0;
+    d.transitions = d.heads * d.rec.bytes();
+    d.ends = d.transitions + (d.segs > 2 ? up256(d.segs * bh * p.DK * p.DK * sizeof(float)) : 0);
+    d.fwd_bytes = d.news = d.ends + ends;
     d.states = d.news + up256(pieces * DeltaPlan::news_bytes());
     d.keep_bytes = d.states + up256(pieces * DeltaPlan::state_bytes(d.rec.key));
     d.dstates = up256(pieces * DeltaPlan::x_bytes());
-    d.bwd_bytes = d.dstates + up256(pieces * DeltaPlan::state_bytes(d.rec.key));
+    d.bwd_ends = d.dstates + up256(pieces * DeltaPlan::state_bytes(d.rec.key));
+    d.bwd_bytes = d.bwd_ends + ends;
     return d;
 }
 
@@ -31,7 +45,7 @@ cudaError_t launch_delta_fwd(const aussm_b200_delta_t& p, const DeltaInputs& in,
     if (e != cudaSuccess) return e;
     uint8_t* k = static_cast<uint8_t*>(keep);
     void *news = train ? k + plan.news : nullptr, *states = train ? k + plan.states : nullptr;
-    return launch_delta_scan(p, plan, {keep, in.v, s0, s1, o, news, states}, false, st);
+    return launch_delta_scan(p, plan, {keep, in.v, s0, s1, o, news, states, k + plan.transitions, k + plan.ends}, false, st);
 }
 
 cudaError_t launch_delta_bwd(const aussm_b200_delta_t& p, const DeltaInputs& in, const void* go, const float* gs1,
@@ -40,7 +54,8 @@ cudaError_t launch_delta_bwd(const aussm_b200_delta_t& p, const DeltaInputs& in,
     const DeltaPlan plan = delta_plan(p);
     const uint8_t* k = static_cast<const uint8_t*>(keep);
     uint8_t* w = static_cast<uint8_t*>(workspace);
-    cudaError_t e = launch_delta_scan(p, plan, {keep, go, gs1, ds0, dv, w, w + plan.dstates}, true, st);
+    cudaError_t e = launch_delta_scan(p, plan, {keep, go, gs1, ds0, dv, w, w + plan.dstates,
+                                              const_cast<uint8_t*>(k) + plan.transitions, w + plan.bwd_ends}, true, st);
     if (e != cudaSuccess) return e;
     return launch_delta_grads(p, plan, in, {keep, go, k + plan.news, w, k + plan.states, w + plan.dstates, dq, dk, dg, dbeta}, st);
 }

@@ -43,6 +43,14 @@ struct ScanParams {
     const float* s0;                     // forward: initial state, backward: gradient of the final state (NULL = 0)
     float* s1;                           // forward: final state, backward: gradient of the initial state (NULL)
     void* out;                           // forward: O; backward: dV
+    // A block walks one of `segs` segments of `span` chunks (in the order of the walk the first is blockIdx.z +
+    // first_seg = 0; the boundaries are the forward walk's both ways).  Segment 0 starts from s0, segment z from seg_in + z
+    // * seg_stride (NULL: from zero) and leaves its last state at seg_out + z * seg_stride.
+    int span, segs, first_seg;
+    const float* seg_in;
+    float* seg_out;
+    size_t seg_stride;
+    int transition;                      // 1: V is zero and the state starts as the identity: what a segment does to a state
     uint4* rows;                         // forward: V' of every chunk (NULL = not kept); backward: X
     uint4* states;                       // forward: entry states (NULL); backward: gradients of the exit states
     int vec_v;                           // rows of v can be copied 16 bytes at a time
@@ -202,9 +210,12 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int bh = blockIdx.x, b = bh / p.HV, h = bh % p.HV;
     const int me = threadIdx.x & 127, v = blockIdx.y * 128 + me;      // row (value column) of the threads of warps 0-15
-    const bool mine = v < p.DV;
-    const int count = a.n;                                            // chunks this block walks
-    auto chunk_at = [&](int i) { return BWD ? a.n - 1 - i : i; };
+    const int width_all = a.transition ? p.DK : p.DV;                 // value columns (a transition: the state's own keys)
+    const bool mine = v < width_all;
+    const int seg = a.first_seg + (int)blockIdx.z, c0 = (BWD ? a.segs - 1 - seg : seg) * a.span;
+    const int count = min(a.span, a.n - c0);                          // chunks this block walks
+    const bool full = a.out != nullptr;                               // otherwise only the state at the end is wanted
+    auto chunk_at = [&](int i) { return BWD ? c0 + count - 1 - i : c0 + i; };
     auto record = [&](int i) { return a.records + ((size_t)bh * a.n + chunk_at(i)) * a.rec.bytes(); };
 
     if (threadIdx.x == 0) {
@@ -233,11 +244,17 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         const int half = warp >> 2;
         const uint32_t sc = half * HALF;                              // first column in a float32 row
         float2 s[HALF / 2];
+        const float* from = seg == 0 ? a.s0 : a.seg_in ? a.seg_in + seg * a.seg_stride : nullptr;
+        if (from) from += (size_t)bh * p.DK * p.DV + v;
 #pragma unroll
         for (int x = 0; x < HALF / 2; ++x) {
             const int k0 = sc + 2 * x;
-            const float* src = a.s0 + ((size_t)bh * p.DK + k0) * p.DV + v;
-            s[x] = make_float2(a.s0 && mine && k0 < p.DK ? src[0] : 0.f, a.s0 && mine && k0 + 1 < p.DK ? src[p.DV] : 0.f);
+            s[x] = make_float2(0.f, 0.f);
+            if (a.transition) s[x] = make_float2(k0 == me ? 1.f : 0.f, k0 + 1 == me ? 1.f : 0.f);
+            else if (from && mine) {
+                if (k0 < p.DK) s[x].x = from[(size_t)k0 * p.DV];
+                if (k0 + 1 < p.DK) s[x].y = from[(size_t)(k0 + 1) * p.DV];
+            }
         }
         // s = s * keep + r * f over the columns of a product
         auto add = [&](uint32_t t, float keep, float f) {
@@ -289,7 +306,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             if (!warp_wait(&pair_n[warp & 3], ph, a.status)) break;
             const int en = part_exponent(fmaxf(max_n[0][me], max_n[1][me]));
             const float unn = pow2_float(-en);
-            if (i && !warp_wait(&x_free, ph ^ 1, a.status)) break;      // the last V' has been taken out
+            if (full && i && !warp_wait(&x_free, ph ^ 1, a.status)) break;      // the last V' has been taken out
             store_parts<32>(lanes + kNew + half * 16, C / 2, w, pow2_float(en));
             if (half == 0) un_n[me] = unn;
             tc_wait_st();
@@ -306,13 +323,14 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             tc_after();
             add(Y, BWD ? 1.f : gamma, (BWD ? -unn : unn) * un3);
         }
-        if (a.s1 && mine) {
+        float* to = a.seg_out ? a.seg_out + seg * a.seg_stride : seg == a.segs - 1 ? a.s1 : nullptr;
+        if (to && mine) {
+            to += (size_t)bh * p.DK * width_all + v;
 #pragma unroll
             for (int x = 0; x < HALF / 2; ++x) {
                 const int k0 = sc + 2 * x;
-                float* dst = a.s1 + ((size_t)bh * p.DK + k0) * p.DV + v;
-                if (k0 < p.DK) dst[0] = s[x].x;
-                if (k0 + 1 < p.DK) dst[p.DV] = s[x].y;
+                if (k0 < p.DK) to[(size_t)k0 * width_all] = s[x].x;
+                if (k0 + 1 < p.DK) to[(size_t)(k0 + 1) * width_all] = s[x].y;
             }
         }
     } else if (warp < 12) {
@@ -320,7 +338,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         fewer_registers<IN_REGS>();
         const T* src = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + blockIdx.y * 128;
         T* tile = reinterpret_cast<T*>(sm + Smem::kV);
-        const int width = min(128, p.DV - (int)blockIdx.y * 128);
+        const int width = a.transition ? 0 : min(128, p.DV - (int)blockIdx.y * 128);
         // rows of chunk i to shared memory, [64][128]: 16-byte pieces in flight, or each lane its own column
         auto fetch = [&](int i) {
             const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
@@ -338,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                     at += ROWS * a.v_stride[1];
                     to += ROWS * 128 * (uint32_t)sizeof(T);
                 }
-            } else if (mine) {
+            } else if (me < width) {
 #pragma unroll 4
                 for (int row = 0; row < rows; ++row) tile[row * 128 + me] = from[row * a.v_stride[1] + me];
             }
@@ -346,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         };
         // chunk i's row of this lane from shared memory to the parts in tensor memory; false: a wait ran out
         auto hand_over = [&](int i) {
-            const int rows = mine ? min(C, p.L - chunk_at(i) * C) : 0;
+            const int rows = me < width ? min(C, p.L - chunk_at(i) * C) : 0;
             cp_async_wait<0>();
             arrive(&v_loaded);
             if (!warp_wait(&v_loaded, i & 1, a.status)) return false;
@@ -417,7 +435,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                     if (mine) to[(x / 4 + z) * 128] = make_uint4(r[4 * z], r[4 * z + 1], r[4 * z + 2], r[4 * z + 3]);
             }
         };
-        for (int i = 0; i < count; ++i) {
+        for (int i = 0; full && i < count; ++i) {
             const uint32_t ph = i & 1;
             const float* head = reinterpret_cast<const float*>(record(i));
             const float unq = head[kUnQ], un2 = head[BWD ? kUnT : kUnP];
@@ -483,23 +501,28 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 bulk_g2s(to, rec + tile_a, TILE, &full_a[st]);
                 bulk_g2s(to + TILE, rec + square_a, SQUARE, &full_a[st]);
                 done_a = i + 1;
-                if (i >= 1 && (!poll(&empty_b, (i - 1) & 1, a.status) || !poll(&empty_c, (i - 1) & 1, a.status) ||
-                               !poll(&empty_e, (i - 1) & 1, a.status)))
+                const bool c = full || BWD;                     // Qt: for O, or for the backward state
+                if (i >= 1 && (!poll(&empty_b, (i - 1) & 1, a.status) || (c && !poll(&empty_c, (i - 1) & 1, a.status)) ||
+                               (full && !poll(&empty_e, (i - 1) & 1, a.status))))
                     break;
                 mbar_arrive_expect_tx(&full_b, TILE);
                 bulk_g2s(sm + Smem::kB, rec + tile_b, TILE, &full_b);
-                mbar_arrive_expect_tx(&full_c, TILE);
-                bulk_g2s(sm + Smem::kC, rec + a.rec.q(), TILE, &full_c);
-                mbar_arrive_expect_tx(&full_e, SQUARE);
-                bulk_g2s(sm + Smem::kE, rec + square_e, SQUARE, &full_e);
+                if (c) {
+                    mbar_arrive_expect_tx(&full_c, TILE);
+                    bulk_g2s(sm + Smem::kC, rec + a.rec.q(), TILE, &full_c);
+                }
+                if (full) {
+                    mbar_arrive_expect_tx(&full_e, SQUARE);
+                    bulk_g2s(sm + Smem::kE, rec + square_e, SQUARE, &full_e);
+                }
                 done_b = i + 1;
             }
             // no copy may be in flight when the block ends, also not when a wait ran out
             for (int i = max(0, done_a - 2); i < done_a; ++i) poll(&full_a[i & 1], (i >> 1) & 1, a.status);
             if (done_b) {
                 poll(&full_b, (done_b - 1) & 1, a.status);
-                poll(&full_c, (done_b - 1) & 1, a.status);
-                poll(&full_e, (done_b - 1) & 1, a.status);
+                if (full || BWD) poll(&full_c, (done_b - 1) & 1, a.status);
+                if (full) poll(&full_e, (done_b - 1) & 1, a.status);
             }
         } else if (warp == 17) {
             // ---- MMAs --------------------------------------------------------------------------------------------
@@ -508,7 +531,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             for (int i = 0; i < count; ++i) {
                 const uint32_t ph = i & 1, X = tm + (ph ? kY : kX), Y = tm + (ph ? kX : kY);
                 const uint32_t ta = base + Smem::kA + ph * (TILE + SQUARE);
-                if (!wait(&full_a[ph], (i >> 1) & 1) || !wait(&v_ready, ph) || (i && !wait(&o_free, ph ^ 1))) break;
+                if (!wait(&full_a[ph], (i >> 1) & 1) || !wait(&v_ready, ph) || (full && i && !wait(&o_free, ph ^ 1))) break;
                 tc_after();
                 product<C, C / 16, BWD>(tm + kAcc2, tm + kVal, ta + TILE, SQ_LO, one);       // no state in it
                 if (!wait(&s_ready, ph)) break;
@@ -517,20 +540,21 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 commit(&v_done, one);
                 commit(&empty_a[ph], one);
                 if (BWD) {
-                    if (!wait(&full_c, ph) || (i && !wait(&x_free, ph ^ 1))) break;
+                    if (!wait(&full_c, ph) || (full && i && !wait(&x_free, ph ^ 1))) break;
                     product<KEY, C / 16, true>(Y, tm + kVal, base + Smem::kC, LO, one);
                     commit(&a_done, one);
                     commit(&empty_c, one);
                     if (!wait(&y_free, ph)) break;
                 }
                 // Y held the parts of the state before this one: they have been taken out.  V' comes last.
-                if (!wait(&full_b, ph) || !wait(&full_e, ph) || (!BWD && !wait(&full_c, ph)) || (i && !wait(&x_free, ph ^ 1)) ||
+                if (!wait(&full_b, ph) || (full && (!wait(&full_e, ph) || (!BWD && !wait(&full_c, ph)) || (i && !wait(&x_free, ph ^ 1)))) ||
                     !wait(&n_ready, ph))
                     break;
                 tc_after();
                 product<KEY, C / 16, true>(Y, tm + kNew, base + Smem::kB, LO, one);
                 commit(&d_done, one);
                 commit(&empty_b, one);
+                if (!full) continue;
                 if (!BWD) {
                     product<C, KEY / 16, false>(tm + kAcc, X, base + Smem::kC, LO, one);
                     commit(&empty_c, one);
@@ -547,26 +571,88 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     if (warp == 17) tmem_dealloc512(tm);
 }
 
+// States at the segments' boundaries, from what each segment makes of a zero state and what it does to a state:
+//     S_1 = N_0,   S_{z+1} = M_z S_z + N_z     (backward M^T of the mirrored segment),
+// S_{z+1} in the place of N_z.  A block owns 8 value columns of a head and keeps their states in shared memory; a thread
+// adds up 4 rows of one column in float32, M comes through the caches.
+constexpr int CHAIN_COLS = 8;
+__global__ void __launch_bounds__(256) delta_chain_kernel(const float* __restrict__ m, float* ends, int dk, int dv, int segs,
+                                                          size_t m_stride, size_t end_stride, bool backward) {
+    __shared__ float s[AUSSM_MAX_DELTA_KEY][CHAIN_COLS];
+    const int bh = blockIdx.x, v0 = blockIdx.y * CHAIN_COLS, col = threadIdx.x & 7, row = (threadIdx.x >> 3) * 4;
+    const bool mine = v0 + col < dv;
+    float* end = ends + (size_t)bh * dk * dv + v0 + col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[row + i][col] = mine && row + i < dk ? end[(size_t)(row + i) * dv] : 0.f;
+    __syncthreads();
+    for (int z = 1; z < segs - 1; ++z) {
+        const float* M = m + (size_t)(backward ? segs - 1 - z : z) * m_stride + (size_t)bh * dk * dk;
+        float* to = end + z * end_stride;
+        float acc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = mine && row + i < dk ? to[(size_t)(row + i) * dv] : 0.f;
+        const int down = backward ? 1 : dk, along = backward ? dk : 1;      // M or M^T
+#pragma unroll 16
+        for (int x = 0; x < dk; ++x) {
+            const float f = s[x][col];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (row + i < dk) acc[i] = fmaf(__ldg(M + (size_t)(row + i) * down + (size_t)x * along), f, acc[i]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[row + i][col] = acc[i];
+            if (mine && row + i < dk) to[(size_t)(row + i) * dv] = acc[i];
+        }
+        __syncthreads();
+    }
+}
+
 template <typename T, int KEY, bool BWD>
-cudaError_t scan(const ScanParams& a, cudaStream_t st) {
+cudaError_t scan(ScanParams a, const DeltaPlan& plan, float* m, float* ends, cudaStream_t st) {
     constexpr int smem = ScanSmem<T, KEY>::kBytes;
     cudaError_t e = cudaFuncSetAttribute(delta_scan_kernel<T, KEY, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    delta_scan_kernel<T, KEY, BWD><<<dim3(a.p.B * a.p.HV, (a.p.DV + 127) / 128), THREADS, smem, st>>>(a);
+    const int heads = a.p.B * a.p.HV, segs = plan.segs;
+    a.span = plan.span;
+    a.segs = segs;
+    if (segs > 1) {
+        const size_t m_stride = (size_t)heads * a.p.DK * a.p.DK, end_stride = (size_t)heads * a.p.DK * a.p.DV;
+        ScanParams q = a;
+        q.out = nullptr; q.rows = nullptr; q.states = nullptr;
+        if (!BWD && segs > 2) {              // what the segments between the first and the last do to a state
+            q.transition = 1; q.first_seg = 1; q.seg_out = m; q.seg_stride = m_stride;
+            delta_scan_kernel<T, KEY, BWD><<<dim3(heads, 1, segs - 2), THREADS, smem, st>>>(q);
+            count_launch();
+        }
+        q.transition = 0; q.first_seg = 0; q.seg_out = ends; q.seg_stride = end_stride;
+        delta_scan_kernel<T, KEY, BWD><<<dim3(heads, plan.slices, segs - 1), THREADS, smem, st>>>(q);
+        count_launch();
+        if (segs > 2) {
+            delta_chain_kernel<<<dim3(heads, (a.p.DV + CHAIN_COLS - 1) / CHAIN_COLS), 256, 0, st>>>(
+                m, ends, a.p.DK, a.p.DV, segs, m_stride, end_stride, BWD);
+            count_launch();
+        }
+        a.seg_in = ends - end_stride;        // segment z starts from the state behind segment z - 1
+        a.seg_stride = end_stride;
+    }
+    delta_scan_kernel<T, KEY, BWD><<<dim3(heads, plan.slices, segs), THREADS, smem, st>>>(a);
     count_launch();
     return cudaGetLastError();
 }
 template <typename T, bool BWD>
-cudaError_t scan_key(ScanParams& a, cudaStream_t st) {
+cudaError_t scan_key(ScanParams& a, const DeltaPlan& plan, float* m, float* ends, cudaStream_t st) {
     const long long* vs = a.v_stride;
     a.vec_v = reinterpret_cast<uintptr_t>(a.v) % 16 == 0 && vs[0] * sizeof(T) % 16 == 0 && vs[1] * sizeof(T) % 16 == 0 &&
               vs[2] * sizeof(T) % 16 == 0 && a.p.DV * sizeof(T) % 16 == 0;
-    return a.rec.key == 64 ? scan<T, 64, BWD>(a, st) : scan<T, 128, BWD>(a, st);
+    return a.rec.key == 64 ? scan<T, 64, BWD>(a, plan, m, ends, st) : scan<T, 128, BWD>(a, plan, m, ends, st);
 }
 template <bool BWD>
-cudaError_t scan_typed(ScanParams& a, cudaStream_t st) {
-    return a.p.dtype == AUSSM_FLOAT32 ? scan_key<float, BWD>(a, st)
-           : a.p.dtype == AUSSM_BFLOAT16 ? scan_key<__nv_bfloat16, BWD>(a, st) : scan_key<__half, BWD>(a, st);
+cudaError_t scan_typed(ScanParams& a, const DeltaPlan& plan, float* m, float* ends, cudaStream_t st) {
+    return a.p.dtype == AUSSM_FLOAT32 ? scan_key<float, BWD>(a, plan, m, ends, st)
+           : a.p.dtype == AUSSM_BFLOAT16 ? scan_key<__nv_bfloat16, BWD>(a, plan, m, ends, st)
+                                         : scan_key<__half, BWD>(a, plan, m, ends, st);
 }
 
 }  // namespace
@@ -579,7 +665,8 @@ cudaError_t launch_delta_scan(const aussm_b200_delta_t& p, const DeltaPlan& plan
     for (int i = 0; i < 3; ++i) a.v_stride[i] = backward ? p.go_stride[i] : p.v_stride[i];
     a.status = device_status_ptr();
     if (!a.status) return cudaErrorUnknown;
-    return backward ? scan_typed<true>(a, st) : scan_typed<false>(a, st);
+    float *m = static_cast<float*>(io.transitions), *ends = static_cast<float*>(io.ends);
+    return backward ? scan_typed<true>(a, plan, m, ends, st) : scan_typed<false>(a, plan, m, ends, st);
 }
 
 }  // namespace aussm

@@ -329,3 +329,9 @@ def test_streams_and_graph_replay():
         assert torch.equal(new, e["state"])
     with pytest.raises(RuntimeError, match="inplace"):      # the eager graph's inputs are gone, and torch says so
         torch.autograd.grad(alive.sum(), x["g"])
+
+
+@pytest.mark.parametrize("l,heads,dk,dv,rate", [(800, 1, 128, 128, 0.01), (1111, 3, 64, 64, 1e-3), (2500, 2, 72, 100, 0.1), (1030, 1, 128, 200, 1.0)])
+def test_few_heads_in_segments(l, heads, dk, dv, rate):
+    """Long sequences of few heads are cut along time: lengths that fill no segment, states that live through all of it."""
+    compare(both(make(l, 1, l, heads, heads, dk, dv, rate=rate)))
