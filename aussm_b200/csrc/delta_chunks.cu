@@ -28,7 +28,7 @@ DeltaPlan delta_plan(const aussm_b200_delta_t& p) {
     d.segs = (d.n + d.span - 1) / d.span;
     const size_t bh = (size_t)p.B * p.HV, ends = d.segs > 1 ? up256((d.segs - 1) * bh * p.DK * p.DV * sizeof(float)) : 0;
     d.transitions = d.heads * d.rec.bytes();
-    d.ends = d.transitions + (d.segs > 2 ? up256(d.segs * bh * p.DK * p.DK * sizeof(float)) : 0);
+    d.ends = d.transitions + (d.segs > 2 ? d.segs * bh * d.rec.key * d.rec.key * sizeof(float) : 0);
     d.fwd_bytes = d.news = d.ends + ends;
     d.states = d.news + up256(pieces * DeltaPlan::news_bytes());
     d.keep_bytes = d.states + up256(pieces * DeltaPlan::state_bytes(d.rec.key));

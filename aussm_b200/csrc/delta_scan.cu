@@ -325,12 +325,13 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         }
         float* to = a.seg_out ? a.seg_out + seg * a.seg_stride : seg == a.segs - 1 ? a.s1 : nullptr;
         if (to && mine) {
-            to += (size_t)bh * p.DK * width_all + v;
+            const int pitch = a.transition ? KEY : p.DV;
+            to += (size_t)bh * (a.transition ? KEY : p.DK) * pitch + v;
 #pragma unroll
             for (int x = 0; x < HALF / 2; ++x) {
                 const int k0 = sc + 2 * x;
-                if (k0 < p.DK) to[(size_t)k0 * width_all] = s[x].x;
-                if (k0 + 1 < p.DK) to[(size_t)(k0 + 1) * width_all] = s[x].y;
+                if (k0 < p.DK) to[(size_t)k0 * pitch] = s[x].x;
+                if (k0 + 1 < p.DK) to[(size_t)(k0 + 1) * pitch] = s[x].y;
             }
         }
     } else if (warp < 12) {
@@ -573,39 +574,70 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
 
 // States at the segments' boundaries, from what each segment makes of a zero state and what it does to a state:
 //     S_1 = N_0,   S_{z+1} = M_z S_z + N_z     (backward M^T of the mirrored segment),
-// S_{z+1} in the place of N_z.  A block owns 8 value columns of a head and keeps their states in shared memory; a thread
-// adds up 4 rows of one column in float32, M comes through the caches.
-constexpr int CHAIN_COLS = 8;
-__global__ void __launch_bounds__(256) delta_chain_kernel(const float* __restrict__ m, float* ends, int dk, int dv, int segs,
-                                                          size_t m_stride, size_t end_stride, bool backward) {
-    __shared__ float s[AUSSM_MAX_DELTA_KEY][CHAIN_COLS];
-    const int bh = blockIdx.x, v0 = blockIdx.y * CHAIN_COLS, col = threadIdx.x & 7, row = (threadIdx.x >> 3) * 4;
-    const bool mine = v0 + col < dv;
+// S_{z+1} in the place of N_z.  A block owns 16 value columns of a head and keeps their states in shared memory, where the
+// next M is on its way (M is stored with KEY columns a row) while this one is worked on: a thread adds up rows r, r + 32, ..
+// of two columns in float32.
+constexpr int CHAIN_COLS = 16;
+template <int KEY>
+struct ChainSmem {
+    static constexpr int kPitch = KEY + 4;               // floats of a row of M: neighbouring rows in other banks
+    static constexpr int kBytes = (2 * KEY * kPitch + KEY * CHAIN_COLS) * 4;
+};
+template <int KEY, bool BWD>
+__global__ void __launch_bounds__(256) delta_chain_kernel(const float* m, float* ends, int dk, int dv, int segs, size_t m_stride,
+                                                          size_t end_stride) {
+    constexpr int PITCH = ChainSmem<KEY>::kPitch, ROWS = KEY / 32;
+    extern __shared__ __align__(16) float chain[];
+    float* s = chain + 2 * KEY * PITCH;                  // [KEY][16]
+    const int bh = blockIdx.x, v0 = blockIdx.y * CHAIN_COLS, col = (threadIdx.x & 7) * 2, row = threadIdx.x >> 3;
     float* end = ends + (size_t)bh * dk * dv + v0 + col;
+    const bool in0 = v0 + col < dv, in1 = v0 + col + 1 < dv;
+    auto fetch = [&](int z) {
+        const float* from = m + (size_t)(BWD ? segs - 1 - z : z) * m_stride + (size_t)bh * KEY * KEY;
+        float* to = chain + (z & 1) * KEY * PITCH;
+        for (int e = threadIdx.x; e < dk * (KEY / 4); e += 256)
+            cp_async16(to + e / (KEY / 4) * PITCH + e % (KEY / 4) * 4, from + e * 4);
+        cp_async_commit();
+    };
+    fetch(1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[row + i][col] = mine && row + i < dk ? end[(size_t)(row + i) * dv] : 0.f;
-    __syncthreads();
+    for (int i = 0; i < ROWS; ++i) {
+        const int x = row + 32 * i;
+        const bool there = x < dk;
+        *reinterpret_cast<float2*>(s + x * CHAIN_COLS + col) =
+            make_float2(there && in0 ? end[(size_t)x * dv] : 0.f, there && in1 ? end[(size_t)x * dv + 1] : 0.f);
+    }
     for (int z = 1; z < segs - 1; ++z) {
-        const float* M = m + (size_t)(backward ? segs - 1 - z : z) * m_stride + (size_t)bh * dk * dk;
         float* to = end + z * end_stride;
-        float acc[4];
+        float2 acc[ROWS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = mine && row + i < dk ? to[(size_t)(row + i) * dv] : 0.f;
-        const int down = backward ? 1 : dk, along = backward ? dk : 1;      // M or M^T
-#pragma unroll 16
+        for (int i = 0; i < ROWS; ++i) {
+            const int x = row + 32 * i;
+            acc[i] = make_float2(x < dk && in0 ? to[(size_t)x * dv] : 0.f, x < dk && in1 ? to[(size_t)x * dv + 1] : 0.f);
+        }
+        cp_async_wait<0>();
+        __syncthreads();                                 // M and the states are there, the other M is free
+        if (z + 1 < segs - 1) fetch(z + 1);
+        const float* M = chain + (z & 1) * KEY * PITCH;
+#pragma unroll 8
         for (int x = 0; x < dk; ++x) {
-            const float f = s[x][col];
+            const float2 f = *reinterpret_cast<const float2*>(s + x * CHAIN_COLS + col);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (row + i < dk) acc[i] = fmaf(__ldg(M + (size_t)(row + i) * down + (size_t)x * along), f, acc[i]);
+            for (int i = 0; i < ROWS; ++i) {
+                const float w = BWD ? M[x * PITCH + row + 32 * i] : M[(row + 32 * i) * PITCH + x];
+                acc[i].x = fmaf(w, f.x, acc[i].x);
+                acc[i].y = fmaf(w, f.y, acc[i].y);
+            }
         }
-        __syncthreads();
+        __syncthreads();                                 // the states have been read
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[row + i][col] = acc[i];
-            if (mine && row + i < dk) to[(size_t)(row + i) * dv] = acc[i];
+        for (int i = 0; i < ROWS; ++i) {
+            const int x = row + 32 * i;
+            if (x >= dk) continue;                       // (M has no such rows)
+            *reinterpret_cast<float2*>(s + x * CHAIN_COLS + col) = acc[i];
+            if (in0) to[(size_t)x * dv] = acc[i].x;
+            if (in1) to[(size_t)x * dv + 1] = acc[i].y;
         }
-        __syncthreads();
     }
 }
 
@@ -618,7 +650,7 @@ cudaError_t scan(ScanParams a, const DeltaPlan& plan, float* m, float* ends, cud
     a.span = plan.span;
     a.segs = segs;
     if (segs > 1) {
-        const size_t m_stride = (size_t)heads * a.p.DK * a.p.DK, end_stride = (size_t)heads * a.p.DK * a.p.DV;
+        const size_t m_stride = (size_t)heads * KEY * KEY, end_stride = (size_t)heads * a.p.DK * a.p.DV;
         ScanParams q = a;
         q.out = nullptr; q.rows = nullptr; q.states = nullptr;
         if (!BWD && segs > 2) {              // what the segments between the first and the last do to a state
@@ -630,8 +662,10 @@ cudaError_t scan(ScanParams a, const DeltaPlan& plan, float* m, float* ends, cud
         delta_scan_kernel<T, KEY, BWD><<<dim3(heads, plan.slices, segs - 1), THREADS, smem, st>>>(q);
         count_launch();
         if (segs > 2) {
-            delta_chain_kernel<<<dim3(heads, (a.p.DV + CHAIN_COLS - 1) / CHAIN_COLS), 256, 0, st>>>(
-                m, ends, a.p.DK, a.p.DV, segs, m_stride, end_stride, BWD);
+            e = cudaFuncSetAttribute(delta_chain_kernel<KEY, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChainSmem<KEY>::kBytes);
+            if (e != cudaSuccess) return e;
+            delta_chain_kernel<KEY, BWD><<<dim3(heads, (a.p.DV + CHAIN_COLS - 1) / CHAIN_COLS), 256, ChainSmem<KEY>::kBytes, st>>>(
+                m, ends, a.p.DK, a.p.DV, segs, m_stride, end_stride);
             count_launch();
         }
         a.seg_in = ends - end_stride;        // segment z starts from the state behind segment z - 1
