@@ -5,8 +5,8 @@
 // Backward, with h = R^T dy and the mean / sum over the head:  dw = sum h x r,  dx = r (h w - x r^2 mean(h w x)).
 //
 // Bound: memory, every element read once and written once.  A group of 8, 16 or 32 lanes holds a head, both elements
-// of a pair in the same lane: the norm is a few shuffles, the rotation none.  The lane's angles serve all heads that
-// the group walks (8 of a token where that leaves enough groups, else 1).  Angles are reduced in 64 bits: position *
+// of a pair in the same lane: the norm is a few shuffles, the rotation none.  The lane's angles and weights serve the
+// heads of a token that the group walks: all of them where the tokens fill the GPU, fewer otherwise.  Angles are reduced in 64 bits: position *
 // (frequency / 2 pi), less its nearest integer, so a position of 2^22 is turned as exactly as position 1.
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -30,11 +30,10 @@ struct RotateParams {
     const double* frequencies;
     const long long* positions;
     float* part;                         // (blocks, 2, d) partial sums of dw, or NULL
-    int heads_per_group, head_groups, units, rot_units;
-    long long groups;
+    int split;                           // groups a token: group k walks heads k, k + split, ..
+    int units, rot_units;
+    unsigned groups;
 };
-
-template <typename T, int VEC> struct Pack { T v[VEC]; };
 
 // VEC consecutive elements as one access (VEC 4: the row is aligned to 4 elements)
 template <int VEC, typename T>
@@ -124,109 +123,92 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-// row of head hh of the two tensors together: which tensor, and where it starts
-struct Row {
-    int which;
-    long long in, dy, out;
-    __device__ Row(const RotateParams& a, int b, int t, int hh) {
-        which = hh >= a.p.HQ;
-        const int h = which ? hh - a.p.HQ : hh, heads = which ? a.p.HK : a.p.HQ;
-        const long long* s = which ? a.p.k_stride : a.p.q_stride;
-        const long long* g = which ? a.p.gk_stride : a.p.gq_stride;
-        in = b * s[0] + t * s[1] + h * s[2];
-        dy = b * g[0] + t * g[1] + h * g[2];
-        out = (((long long)b * a.p.L + t) * heads + h) * a.p.d;
-    }
-};
-
-// G lanes a head, UPL units a lane (UPL > 1 only for VEC 1)
+// The heads of one token and tensor that this group walks.  FLY of them are in flight together.
 template <typename T, int VEC, int G, int UPL, bool BWD>
-__global__ void __launch_bounds__(NT) rotate_kernel(const RotateParams a) {
-    constexpr int FLY = UPL > 1 ? 1 : BWD ? IN_FLIGHT / 2 : IN_FLIGHT;
-    const int lane = threadIdx.x % G;
-    const long long first = ((long long)blockIdx.x * NT + threadIdx.x) / G, stride = (long long)gridDim.x * (NT / G);
-    const int heads = a.p.HQ + a.p.HK;
-    const bool norm = a.p.norm != AUSSM_NORM_NONE;
-    const float inv_d = a.p.norm == AUSSM_NORM_RMS ? 1.f / (float)a.p.d : 1.f;
-    float dw[2][UPL][2][VEC] = {};
-    // all lanes of a warp stay together for the shuffles: a group behind the last one repeats it without storing
-    const long long rounds = (a.groups + stride - 1) / stride;
-    for (long long it = 0; it < rounds; ++it) {
-        long long gr = first + it * stride;
-        const bool live = gr < a.groups;
-        if (!live) gr = a.groups - 1;
-        const long long token = gr / a.head_groups;
-        const int h0 = (int)(gr % a.head_groups) * a.heads_per_group, h1 = min(heads, h0 + a.heads_per_group);
-        const int b = (int)(token / a.p.L), t = (int)(token % a.p.L);
-        const long long pos = a.positions ? a.positions[b * a.p.position_stride + t] : t;
-        Angles<VEC> ang[UPL];
+struct Walk {
+    static constexpr int FLY = UPL > 1 ? 1 : BWD ? IN_FLIGHT / 2 : IN_FLIGHT;
+    float w[UPL][2][VEC];                // weights of the lane's elements
+    float dw[BWD ? UPL : 1][2][VEC];     // their gradients
+
+    __device__ void start(const RotateParams& a, int which, int lane) {
 #pragma unroll
-        for (int u = 0; u < UPL; ++u) ang[u].set(a, lane + u * G, lane + u * G < a.rot_units, pos);
-        for (int hb = h0; hb < h1; hb += FLY) {
-            float x[FLY][UPL][2][VEC] = {}, g[BWD ? FLY : 1][UPL][2][VEC] = {};
+        for (int u = 0; u < UPL; ++u) {
+            const Unit<VEC> at(a, lane + u * G);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                w[u][0][i] = w[u][1][i] = 1.f;
+                if (BWD) dw[u][0][i] = dw[u][1][i] = 0.f;
+            }
+            if (a.w[which] && at.any) load<VEC>(a.w[which] + at.e0, w[u][0]);
+            if (a.w[which] && at.second) load<VEC>(a.w[which] + at.e1, w[u][1]);
+        }
+    }
+    // x, g, out: the token's first head; `heads` of them, the strides between them
+    __device__ void run(const RotateParams& a, const Angles<VEC> (&ang)[UPL], int lane, const T* x, long long xs, const T* g,
+                        long long gs, T* out, int part, int heads, bool live) {
+        const bool norm = a.p.norm != AUSSM_NORM_NONE, need = !BWD || norm || a.part;
+        const float inv_d = a.p.norm == AUSSM_NORM_RMS ? 1.f / (float)a.p.d : 1.f;
+        for (int base = 0; base < heads; base += FLY * a.split) {          // as often for all groups of a warp: shuffles
+            const int h = base + part;
+            float v[FLY][UPL][2][VEC], y[BWD ? FLY : 1][UPL][2][VEC];
 #pragma unroll
             for (int f = 0; f < FLY; ++f) {
-                if (hb + f >= h1) continue;
-                const Row r(a, b, t, hb + f);
-                const T* src = static_cast<const T*>(a.x[r.which]) + r.in;
-                const T* gsrc = BWD ? static_cast<const T*>(a.dy[r.which]) + r.dy : nullptr;
+                const int hh = h + f * a.split;
 #pragma unroll
                 for (int u = 0; u < UPL; ++u) {
                     const Unit<VEC> at(a, lane + u * G);
-                    if (at.any && (!BWD || norm || a.part)) load<VEC>(src + at.e0, x[f][u][0]);
-                    if (at.second && (!BWD || norm || a.part)) load<VEC>(src + at.e1, x[f][u][1]);
-                    if (BWD && at.any) load<VEC>(gsrc + at.e0, g[BWD ? f : 0][u][0]);
-                    if (BWD && at.second) load<VEC>(gsrc + at.e1, g[BWD ? f : 0][u][1]);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        v[f][u][0][i] = v[f][u][1][i] = 0.f;
+                        if (BWD) y[f % (BWD ? FLY : 1)][u][0][i] = y[f % (BWD ? FLY : 1)][u][1][i] = 0.f;
+                    }
+                    if (hh >= heads) continue;
+                    if (need && at.any) load<VEC>(x + hh * xs + at.e0, v[f][u][0]);
+                    if (need && at.second) load<VEC>(x + hh * xs + at.e1, v[f][u][1]);
+                    if (BWD && at.any) load<VEC>(g + hh * gs + at.e0, y[f % (BWD ? FLY : 1)][u][0]);
+                    if (BWD && at.second) load<VEC>(g + hh * gs + at.e1, y[f % (BWD ? FLY : 1)][u][1]);
                 }
             }
 #pragma unroll
             for (int f = 0; f < FLY; ++f) {
-                float sq = 0.f, rstd = 1.f;
+                const int hh = h + f * a.split;
+                const bool keep = live && hh < heads;
+                float rstd = 1.f, dot = 0.f;
                 if (norm) {
+                    float sq = 0.f;
 #pragma unroll
                     for (int u = 0; u < UPL; ++u)
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) sq += x[f][u][0][i] * x[f][u][0][i] + x[f][u][1][i] * x[f][u][1][i];
+                        for (int i = 0; i < VEC; ++i) sq += v[f][u][0][i] * v[f][u][0][i] + v[f][u][1][i] * v[f][u][1][i];
                     rstd = rsqrtf(group_sum<G>(sq) * inv_d + a.p.eps);
                 }
-                const int hh = min(hb + f, heads - 1);
-                const bool keep = live && hb + f < h1;
-                const Row r(a, b, t, hh);
-                const float* w = a.w[r.which];
-                T* dst = static_cast<T*>(a.out[r.which]) + r.out;
-                float dot = 0.f;
+                T* dst = out + (long long)hh * a.p.d;
 #pragma unroll
                 for (int u = 0; u < UPL; ++u) {
                     const Unit<VEC> at(a, lane + u * G);
-                    float w0[VEC], w1[VEC];
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) w0[i] = w1[i] = 1.f;
-                    if (w && at.any) load<VEC>(w + at.e0, w0);
-                    if (w && at.second) load<VEC>(w + at.e1, w1);
+                    float (&v0)[VEC] = v[f][u][0], (&v1)[VEC] = v[f][u][1];
                     if (!BWD) {
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) {
-                            x[f][u][0][i] *= rstd * w0[i];
-                            x[f][u][1][i] *= rstd * w1[i];
+                            v0[i] *= rstd * w[u][0][i];
+                            v1[i] *= rstd * w[u][1][i];
                         }
-                        if (at.turns) ang[u].turn(a.p.interleaved, x[f][u][0], x[f][u][1], 1.f);
-                        if (keep && at.any) store<VEC>(dst + at.e0, x[f][u][0]);
-                        if (keep && at.second) store<VEC>(dst + at.e1, x[f][u][1]);
+                        if (at.turns) ang[u].turn(a.p.interleaved, v0, v1, 1.f);
+                        if (keep && at.any) store<VEC>(dst + at.e0, v0);
+                        if (keep && at.second) store<VEC>(dst + at.e1, v1);
                     } else {
-                        float (&g0)[VEC] = g[BWD ? f : 0][u][0], (&g1)[VEC] = g[BWD ? f : 0][u][1];
+                        float (&g0)[VEC] = y[f % (BWD ? FLY : 1)][u][0], (&g1)[VEC] = y[f % (BWD ? FLY : 1)][u][1];
                         if (at.turns) ang[u].turn(a.p.interleaved, g0, g1, -1.f);
+                        const float r = keep ? rstd : 0.f;
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) {
-                            if (keep) {
-                                const float q0 = g0[i] * x[f][u][0][i] * rstd, q1 = g1[i] * x[f][u][1][i] * rstd;
-                                dw[0][u][0][i] += r.which ? 0.f : q0;
-                                dw[0][u][1][i] += r.which ? 0.f : q1;
-                                dw[1][u][0][i] += r.which ? q0 : 0.f;
-                                dw[1][u][1][i] += r.which ? q1 : 0.f;
+                            if (a.part && keep) {
+                                dw[u][0][i] = fmaf(g0[i], v0[i] * r, dw[u][0][i]);
+                                dw[u][1][i] = fmaf(g1[i], v1[i] * r, dw[u][1][i]);
                             }
-                            g0[i] *= w0[i];
-                            g1[i] *= w1[i];
-                            dot += g0[i] * x[f][u][0][i] + g1[i] * x[f][u][1][i];
+                            g0[i] *= w[u][0][i];
+                            g1[i] *= w[u][1][i];
+                            dot += g0[i] * v0[i] + g1[i] * v1[i];
                         }
                     }
                 }
@@ -235,12 +217,12 @@ __global__ void __launch_bounds__(NT) rotate_kernel(const RotateParams a) {
 #pragma unroll
                     for (int u = 0; u < UPL; ++u) {
                         const Unit<VEC> at(a, lane + u * G);
-                        float (&g0)[VEC] = g[BWD ? f : 0][u][0], (&g1)[VEC] = g[BWD ? f : 0][u][1];
+                        float (&g0)[VEC] = y[f % (BWD ? FLY : 1)][u][0], (&g1)[VEC] = y[f % (BWD ? FLY : 1)][u][1];
                         if (norm) {
 #pragma unroll
                             for (int i = 0; i < VEC; ++i) {
-                                g0[i] = rstd * (g0[i] - back * x[f][u][0][i]);
-                                g1[i] = rstd * (g1[i] - back * x[f][u][1][i]);
+                                g0[i] = rstd * (g0[i] - back * v[f][u][0][i]);
+                                g1[i] = rstd * (g1[i] - back * v[f][u][1][i]);
                             }
                         }
                         if (keep && at.any) store<VEC>(dst + at.e0, g0);
@@ -250,14 +232,46 @@ __global__ void __launch_bounds__(NT) rotate_kernel(const RotateParams a) {
             }
         }
     }
-    if (BWD && a.part) {                 // the block's groups add up in a fixed order, each element one thread
+};
+
+// G lanes a head, UPL units a lane (UPL > 1 only for VEC 1)
+template <typename T, int VEC, int G, int UPL, bool BWD>
+__global__ void __launch_bounds__(NT) rotate_kernel(const RotateParams a) {
+    const int lane = threadIdx.x % G;
+    const unsigned first = (blockIdx.x * NT + threadIdx.x) / G, stride = gridDim.x * (NT / G);
+    Walk<T, VEC, G, UPL, BWD> q, k;
+    q.start(a, 0, lane);
+    k.start(a, 1, lane);
+    // all lanes of a warp stay together for the shuffles: a group behind the last one repeats it without storing
+    const unsigned rounds = (a.groups + stride - 1) / stride;
+    for (unsigned it = 0; it < rounds; ++it) {
+        unsigned gr = first + it * stride;
+        const bool live = gr < a.groups;
+        if (!live) gr = a.groups - 1;
+        const unsigned token = a.split == 1 ? gr : gr / a.split, part = gr - token * a.split;
+        const unsigned b = token / (unsigned)a.p.L, t = token - b * a.p.L;
+        const long long pos = a.positions ? a.positions[b * a.p.position_stride + t] : t;
+        Angles<VEC> ang[UPL];
+#pragma unroll
+        for (int u = 0; u < UPL; ++u) ang[u].set(a, lane + u * G, lane + u * G < a.rot_units, pos);
+        const long long *xs = a.p.q_stride, *gs = a.p.gq_stride, *ks = a.p.k_stride, *hs = a.p.gk_stride;
+        q.run(a, ang, lane, static_cast<const T*>(a.x[0]) + b * xs[0] + t * xs[1], xs[2],
+              BWD ? static_cast<const T*>(a.dy[0]) + b * gs[0] + t * gs[1] : nullptr, gs[2],
+              static_cast<T*>(a.out[0]) + (long long)token * a.p.HQ * a.p.d, part, a.p.HQ, live);
+        k.run(a, ang, lane, static_cast<const T*>(a.x[1]) + b * ks[0] + t * ks[1], ks[2],
+              BWD ? static_cast<const T*>(a.dy[1]) + b * hs[0] + t * hs[1] : nullptr, hs[2],
+              static_cast<T*>(a.out[1]) + (long long)token * a.p.HK * a.p.d, part, a.p.HK, live);
+    }
+    if constexpr (BWD) {
+        if (!a.part) return;             // the block's groups add up in a fixed order, each element one thread
         __shared__ float sum[NT / G][G * UPL * 2 * VEC];
         for (int which = 0; which < 2; ++which) {
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < UPL; ++u)
 #pragma unroll
-                for (int i = 0; i < 2 * VEC; ++i) sum[threadIdx.x / G][((lane + u * G) * 2 + i / VEC) * VEC + i % VEC] = dw[which][u][i / VEC][i % VEC];
+                for (int i = 0; i < 2 * VEC; ++i)
+                    sum[threadIdx.x / G][((lane + u * G) * 2 + i / VEC) * VEC + i % VEC] = (which ? k : q).dw[u][i / VEC][i % VEC];
             __syncthreads();
             for (int e = threadIdx.x; e < G * UPL * 2 * VEC; e += NT) {
                 const int u = e / (2 * VEC), i = e % (2 * VEC);
@@ -308,15 +322,15 @@ void launch(RotateParams& a, int blocks_max, int* blocks_out, cudaStream_t st) {
     const int vw = vec ? 4 : 1, rest = a.p.d - a.p.rot;
     a.rot_units = a.p.rot / 2 / vw;
     a.units = a.rot_units + (rest + 2 * vw - 1) / (2 * vw);
-    const int heads = a.p.HQ + a.p.HK;
     const long long tokens = (long long)a.p.B * a.p.L;
-    // 8 heads share a lane's angles where that leaves 16 groups an SM or more; below, latency counts: one each
-    a.heads_per_group = tokens * ((heads + 7) / 8) >= 148 * 16 ? (heads < 8 ? heads : 8) : 1;
-    a.head_groups = (heads + a.heads_per_group - 1) / a.heads_per_group;
-    a.groups = tokens * a.head_groups;
+    // as many groups a token as give 16 groups an SM, at most one for each head of the longer of q and k
+    const int heads = a.p.HQ > a.p.HK ? a.p.HQ : a.p.HK;
+    const long long split = (148 * 16 + tokens - 1) / tokens;
+    a.split = (int)(split < heads ? split : heads);
+    a.groups = (unsigned)(tokens * a.split);
     const int g = a.units <= 8 ? 8 : a.units <= 16 ? 16 : 32;
-    const long long want = (a.groups + NT / g - 1) / (NT / g);
-    const unsigned grid = (unsigned)(want < blocks_max ? want : blocks_max);
+    const unsigned want = (a.groups + NT / g - 1) / (NT / g);
+    const unsigned grid = want < (unsigned)blocks_max ? want : (unsigned)blocks_max;
     if (vec) {
         if (g == 8) rotate_kernel<T, 4, 8, 1, BWD><<<grid, NT, 0, st>>>(a);
         else if (g == 16) rotate_kernel<T, 4, 16, 1, BWD><<<grid, NT, 0, st>>>(a);
@@ -343,6 +357,10 @@ int rotate_check(const char* who, const aussm_b200_rotate_t* p) {
     if (p->B <= 0 || p->L <= 0 || p->HQ <= 0 || p->HK <= 0 || p->d <= 0 || p->d > AUSSM_MAX_ROTATE_HEAD) {
         set_error("%s: bad sizes (B=%d L=%d HQ=%d HK=%d d=%d, d at most %d)", who, p->B, p->L, p->HQ, p->HK, p->d,
                   AUSSM_MAX_ROTATE_HEAD);
+        return AUSSM_EINVAL;
+    }
+    if ((long long)p->B * p->L > 0x0fffffffLL) {
+        set_error("%s: B*L=%lld tokens, at most 2^28 are supported", who, (long long)p->B * p->L);
         return AUSSM_EINVAL;
     }
     if (p->rot < 0 || p->rot % 2 || p->rot > p->d) {
