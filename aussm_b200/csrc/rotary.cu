@@ -35,25 +35,72 @@ struct RotateParams {
     unsigned groups;
 };
 
-// VEC consecutive elements as one access (VEC 4: the row is aligned to 4 elements)
+// VEC consecutive elements as one access (VEC > 1: the row is aligned to it), kept as the words they are
+template <typename T, int VEC>
+struct Piece {
+    static constexpr int BYTES = VEC * (int)sizeof(T), N = BYTES < 4 ? 1 : BYTES / 4;
+    uint32_t w[N];
+};
 template <int VEC, typename T>
-__device__ __forceinline__ void load(const T* p, float (&f)[VEC]) {
-    if (VEC == 1) f[0] = to_f32(*p);
-    else {
-        struct alignas(sizeof(T) * VEC) Raw { T v[VEC]; };
-        const Raw r = *reinterpret_cast<const Raw*>(p);
+__device__ __forceinline__ Piece<T, VEC> fetch(const T* p) {
+    using P = Piece<T, VEC>;
+    P r;
+    if constexpr (P::BYTES == 16) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+    } else if constexpr (P::BYTES == 8) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        r.w[0] = v.x; r.w[1] = v.y;
+    } else if constexpr (P::BYTES == 4) {
+        r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+        r.w[0] = *reinterpret_cast<const unsigned short*>(p);
+    }
+    return r;
+}
+__device__ __forceinline__ float2 two(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ float2 two(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const Piece<T, VEC>& r, float (&f)[VEC]) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) f[i] = to_f32(r.v[i]);
+        for (int i = 0; i < VEC; ++i) f[i] = __uint_as_float(r.w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+            const float2 v = two(r.w[i / 2], T());
+            f[i] = v.x;
+            if (i + 1 < VEC) f[i + 1] = v.y;
+        }
     }
 }
 template <int VEC, typename T>
 __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
-    if (VEC == 1) *p = from_f32<T>(f[0]);
+    using P = Piece<T, VEC>;
+    if constexpr (VEC == 1) *p = from_f32<T>(f[0]);
     else {
-        struct alignas(sizeof(T) * VEC) Raw { T v[VEC]; } r;
+        P r;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) r.v[i] = from_f32<T>(f[i]);
-        *reinterpret_cast<Raw*>(p) = r;
+        for (int i = 0; i < P::N; ++i) {
+            if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(f[i]);
+            else if constexpr (sizeof(T) == 2) {
+                const T lo = from_f32<T>(f[2 * i]), hi = from_f32<T>(f[2 * i + 1]);
+                r.w[i] = (uint32_t)*reinterpret_cast<const unsigned short*>(&lo) | (uint32_t)*reinterpret_cast<const unsigned short*>(&hi) << 16;
+            }
+        }
+        if constexpr (P::BYTES == 16) *reinterpret_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+        else *reinterpret_cast<uint2*>(p) = make_uint2(r.w[0], r.w[1]);
+    }
+}
+// weights are float32 whatever the elements are: pieces of 16 bytes
+template <int VEC>
+__device__ __forceinline__ void load_weights(const float* p, float (&f)[VEC]) {
+    constexpr int P = VEC < 4 ? VEC : 4;
+#pragma unroll
+    for (int k = 0; k < VEC; k += P) {
+        const Piece<float, P> r = fetch<P>(p + k);
+#pragma unroll
+        for (int i = 0; i < P; ++i) f[k + i] = __uint_as_float(r.w[i]);
     }
 }
 
@@ -123,110 +170,109 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-// The heads of one token and tensor that this group walks.  FLY of them are in flight together.
+// The heads of one token and tensor that this group walks, FLY of them in flight together: `start` asks for the first ones
+// (before the angles are worked out), `run` does them all.
 template <typename T, int VEC, int G, int UPL, bool BWD>
 struct Walk {
     static constexpr int FLY = UPL > 1 ? 1 : BWD ? IN_FLIGHT / 2 : IN_FLIGHT;
-    float w[UPL][2][VEC];                // weights of the lane's elements
-    float dw[BWD ? UPL : 1][2][VEC];     // their gradients
+    float dw[BWD ? UPL : 1][2][VEC];     // gradients of the weights of the lane's elements
+    const T *x, *g;                      // the token's first head
+    long long xs, gs;                    // strides between heads
+    T* out;
+    int heads, part;
+    Piece<T, VEC> px[FLY][UPL][2], pg[BWD ? FLY : 1][UPL][2];
 
-    __device__ void start(const RotateParams& a, int which, int lane) {
+    __device__ __forceinline__ void ask(const RotateParams& a, int lane, int h) {
+        const bool need = !BWD || a.p.norm != AUSSM_NORM_NONE || a.part;
+#pragma unroll
+        for (int f = 0; f < FLY; ++f) {
+            const int hh = h + f * a.split;
+#pragma unroll
+            for (int u = 0; u < UPL; ++u) {
+                const Unit<VEC> at(a, lane + u * G);
+#pragma unroll
+                for (int i = 0; i < Piece<T, VEC>::N; ++i) {
+                    px[f][u][0].w[i] = px[f][u][1].w[i] = 0;
+                    if (BWD) pg[BWD ? f : 0][u][0].w[i] = pg[BWD ? f : 0][u][1].w[i] = 0;
+                }
+                if (hh >= heads) continue;
+                if (need && at.any) px[f][u][0] = fetch<VEC>(x + hh * xs + at.e0);
+                if (need && at.second) px[f][u][1] = fetch<VEC>(x + hh * xs + at.e1);
+                if (BWD && at.any) pg[BWD ? f : 0][u][0] = fetch<VEC>(g + hh * gs + at.e0);
+                if (BWD && at.second) pg[BWD ? f : 0][u][1] = fetch<VEC>(g + hh * gs + at.e1);
+            }
+        }
+    }
+    __device__ __forceinline__ void run(const RotateParams& a, const Angles<VEC> (&ang)[UPL], int which, int lane, bool live) {
+        const bool norm = a.p.norm != AUSSM_NORM_NONE;
+        const float inv_d = a.p.norm == AUSSM_NORM_RMS ? 1.f / (float)a.p.d : 1.f;
+        float w[UPL][2][VEC];
 #pragma unroll
         for (int u = 0; u < UPL; ++u) {
             const Unit<VEC> at(a, lane + u * G);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                w[u][0][i] = w[u][1][i] = 1.f;
-                if (BWD) dw[u][0][i] = dw[u][1][i] = 0.f;
-            }
-            if (a.w[which] && at.any) load<VEC>(a.w[which] + at.e0, w[u][0]);
-            if (a.w[which] && at.second) load<VEC>(a.w[which] + at.e1, w[u][1]);
+            for (int i = 0; i < VEC; ++i) w[u][0][i] = w[u][1][i] = 1.f;
+            if (a.w[which] && at.any) load_weights<VEC>(a.w[which] + at.e0, w[u][0]);
+            if (a.w[which] && at.second) load_weights<VEC>(a.w[which] + at.e1, w[u][1]);
         }
-    }
-    // x, g, out: the token's first head; `heads` of them, the strides between them
-    __device__ void run(const RotateParams& a, const Angles<VEC> (&ang)[UPL], int lane, const T* x, long long xs, const T* g,
-                        long long gs, T* out, int part, int heads, bool live) {
-        const bool norm = a.p.norm != AUSSM_NORM_NONE, need = !BWD || norm || a.part;
-        const float inv_d = a.p.norm == AUSSM_NORM_RMS ? 1.f / (float)a.p.d : 1.f;
         for (int base = 0; base < heads; base += FLY * a.split) {          // as often for all groups of a warp: shuffles
-            const int h = base + part;
-            float v[FLY][UPL][2][VEC], y[BWD ? FLY : 1][UPL][2][VEC];
+            if (base) ask(a, lane, base + part);
 #pragma unroll
             for (int f = 0; f < FLY; ++f) {
-                const int hh = h + f * a.split;
-#pragma unroll
-                for (int u = 0; u < UPL; ++u) {
-                    const Unit<VEC> at(a, lane + u * G);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        v[f][u][0][i] = v[f][u][1][i] = 0.f;
-                        if (BWD) y[f % (BWD ? FLY : 1)][u][0][i] = y[f % (BWD ? FLY : 1)][u][1][i] = 0.f;
-                    }
-                    if (hh >= heads) continue;
-                    if (need && at.any) load<VEC>(x + hh * xs + at.e0, v[f][u][0]);
-                    if (need && at.second) load<VEC>(x + hh * xs + at.e1, v[f][u][1]);
-                    if (BWD && at.any) load<VEC>(g + hh * gs + at.e0, y[f % (BWD ? FLY : 1)][u][0]);
-                    if (BWD && at.second) load<VEC>(g + hh * gs + at.e1, y[f % (BWD ? FLY : 1)][u][1]);
-                }
-            }
-#pragma unroll
-            for (int f = 0; f < FLY; ++f) {
-                const int hh = h + f * a.split;
+                const int hh = base + part + f * a.split;
                 const bool keep = live && hh < heads;
-                float rstd = 1.f, dot = 0.f;
-                if (norm) {
-                    float sq = 0.f;
-#pragma unroll
-                    for (int u = 0; u < UPL; ++u)
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) sq += v[f][u][0][i] * v[f][u][0][i] + v[f][u][1][i] * v[f][u][1][i];
-                    rstd = rsqrtf(group_sum<G>(sq) * inv_d + a.p.eps);
-                }
-                T* dst = out + (long long)hh * a.p.d;
+                float v[UPL][2][VEC], rstd = 1.f, dot = 0.f, sq = 0.f;
 #pragma unroll
                 for (int u = 0; u < UPL; ++u) {
-                    const Unit<VEC> at(a, lane + u * G);
-                    float (&v0)[VEC] = v[f][u][0], (&v1)[VEC] = v[f][u][1];
-                    if (!BWD) {
+                    unpack(px[f][u][0], v[u][0]);
+                    unpack(px[f][u][1], v[u][1]);
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) {
-                            v0[i] *= rstd * w[u][0][i];
-                            v1[i] *= rstd * w[u][1][i];
-                        }
-                        if (at.turns) ang[u].turn(a.p.interleaved, v0, v1, 1.f);
-                        if (keep && at.any) store<VEC>(dst + at.e0, v0);
-                        if (keep && at.second) store<VEC>(dst + at.e1, v1);
-                    } else {
-                        float (&g0)[VEC] = y[f % (BWD ? FLY : 1)][u][0], (&g1)[VEC] = y[f % (BWD ? FLY : 1)][u][1];
-                        if (at.turns) ang[u].turn(a.p.interleaved, g0, g1, -1.f);
-                        const float r = keep ? rstd : 0.f;
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) {
-                            if (a.part && keep) {
-                                dw[u][0][i] = fmaf(g0[i], v0[i] * r, dw[u][0][i]);
-                                dw[u][1][i] = fmaf(g1[i], v1[i] * r, dw[u][1][i]);
-                            }
-                            g0[i] *= w[u][0][i];
-                            g1[i] *= w[u][1][i];
-                            dot += g0[i] * v0[i] + g1[i] * v1[i];
-                        }
-                    }
+                    for (int i = 0; i < VEC; ++i) sq += v[u][0][i] * v[u][0][i] + v[u][1][i] * v[u][1][i];
                 }
-                if (BWD) {
+                if (norm) rstd = rsqrtf(group_sum<G>(sq) * inv_d + a.p.eps);
+                T* dst = out + (long long)hh * a.p.d;
+                if (!BWD) {
+#pragma unroll
+                    for (int u = 0; u < UPL; ++u) {
+                        const Unit<VEC> at(a, lane + u * G);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) {
+                            v[u][0][i] *= rstd * w[u][0][i];
+                            v[u][1][i] *= rstd * w[u][1][i];
+                        }
+                        if (at.turns) ang[u].turn(a.p.interleaved, v[u][0], v[u][1], 1.f);
+                        if (keep && at.any) store<VEC>(dst + at.e0, v[u][0]);
+                        if (keep && at.second) store<VEC>(dst + at.e1, v[u][1]);
+                    }
+                } else {
+                    float y[UPL][2][VEC];
+#pragma unroll
+                    for (int u = 0; u < UPL; ++u) {
+                        const Unit<VEC> at(a, lane + u * G);
+                        unpack(pg[BWD ? f : 0][u][0], y[u][0]);
+                        unpack(pg[BWD ? f : 0][u][1], y[u][1]);
+                        if (at.turns) ang[u].turn(a.p.interleaved, y[u][0], y[u][1], -1.f);
+#pragma unroll
+                        for (int z = 0; z < 2; ++z)
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) {
+                                if (a.part && keep) dw[BWD ? u : 0][z][i] = fmaf(y[u][z][i], v[u][z][i] * rstd, dw[BWD ? u : 0][z][i]);
+                                y[u][z][i] *= w[u][z][i];
+                                dot += y[u][z][i] * v[u][z][i];
+                            }
+                    }
                     const float back = norm ? group_sum<G>(dot) * inv_d * rstd * rstd : 0.f;
 #pragma unroll
                     for (int u = 0; u < UPL; ++u) {
                         const Unit<VEC> at(a, lane + u * G);
-                        float (&g0)[VEC] = y[f % (BWD ? FLY : 1)][u][0], (&g1)[VEC] = y[f % (BWD ? FLY : 1)][u][1];
                         if (norm) {
 #pragma unroll
-                            for (int i = 0; i < VEC; ++i) {
-                                g0[i] = rstd * (g0[i] - back * v[f][u][0][i]);
-                                g1[i] = rstd * (g1[i] - back * v[f][u][1][i]);
-                            }
+                            for (int z = 0; z < 2; ++z)
+#pragma unroll
+                                for (int i = 0; i < VEC; ++i) y[u][z][i] = rstd * (y[u][z][i] - back * v[u][z][i]);
                         }
-                        if (keep && at.any) store<VEC>(dst + at.e0, g0);
-                        if (keep && at.second) store<VEC>(dst + at.e1, g1);
+                        if (keep && at.any) store<VEC>(dst + at.e0, y[u][0]);
+                        if (keep && at.second) store<VEC>(dst + at.e1, y[u][1]);
                     }
                 }
             }
@@ -236,12 +282,16 @@ struct Walk {
 
 // G lanes a head, UPL units a lane (UPL > 1 only for VEC 1)
 template <typename T, int VEC, int G, int UPL, bool BWD>
-__global__ void __launch_bounds__(NT) rotate_kernel(const RotateParams a) {
+__global__ void __launch_bounds__(NT, BWD ? 2 : 3) rotate_kernel(const RotateParams a) {
     const int lane = threadIdx.x % G;
     const unsigned first = (blockIdx.x * NT + threadIdx.x) / G, stride = gridDim.x * (NT / G);
     Walk<T, VEC, G, UPL, BWD> q, k;
-    q.start(a, 0, lane);
-    k.start(a, 1, lane);
+    if (BWD) {
+#pragma unroll
+        for (int u = 0; u < (BWD ? UPL : 1); ++u)
+#pragma unroll
+            for (int i = 0; i < 2 * VEC; ++i) q.dw[u][i / VEC][i % VEC] = k.dw[u][i / VEC][i % VEC] = 0.f;
+    }
     // all lanes of a warp stay together for the shuffles: a group behind the last one repeats it without storing
     const unsigned rounds = (a.groups + stride - 1) / stride;
     for (unsigned it = 0; it < rounds; ++it) {
@@ -251,16 +301,24 @@ __global__ void __launch_bounds__(NT) rotate_kernel(const RotateParams a) {
         const unsigned token = a.split == 1 ? gr : gr / a.split, part = gr - token * a.split;
         const unsigned b = token / (unsigned)a.p.L, t = token - b * a.p.L;
         const long long pos = a.positions ? a.positions[b * a.p.position_stride + t] : t;
+        auto place = [&](Walk<T, VEC, G, UPL, BWD>& w, int which, const long long* xs, const long long* gs, int heads) {
+            w.x = static_cast<const T*>(a.x[which]) + b * xs[0] + t * xs[1];
+            w.g = BWD ? static_cast<const T*>(a.dy[which]) + b * gs[0] + t * gs[1] : nullptr;
+            w.xs = xs[2];
+            w.gs = gs[2];
+            w.out = static_cast<T*>(a.out[which]) + (long long)token * heads * a.p.d;
+            w.heads = heads;
+            w.part = part;
+        };
+        place(q, 0, a.p.q_stride, a.p.gq_stride, a.p.HQ);
+        q.ask(a, lane, part);
         Angles<VEC> ang[UPL];
 #pragma unroll
         for (int u = 0; u < UPL; ++u) ang[u].set(a, lane + u * G, lane + u * G < a.rot_units, pos);
-        const long long *xs = a.p.q_stride, *gs = a.p.gq_stride, *ks = a.p.k_stride, *hs = a.p.gk_stride;
-        q.run(a, ang, lane, static_cast<const T*>(a.x[0]) + b * xs[0] + t * xs[1], xs[2],
-              BWD ? static_cast<const T*>(a.dy[0]) + b * gs[0] + t * gs[1] : nullptr, gs[2],
-              static_cast<T*>(a.out[0]) + (long long)token * a.p.HQ * a.p.d, part, a.p.HQ, live);
-        k.run(a, ang, lane, static_cast<const T*>(a.x[1]) + b * ks[0] + t * ks[1], ks[2],
-              BWD ? static_cast<const T*>(a.dy[1]) + b * hs[0] + t * hs[1] : nullptr, hs[2],
-              static_cast<T*>(a.out[1]) + (long long)token * a.p.HK * a.p.d, part, a.p.HK, live);
+        q.run(a, ang, 0, lane, live);
+        place(k, 1, a.p.k_stride, a.p.gk_stride, a.p.HK);
+        k.ask(a, lane, part);
+        k.run(a, ang, 1, lane, live);
     }
     if constexpr (BWD) {
         if (!a.part) return;             // the block's groups add up in a fixed order, each element one thread
@@ -299,29 +357,25 @@ __global__ void __launch_bounds__(128) rotate_weights_kernel(const float* part, 
     if (threadIdx.x == 0 && out) out[e] = s[0] + s[1] + s[2] + s[3];
 }
 
-// Whether rows can be taken four elements at a time: every piece of a row starts on a multiple of 4 elements.
-bool quads(const aussm_b200_rotate_t& p, const RotateParams& a, size_t size, bool bwd) {
-    const int rest = p.d - p.rot;
-    bool ok = p.rot % 8 == 0 && rest % 4 == 0;
+// Whether rows can be taken n elements at a time: every piece of a row starts on a multiple of n elements.
+bool pieces(const aussm_b200_rotate_t& p, const RotateParams& a, int n, size_t size, bool bwd) {
     auto row = [&](const void* base, const long long* s) {
-        if (!base) return true;
-        return reinterpret_cast<uintptr_t>(base) % (4 * size) == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0;
+        return reinterpret_cast<uintptr_t>(base) % (n * size) == 0 && s[0] % n == 0 && s[1] % n == 0 && s[2] % n == 0;
     };
-    ok = ok && row(a.x[0], p.q_stride) && row(a.x[1], p.k_stride);
+    bool ok = p.rot % (2 * n) == 0 && (p.d - p.rot) % n == 0 && row(a.x[0], p.q_stride) && row(a.x[1], p.k_stride);
     if (bwd) ok = ok && row(a.dy[0], p.gq_stride) && row(a.dy[1], p.gk_stride);
-    for (int i = 0; i < 2; ++i) {
-        ok = ok && reinterpret_cast<uintptr_t>(a.out[i]) % (4 * size) == 0;
-        ok = ok && reinterpret_cast<uintptr_t>(a.w[i]) % 16 == 0;
-    }
+    for (int i = 0; i < 2; ++i)
+        ok = ok && reinterpret_cast<uintptr_t>(a.out[i]) % (n * size) == 0 && reinterpret_cast<uintptr_t>(a.w[i]) % 16 == 0;
     return ok;
 }
 
-template <typename T, bool BWD>
-void launch(RotateParams& a, int blocks_max, int* blocks_out, cudaStream_t st) {
-    const bool vec = quads(a.p, a, sizeof(T), BWD);
-    const int vw = vec ? 4 : 1, rest = a.p.d - a.p.rot;
-    a.rot_units = a.p.rot / 2 / vw;
-    a.units = a.rot_units + (rest + 2 * vw - 1) / (2 * vw);
+// VEC elements an access: 4 where rows allow it, single ones otherwise.  (8 of a 16-bit type, 16 bytes a lane, need more
+// registers than three blocks an SM have: 231 us against 213 us, forward, 2 x 65536 steps of 12 heads of 128.)
+template <typename T, int VEC, bool BWD>
+int launch_vec(RotateParams& a, int blocks_max, cudaStream_t st) {
+    const int rest = a.p.d - a.p.rot;
+    a.rot_units = a.p.rot / 2 / VEC;
+    a.units = a.rot_units + (rest + 2 * VEC - 1) / (2 * VEC);
     const long long tokens = (long long)a.p.B * a.p.L;
     // as many groups a token as give 16 groups an SM, at most one for each head of the longer of q and k
     const int heads = a.p.HQ > a.p.HK ? a.p.HQ : a.p.HK;
@@ -331,15 +385,16 @@ void launch(RotateParams& a, int blocks_max, int* blocks_out, cudaStream_t st) {
     const int g = a.units <= 8 ? 8 : a.units <= 16 ? 16 : 32;
     const unsigned want = (a.groups + NT / g - 1) / (NT / g);
     const unsigned grid = want < (unsigned)blocks_max ? want : (unsigned)blocks_max;
-    if (vec) {
-        if (g == 8) rotate_kernel<T, 4, 8, 1, BWD><<<grid, NT, 0, st>>>(a);
-        else if (g == 16) rotate_kernel<T, 4, 16, 1, BWD><<<grid, NT, 0, st>>>(a);
-        else rotate_kernel<T, 4, 32, 1, BWD><<<grid, NT, 0, st>>>(a);
-    } else if (g == 8) rotate_kernel<T, 1, 8, 1, BWD><<<grid, NT, 0, st>>>(a);
-    else if (g == 16) rotate_kernel<T, 1, 16, 1, BWD><<<grid, NT, 0, st>>>(a);
-    else rotate_kernel<T, 1, 32, 4, BWD><<<grid, NT, 0, st>>>(a);
+    constexpr int MOST = AUSSM_MAX_ROTATE_HEAD / 2 / VEC;         // units of the widest head
+    if (g == 8) rotate_kernel<T, VEC, 8, 1, BWD><<<grid, NT, 0, st>>>(a);
+    else if (g == 16) rotate_kernel<T, VEC, 16, 1, BWD><<<grid, NT, 0, st>>>(a);
+    else if constexpr (MOST > 16) rotate_kernel<T, VEC, 32, (MOST + 31) / 32, BWD><<<grid, NT, 0, st>>>(a);
     count_launch();
-    *blocks_out = (int)grid;
+    return (int)grid;
+}
+template <typename T, bool BWD>
+void launch(RotateParams& a, int blocks_max, int* blocks_out, cudaStream_t st) {
+    *blocks_out = pieces(a.p, a, 4, sizeof(T), BWD) ? launch_vec<T, 4, BWD>(a, blocks_max, st) : launch_vec<T, 1, BWD>(a, blocks_max, st);
 }
 
 template <bool BWD>

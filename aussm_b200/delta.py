@@ -12,14 +12,16 @@ every input type.  CUDA tensors only; all arithmetic runs in libaussm_b200.so.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 from typing import Optional
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from .ops import _PLAIN, _eager, _ptr, _stream, _workspace
+from .ops import _PLAIN, _eager, _ptr, _workspace
 
 __all__ = ["gated_delta_rule", "gated_delta_step", "MAX_KEY", "MAX_VALUE"]
 
@@ -52,8 +54,27 @@ def _typed(name: str, t: Tensor, dtype, shape, device) -> Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """The device as the current one.  Short calls are bound by the host: nothing is entered where it is already."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _raw_stream(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _strides(t: Tensor):
     return (ctypes.c_longlong * 3)(*t.stride()[:3])
+
+
+@functools.lru_cache(maxsize=256)
+def _problem(b, l, hk, hv, dk, dv, dtype, scale, *strides):
+    """The problem of these sizes, types and strides: read only (the backward call takes a copy)."""
+    q, k, v = ((ctypes.c_longlong * 3)(*strides[i:i + 3]) for i in (0, 3, 6))
+    return _lib.DeltaProblem(b, l, hk, hv, dk, dv, dtype, scale, q, k, v)
 
 
 def _check(q, k, v, g, beta, scale):
@@ -75,8 +96,8 @@ def _check(q, k, v, g, beta, scale):
     v = _typed("v", v, q.dtype, (b, l, hv, dv), q.device)
     g = _typed("g", g, torch.float32, (b, l, hv), q.device).contiguous()
     beta = _typed("beta", beta, torch.float32, (b, l, hv), q.device).contiguous()
-    p = _lib.DeltaProblem(b, l, hk, hv, dk, dv, _DTYPES[q.dtype], dk ** -0.5 if scale is None else float(scale),
-                          _strides(q), _strides(k), _strides(v))
+    p = _problem(b, l, hk, hv, dk, dv, _DTYPES[q.dtype], dk ** -0.5 if scale is None else float(scale), *q.stride()[:3],
+                 *k.stride()[:3], *v.stride()[:3])
     return p, q, k, v, g, beta
 
 
@@ -84,31 +105,33 @@ def _state(name: str, s: Tensor, p, device) -> Tensor:
     return _typed(name, s, torch.float32, (p.B, p.HV, p.DK, p.DV), device).contiguous()
 
 
+def _forward(p, q, k, v, g, beta, state, want_state, train):
+    """``(o, final state or None, what the backward call reads or None)``"""
+    o = torch.empty((p.B, p.L, p.HV, p.DV), device=q.device, dtype=q.dtype)
+    last = torch.empty((p.B, p.HV, p.DK, p.DV), device=q.device, dtype=torch.float32) if want_state else None
+    if o.numel() == 0:
+        if last is not None:
+            last.zero_() if state is None else last.copy_(state)
+        return o, last, None
+    lib = _lib.load()
+    with _on(q.device):
+        size = lib.aussm_b200_delta_keep_bytes(p) if train else lib.aussm_b200_delta_workspace_bytes(p, 0)
+        room = _workspace(size, q.device)
+        rc = lib.aussm_b200_delta_fwd(p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(o), _ptr(last),
+                                      _ptr(room) if train else None, size if train else 0, None if train else _ptr(room),
+                                      0 if train else size, _raw_stream(q.device))
+    _lib.check(rc, "gated_delta_rule")
+    return o, last, room if train else None
+
+
 class _GatedDelta(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, state, scale, want_state, keep_for_backward):
+    def forward(ctx, q, k, v, g, beta, state, scale, want_state):
         p, q, k, v, g, beta = _check(q, k, v, g, beta, scale)
         state = None if state is None else _state("initial_state", state, p, q.device)
-        o = torch.empty(p.B, p.L, p.HV, p.DV, device=q.device, dtype=q.dtype)
-        last = torch.empty(p.B, p.HV, p.DK, p.DV, device=q.device, dtype=torch.float32) if want_state else None
+        o, last, keep = _forward(p, q, k, v, g, beta, state, want_state, True)
         ctx.set_materialize_grads(False)
         ctx.p, ctx.has_state = p, state is not None
-        if o.numel() == 0:
-            if last is not None:
-                last.zero_() if state is None else last.copy_(state)
-            ctx.save_for_backward(q, k, v, g, beta, None)
-            return o, last
-        lib = _lib.load()
-        with torch.cuda.device(q.device):
-            keep = ws = None
-            if keep_for_backward:
-                keep = _workspace(lib.aussm_b200_delta_keep_bytes(p), q.device)
-            else:
-                ws = _workspace(lib.aussm_b200_delta_workspace_bytes(p, 0), q.device)
-            rc = lib.aussm_b200_delta_fwd(p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(o), _ptr(last),
-                                          _ptr(keep), 0 if keep is None else keep.numel(), _ptr(ws),
-                                          0 if ws is None else ws.numel(), _stream(q))
-        _lib.check(rc, "gated_delta_rule")
         ctx.save_for_backward(q, k, v, g, beta, keep)
         return o, last
 
@@ -127,18 +150,18 @@ class _GatedDelta(torch.autograd.Function):
         if keep is None:                                # no steps
             if ds0 is not None:
                 ds0.zero_() if glast is None else ds0.copy_(glast)
-            return dq, dk, dv, dg, dbeta, ds0, None, None, None
+            return dq, dk, dv, dg, dbeta, ds0, None, None
         go = torch.zeros(v.shape, device=v.device, dtype=v.dtype) if go is None else go
         go = go if go.stride(-1) == 1 or go.shape[-1] == 1 else go.contiguous()
         p.go_stride = _strides(go)
         lib = _lib.load()
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             ws = _workspace(lib.aussm_b200_delta_workspace_bytes(p, 1), q.device)
             rc = lib.aussm_b200_delta_bwd(p, _ptr(go), _ptr(glast), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(keep),
                                           keep.numel(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dg), _ptr(dbeta), _ptr(ds0),
-                                          _ptr(ws), ws.numel(), _stream(q))
+                                          _ptr(ws), ws.numel(), _raw_stream(q.device))
         _lib.check(rc, "gated_delta_rule backward")
-        return dq, dk, dv, dg, dbeta, ds0, None, None, None
+        return dq, dk, dv, dg, dbeta, ds0, None, None
 
 
 def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, scale: Optional[float] = None,
@@ -155,7 +178,12 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     Returns ``o`` ``(b, l, hv, dv)`` of the inputs' type, or ``(o, final_state)``."""
     _refuse_traced("gated_delta_rule", q, k, v, g, beta, initial_state)
     grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
-    o, last = _GatedDelta.apply(q, k, v, g, beta, initial_state, scale, bool(return_final_state), grad)
+    if grad:
+        o, last = _GatedDelta.apply(q, k, v, g, beta, initial_state, scale, bool(return_final_state))
+    else:
+        p, q, k, v, g, beta = _check(q, k, v, g, beta, scale)
+        state = None if initial_state is None else _state("initial_state", initial_state, p, q.device)
+        o, last, _ = _forward(p, q, k, v, g, beta, state, bool(return_final_state), False)
     return (o, last) if return_final_state else o
 
 
@@ -179,13 +207,13 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
         lo, hi, size = sorted((state.data_ptr(), out.data_ptr())) + [4 * state.numel()]
         if lo != hi and hi < lo + size:
             raise RuntimeError("new_state overlaps state in part")
-    o = torch.empty(p.B, p.L, p.HV, p.DV, device=q.device, dtype=q.dtype)
+    o = torch.empty((p.B, p.L, p.HV, p.DV), device=q.device, dtype=q.dtype)
     if o.numel() == 0:
         if out.data_ptr() != state.data_ptr():
             out.copy_(state)
         return o
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         rc = _lib.load().aussm_b200_delta_step(p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(out),
-                                               _ptr(o), _stream(q))
+                                               _ptr(o), _raw_stream(q.device))
     _lib.check(rc, "gated_delta_step")
     return o

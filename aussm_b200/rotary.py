@@ -7,6 +7,8 @@ a model was trained on.  CUDA tensors only; all arithmetic runs in libaussm_b200
 """
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -14,8 +16,8 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .delta import _DTYPES, _refuse_traced, _strides, _typed
-from .ops import _ptr, _stream, _workspace
+from .delta import _DTYPES, _on, _raw_stream, _refuse_traced, _strides, _typed
+from .ops import _ptr, _workspace
 
 __all__ = ["qk_norm_rotate", "rotary_frequencies", "MAX_HEAD"]
 
@@ -54,19 +56,30 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] =
     return f, magnitude
 
 
+@functools.lru_cache(maxsize=256)
+def _problem(b, l, hq, hk, d, rot, dtype, norm, interleaved, eps, magnitude, position_stride, *strides):
+    """The problem of these sizes, types and strides: read only (the backward call takes a copy)."""
+    q, k = ((ctypes.c_longlong * 3)(*strides[i:i + 3]) for i in (0, 3))
+    return _lib.RotateProblem(b, l, hq, hk, d, rot, dtype, norm, interleaved, eps, magnitude, position_stride, q, k)
+
+
+def _forward(q, k, q_weight, k_weight, frequencies, positions, p):
+    yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    yk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+    if p.B and p.L:
+        with _on(q.device):
+            rc = _lib.load().aussm_b200_rotate_fwd(p, _ptr(q), _ptr(k), _ptr(frequencies), _ptr(positions), _ptr(q_weight),
+                                                   _ptr(k_weight), _ptr(yq), _ptr(yk), _raw_stream(q.device))
+        _lib.check(rc, "qk_norm_rotate")
+    return yq, yk
+
+
 class _NormRotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, frequencies, positions, p):
-        yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        yk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
         ctx.p = p
         ctx.save_for_backward(q, k, q_weight, k_weight, frequencies, positions)
-        if p.B and p.L:
-            with torch.cuda.device(q.device):
-                rc = _lib.load().aussm_b200_rotate_fwd(p, _ptr(q), _ptr(k), _ptr(frequencies), _ptr(positions), _ptr(q_weight),
-                                                       _ptr(k_weight), _ptr(yq), _ptr(yk), _stream(q))
-            _lib.check(rc, "qk_norm_rotate")
-        return yq, yk
+        return _forward(q, k, q_weight, k_weight, frequencies, positions, p)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -81,13 +94,13 @@ class _NormRotate(torch.autograd.Function):
         gq, gk = (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (gq, gk))
         p.gq_stride, p.gk_stride = _strides(gq), _strides(gk)
         lib = _lib.load()
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             ws = None
             if dqw is not None or dkw is not None:
                 ws = _workspace(lib.aussm_b200_rotate_bwd_workspace_bytes(p), q.device)
             rc = lib.aussm_b200_rotate_bwd(p, _ptr(gq), _ptr(gk), _ptr(q), _ptr(k), _ptr(frequencies), _ptr(positions),
                                            _ptr(q_weight), _ptr(k_weight), _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(ws),
-                                           0 if ws is None else ws.numel(), _stream(q))
+                                           0 if ws is None else ws.numel(), _raw_stream(q.device))
         _lib.check(rc, "qk_norm_rotate backward")
         return dq, dk, dqw, dkw, None, None, None
 
@@ -131,6 +144,8 @@ def qk_norm_rotate(q: Tensor, k: Tensor, frequencies: Optional[Tensor] = None, p
         shape = (l,) if positions.dim() == 1 else (b, l)
         positions = _typed("positions", positions, torch.int64, shape, dev).contiguous()
         stride = 0 if positions.dim() == 1 else l
-    p = _lib.RotateProblem(b, l, hq, k.shape[2], d, 2 * n, _DTYPES[q.dtype], _NORMS[norm], int(bool(interleaved)), float(eps),
-                           float(magnitude), stride, _strides(q), _strides(k))
-    return _NormRotate.apply(q, k, q_weight, k_weight, frequencies, positions, p)
+    p = _problem(b, l, hq, k.shape[2], d, 2 * n, _DTYPES[q.dtype], _NORMS[norm], int(bool(interleaved)), float(eps), float(magnitude),
+                 stride, *q.stride()[:3], *k.stride()[:3])
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return _NormRotate.apply(q, k, q_weight, k_weight, frequencies, positions, p)
+    return _forward(q, k, q_weight, k_weight, frequencies, positions, p)
