@@ -12,7 +12,7 @@
 namespace aussm {
 namespace {
 
-constexpr int NT = 256, WARPS = NT / 32, COLS = 32;
+constexpr int NT = 256, WARPS = NT / 32;
 
 struct StepParams {
     aussm_b200_delta_t p;
@@ -23,7 +23,7 @@ struct StepParams {
 };
 
 // VEC 4: 8 lanes a row, VEC 1 (DV no multiple of 4, or unaligned states): 32 lanes a row
-template <typename T, int VEC>
+template <typename T, int VEC, int COLS>
 __global__ void __launch_bounds__(NT) delta_step_kernel(const StepParams a) {
     constexpr int LANES = COLS / VEC, ROWS = NT / LANES, RPT = AUSSM_MAX_DELTA_KEY / ROWS;
     __shared__ float ks[2][AUSSM_MAX_DELTA_KEY], qs[2][AUSSM_MAX_DELTA_KEY];
@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(NT) delta_step_kernel(const StepParams a) {
         for (int c = 0; c < VEC; ++c) S[i][c] = 0.f;
         if (mine && row < p.DK) {
             if (VEC == 4) {
-                const float4 x = *reinterpret_cast<const float4*>(src);
+                const float4 x = __ldcs(reinterpret_cast<const float4*>(src));     // read once: first to leave the L2
                 S[i][0] = x.x; S[i][1 % VEC] = x.y; S[i][2 % VEC] = x.z; S[i][3 % VEC] = x.w;
             } else {
                 S[i][0] = *src;
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(NT) delta_step_kernel(const StepParams a) {
         const int row = row0 + i * ROWS;
         float* dst = a.new_state + base + (size_t)row * p.DV;
         if (mine && row < p.DK) {
-            if (VEC == 4) *reinterpret_cast<float4*>(dst) = make_float4(S[i][0], S[i][1 % VEC], S[i][2 % VEC], S[i][3 % VEC]);
+            if (VEC == 4) __stcs(reinterpret_cast<float4*>(dst), make_float4(S[i][0], S[i][1 % VEC], S[i][2 % VEC], S[i][3 % VEC]));
             else *dst = S[i][0];
         }
     }
@@ -137,10 +137,12 @@ __global__ void __launch_bounds__(NT) delta_step_kernel(const StepParams a) {
 
 template <typename T>
 void step(const StepParams& a, cudaStream_t st) {
-    const unsigned grid = (unsigned)((long long)a.p.B * a.p.HV * ((a.p.DV + COLS - 1) / COLS));
+    const long long heads = (long long)a.p.B * a.p.HV;
     const uintptr_t bits = reinterpret_cast<uintptr_t>(a.state) | reinterpret_cast<uintptr_t>(a.new_state);
-    if (a.p.DV % 4 == 0 && bits % 16 == 0) delta_step_kernel<T, 4><<<grid, NT, 0, st>>>(a);
-    else delta_step_kernel<T, 1><<<grid, NT, 0, st>>>(a);
+    const bool vec = a.p.DV % 4 == 0 && bits % 16 == 0;
+    if (vec && heads >= 148 * 4 && a.p.DV > 64) delta_step_kernel<T, 4, 128><<<(unsigned)(heads * ((a.p.DV + 127) / 128)), NT, 0, st>>>(a);
+    else if (vec) delta_step_kernel<T, 4, 32><<<(unsigned)(heads * ((a.p.DV + 31) / 32)), NT, 0, st>>>(a);
+    else delta_step_kernel<T, 1, 32><<<(unsigned)(heads * ((a.p.DV + 31) / 32)), NT, 0, st>>>(a);
     count_launch();
 }
 
