@@ -12,6 +12,10 @@ differ: ``SSMauBlock`` calls ``aussm_b200.ops.ssm_adaptive_interface`` and
 the latter from the third-party package mamba-ssm); and the ``nn.Linear``
 layers are ``aussm_b200.linear.SplitLinear`` (same parameters; the float32
 products run on the tensor cores through the library's split GEMM).
+
+``GatedDeltaBlock`` (layer kind ``g``) has no counterpart in the reference: a
+mixer with a matrix state next to the two with vector states, in the same
+residual blocks and models.
 """
 from __future__ import annotations
 
@@ -21,10 +25,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops, s6, stages
+from . import delta, ops, rotary, s6, stages
 from .linear import SplitLinear, split_linear
 
-__all__ = ["RMSNorm", "SSMauBlock", "MambaBlock", "ResidualBlock", "SSMTS", "SSMSequenceClassifier"]
+__all__ = ["RMSNorm", "SSMauBlock", "MambaBlock", "GatedDeltaBlock", "ResidualBlock", "SSMTS", "SSMSequenceClassifier"]
 
 
 class RMSNorm(nn.Module):
@@ -168,6 +172,93 @@ class MambaBlock(nn.Module):
         return stages.project_back(self.out_proj.weight, y, self.out_proj.bias)
 
 
+class GatedDeltaBlock(nn.Module):
+    """Gated delta rule mixer: in_proj -> depthwise conv, SiLU -> queries and keys to unit length (and rotated) -> gated
+    delta rule -> norm of every head, gate -> out_proj.
+
+    ``n_heads`` heads of ``d_model / n_heads`` keys and values (default: the fewest of at most 128); ``rotary_dim`` > 0
+    rotates that many elements of every query and key by position.  ``forward`` takes whole sequences (b, l, d),
+    ``step`` one token of each with the ``cache`` of ``init_cache``, for serving."""
+
+    def __init__(self, d_model: int, n_heads: int = None, d_conv: int = 4, conv_bias: bool = True, bias: bool = False,
+                 rotary_dim: int = 0, rotary_base: float = 10000.0):
+        super().__init__()
+        if n_heads is None:
+            n_heads = next(h for h in range(1, d_model + 1) if d_model % h == 0 and d_model // h <= delta.MAX_KEY)
+        if d_model % n_heads or d_model // n_heads > delta.MAX_KEY:
+            raise ValueError(f"{n_heads} heads do not cut {d_model} channels into heads of at most {delta.MAX_KEY}")
+        if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > d_model // n_heads:
+            raise ValueError(f"rotary_dim must be even and at most the head's {d_model // n_heads}, got {rotary_dim}")
+        self.d_model, self.n_heads, self.d_head = d_model, n_heads, d_model // n_heads
+        self.rotary_dim, self.rotary_base = rotary_dim, rotary_base
+        self.in_proj = SplitLinear(d_model, 4 * d_model, bias=bias)          # q, k, v and the gate z
+        self.gate_proj = SplitLinear(d_model, 2 * n_heads, bias=False)       # decay and step size of every head
+        self.conv1d = nn.Conv1d(3 * d_model, 3 * d_model, kernel_size=d_conv, groups=3 * d_model, padding=d_conv - 1, bias=conv_bias)
+        self.out_proj = SplitLinear(d_model, d_model, bias=bias)
+        self.norm = RMSNorm(self.d_head)
+        self.A_log = nn.Parameter(torch.log(torch.empty(n_heads).uniform_(1, 16)))
+        # softplus(dt_bias) spread over 0.001 .. 0.1: heads that remember a thousand steps and heads that remember ten
+        dt = torch.exp(torch.empty(n_heads).uniform_(math.log(0.001), math.log(0.1)))
+        self.dt_bias = nn.Parameter(dt + torch.log(-torch.expm1(-dt)))
+        self.A_log._no_weight_decay = True
+        self._angles = {}
+
+    def _frequencies(self, device):
+        if not self.rotary_dim:
+            return None
+        if device not in self._angles:       # float64 whatever type the module is cast to
+            self._angles[device] = rotary.rotary_frequencies(self.rotary_dim, self.rotary_base, device=device)[0]
+        return self._angles[device]
+
+    def _inputs(self, x, conv, positions):
+        """q, k, v, g, beta from the tokens x and their convolved q, k, v channels (b, l, 3 d)."""
+        b, l, _ = x.shape
+        q, k, v = F.silu(conv).view(b, l, 3, self.n_heads, self.d_head).unbind(2)
+        q, k = rotary.qk_norm_rotate(q, k, self._frequencies(x.device), positions, norm="l2")
+        a, beta = self.gate_proj(x).float().split([self.n_heads, self.n_heads], dim=-1)
+        g = -torch.exp(self.A_log.float()) * F.softplus(a + self.dt_bias.float())
+        return q, k, v, g, torch.sigmoid(beta)
+
+    def _output(self, o, z):
+        b, l = o.shape[:2]
+        return self.out_proj((self.norm(o) * F.silu(z.view(b, l, self.n_heads, self.d_head))).reshape(b, l, self.d_model))
+
+    def forward(self, x):
+        d = self.d_model
+        if x.is_cuda and x.dtype == torch.float32 and self.conv1d.kernel_size[0] <= 4:
+            w, bias = self.in_proj.weight, self.in_proj.bias
+            xs = stages.project_tokens(w[:3 * d], x)                         # (b, 3d, l): the convolution's layout
+            xs = xs if bias is None else xs + bias[:3 * d, None]
+            z = split_linear(x, w[3 * d:], None if bias is None else bias[3 * d:])
+            conv = stages.causal_conv_bias(xs, self.conv1d.weight, self.conv1d.bias).transpose(1, 2).contiguous()
+        else:
+            xs, z = self.in_proj(x).split([3 * d, d], dim=-1)
+            conv = _causal_depthwise_conv(self.conv1d, xs).contiguous()
+        q, k, v, g, beta = self._inputs(x, conv, None)
+        return self._output(delta.gated_delta_rule(q, k, v, g, beta), z)
+
+    def init_cache(self, batch: int, device=None, dtype=torch.float32):
+        """What ``step`` carries from token to token: the state (float32), the convolution's last inputs, the position."""
+        h, w = self.n_heads, self.d_head
+        return dict(state=torch.zeros(batch, h, w, w, device=device, dtype=torch.float32), position=0,
+                    conv=torch.zeros(batch, self.conv1d.kernel_size[0] - 1, 3 * self.d_model, device=device, dtype=dtype))
+
+    @torch.no_grad()
+    def step(self, x, cache):
+        """One token of every sequence: x (b, 1, d) -> (b, 1, d); ``cache`` is updated in place."""
+        d = self.d_model
+        xs, z = self.in_proj(x).split([3 * d, d], dim=-1)
+        window = torch.cat((cache["conv"], xs), 1)                           # (b, k, 3d)
+        conv = torch.einsum("bkc,ck->bc", window, self.conv1d.weight[:, 0])[:, None]
+        if self.conv1d.bias is not None:
+            conv = conv + self.conv1d.bias
+        cache["conv"].copy_(window[:, 1:])
+        positions = torch.full((1,), cache["position"], device=x.device, dtype=torch.int64) if self.rotary_dim else None
+        q, k, v, g, beta = self._inputs(x, conv.contiguous(), positions)
+        cache["position"] += 1
+        return self._output(delta.gated_delta_step(q, k, v, g, beta, cache["state"]), z)
+
+
 def _has_hooks(m: nn.Module) -> bool:
     from torch.nn.modules import module as hooks
     return bool(type(m) is not RMSNorm or "forward" in m.__dict__ or m._forward_hooks or m._forward_pre_hooks
@@ -198,6 +289,8 @@ def _build_layers(layers: str, d_model, d_state, mamba_expand, dt_rank, d_conv, 
             mixer = SSMauBlock(d_model, d_state, dt_rank, d_conv, conv_bias, bias, ssmau_conv_1d)
         elif kind == "m":
             mixer = MambaBlock(d_model, d_state, mamba_expand, dt_rank, d_conv, conv_bias, bias)
+        elif kind == "g":
+            mixer = GatedDeltaBlock(d_model, d_conv=d_conv, conv_bias=conv_bias, bias=bias)
         else:
             raise NotImplementedError(f'Layer type "{kind}" not recognized')
         blocks.append(ResidualBlock(mixer, d_model))
@@ -205,7 +298,7 @@ def _build_layers(layers: str, d_model, d_state, mamba_expand, dt_rank, d_conv, 
 
 
 class SSMTS(nn.Module):
-    """Time-series model: Linear embedding -> 'a|m|...' residual blocks -> RMSNorm -> Linear head, per step."""
+    """Time-series model: Linear embedding -> 'a|m|g|...' residual blocks -> RMSNorm -> Linear head, per step."""
 
     def __init__(self, d_model: int, input_dim: int, output_dim: int, layers: str = "m|a", d_state: int = 16,
                  mamba_expand: int = 2, dt_rank="auto", d_conv: int = 4, conv_bias: bool = True, bias: bool = False,

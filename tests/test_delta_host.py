@@ -80,3 +80,51 @@ def test_c_entries_refuse_on_the_host():
     for i, value in ((0, 0), (4, 257), (5, 3), (5, 66), (6, 5), (7, 3)):
         p = aussm_b200._lib.RotateProblem(*(good[:i] + (value,) + good[i + 1:]))
         assert lib.aussm_b200_rotate_fwd(p, *([None] * 9)) == -1 and lib.aussm_b200_rotate_bwd_workspace_bytes(p) == 0
+
+
+def _with_oracle(monkeypatch):
+    """The block's glue on the CPU: the oracle in place of the operators."""
+    from aussm_b200 import models
+
+    def rule(q, k, v, g, beta, **kw):
+        return gated_delta_ref(q, k, v, g, beta)[0]
+
+    def step(q, k, v, g, beta, state):
+        o, new = gated_delta_ref(q, k, v, g, beta, initial_state=state)
+        state.copy_(new)
+        return o
+
+    def rotate(q, k, frequencies=None, positions=None, **kw):
+        return tuple(norm_rotate_ref(t, frequencies, positions, **kw) for t in (q, k))
+
+    monkeypatch.setattr(models.delta, "gated_delta_rule", rule)
+    monkeypatch.setattr(models.delta, "gated_delta_step", step)
+    monkeypatch.setattr(models.rotary, "qk_norm_rotate", rotate)
+    return models
+
+
+@pytest.mark.parametrize("rotary_dim,bias", [(0, False), (8, True)])
+def test_block_steps_are_its_sequence(monkeypatch, rotary_dim, bias):
+    models = _with_oracle(monkeypatch)
+    torch.manual_seed(0)
+    block = models.GatedDeltaBlock(32, n_heads=2, rotary_dim=rotary_dim, bias=bias).double()
+    x = torch.randn(2, 9, 32, dtype=torch.float64)
+    whole = block(x)
+    cache = block.init_cache(2, dtype=torch.float64)
+    cache["state"] = cache["state"].double()
+    steps = torch.cat([block.step(x[:, t:t + 1], cache) for t in range(9)], 1)
+    assert torch.allclose(steps, whole, atol=1e-12) and cache["position"] == 9
+    assert torch.equal(whole[:, :5], block(torch.cat((x[:, :5], torch.randn(2, 4, 32, dtype=torch.float64)), 1))[:, :5])   # causal
+
+
+def test_block_in_the_models(monkeypatch):
+    models = _with_oracle(monkeypatch)
+    torch.manual_seed(0)
+    net = models.SSMTS(d_model=16, input_dim=3, output_dim=2, layers="g|g")
+    y = net(torch.randn(2, 7, 3))
+    y.square().mean().backward()
+    assert y.shape == (2, 7, 2) and all(torch.isfinite(p.grad).all() for p in net.parameters())
+    assert models.GatedDeltaBlock(512).n_heads == 4 and models.GatedDeltaBlock(96).n_heads == 1
+    for bad in (dict(d_model=30, n_heads=4), dict(d_model=512, n_heads=2), dict(d_model=32, rotary_dim=3), dict(d_model=32, n_heads=2, rotary_dim=18)):
+        with pytest.raises(ValueError):
+            models.GatedDeltaBlock(**bad)

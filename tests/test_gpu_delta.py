@@ -335,3 +335,70 @@ def test_streams_and_graph_replay():
 def test_few_heads_in_segments(l, heads, dk, dv, rate):
     """Long sequences of few heads are cut along time: lengths that fill no segment, states that live through all of it."""
     compare(both(make(l, 1, l, heads, heads, dk, dv, rate=rate)))
+
+
+@pytest.mark.parametrize("rotary_dim", [0, 32])
+def test_block(rotary_dim):
+    """The block's operators together, as a model uses them: whole sequences against single tokens, and gradients against
+    the same block in float64 with the recurrence in the operators' place."""
+    from aussm_b200 import models
+    from oracle.delta import norm_rotate_ref
+    torch.manual_seed(3)
+    block = models.GatedDeltaBlock(128, n_heads=2, rotary_dim=rotary_dim).cuda()
+    x = torch.randn(2, 150, 128, device="cuda", requires_grad=True)
+    y = block(x)
+    gy = torch.randn_like(y)
+    names, params = zip(*block.named_parameters())
+    grads = torch.autograd.grad(y, (x, *params), gy)
+    cache = block.init_cache(2, device="cuda")
+    steps = torch.cat([block.step(x[:, t:t + 1].detach(), cache) for t in range(150)], 1)
+
+    def rule(q, k, v, g, beta, **kw):
+        return gated_delta_ref(q, k, v, g, beta)[0]
+
+    def rotate(q, k, frequencies=None, positions=None, **kw):
+        return tuple(norm_rotate_ref(t, frequencies, positions, **kw) for t in (q, k))
+
+    class Wide(torch.nn.Module):             # float64: the block's gate is cast to float32 by design, so it is restated
+        def forward(self, x):
+            b, l, d = x.shape
+            xs, z = block.in_proj(x).split([3 * d, d], dim=-1)
+            conv = models._causal_depthwise_conv(block.conv1d, xs)
+            q, k, v = torch.nn.functional.silu(conv).reshape(b, l, 3, 2, 64).unbind(2)
+            f = None if not rotary_dim else block._frequencies(x.device)
+            q, k = rotate(q, k, f, norm="l2")
+            a, beta = block.gate_proj(x).split([2, 2], dim=-1)
+            g = -torch.exp(block.A_log) * torch.nn.functional.softplus(a + block.dt_bias)
+            o = rule(q, k, v, g, torch.sigmoid(beta))
+            o = o * torch.rsqrt(o.square().mean(-1, keepdim=True) + block.norm.eps) * block.norm.weight
+            return block.out_proj((o * torch.nn.functional.silu(z.reshape(b, l, 2, 64))).reshape(b, l, d))
+
+    block.double()
+    x64 = x.detach().double().requires_grad_()
+    y64 = Wide()(x64)
+    truth = torch.autograd.grad(y64, (x64, *block.parameters()), gy.double())
+    # the operators' tolerance, and as much again for the dozen float32 operations and products around them
+    close("y", y.detach(), y64.detach(), 4 * FWD)
+    close("steps", steps, y64.detach(), 4 * FWD)
+    for n, a, t in zip(("x", *names), grads, truth):
+        close("grad " + n, a, t, 4 * BWD)
+
+
+def test_models_with_delta_layers():
+    from aussm_b200 import models
+    from aussm_b200.train import GraphedTrainStep
+    torch.manual_seed(5)
+    net = models.SSMTS(d_model=64, input_dim=3, output_dim=2, layers="a|g|m").cuda()
+    x, y = torch.randn(2, 96, 3, device="cuda"), torch.randn(2, 96, 2, device="cuda")
+    loss = (net(x) - y).square().mean()
+    grads = torch.autograd.grad(loss, list(net.parameters()))
+    assert all(torch.isfinite(g).all() for g in grads)
+    del loss, grads
+    opt = torch.optim.AdamW(net.parameters(), lr=1e-3, capturable=True)
+    step = GraphedTrainStep(net, opt, x, y, lambda o, t: (o - t).square().mean())
+    assert torch.isfinite(step.step()) and torch.isfinite(step.step(x + 1, y))
+    ids = torch.randint(0, 50, (2, 70), device="cuda")
+    clf = models.SSMSequenceClassifier(d_model=64, vocab_size=50, output_dim=3, layers="g|a").cuda()
+    out = clf(ids, torch.tensor([70, 33], device="cuda"))
+    assert out.shape == (2, 3) and torch.isfinite(out).all()
+    assert aussm_b200.device_status() == 0
