@@ -8,16 +8,16 @@
 // product is converted by the thread that owns the row and goes back as the next product's A without leaving the lane.
 // A row's FP16 parts are scaled by a power of two of the row's own: no reduction between threads.
 //
-// Warps 0-7 own the state, two threads a row, each half of its columns (the chain: convert S, product, convert V',
-// product, add); warps 8-11 bring V (dO) in, a chunk ahead, through shared memory; warps 12-15 take everything out (O or X;
-// the parts of S and V' that a backward pass reads, as they lie in tensor memory); warp 16 copies the records' tiles (bulk
-// copies), warp 17 issues the MMAs (18 and 19 fill their warpgroup, which hands its registers to the others).  Tensor memory, 512
+// Warps 0-15 own the state, four threads a row, each a quarter of its columns (the chain: convert S, product, convert V',
+// product, add); warps 16-19 bring V (dO) in, a chunk ahead, through shared memory; warps 20-23 take everything out (O or X;
+// the parts of S and V' that a backward pass reads, as they lie in tensor memory); warp 24 copies the records' tiles (bulk
+// copies), warp 25 issues the MMAs (26 and 27 fill their warpgroup, which hands its registers to the others).  Tensor memory, 512
 // columns: [X | Y] take turns as the parts of S and as the product that updates it, two accumulators of 64 columns, the
 // parts of V' and of V.  Every wait is bounded: one that runs out sets the status word and the block ends.
 //
 // The roles walk different code, chunk after chunk, out of one instruction cache: with every loop unrolled the issue of 36
 // MMAs took 4700 cycles instead of 1700.  Only what must be (registers that are indexed) is unrolled, and the state's
-// conversions, the longest straight line, are cut in two halves that run side by side.
+// conversions, the longest straight line, are cut into quarters that run side by side.
 #include "common.cuh"
 #include "delta.cuh"
 #include "host_common.cuh"
@@ -26,9 +26,11 @@ namespace aussm {
 namespace {
 
 constexpr int C = kDeltaChunk;
-constexpr int THREADS = 640;             // five warpgroups; launched with 96 registers a thread, 480 for one of each
-constexpr int MAIN_REGS = 136, IN_REGS = 64, OUT_REGS = 104, REST_REGS = 40;
-static_assert(2 * MAIN_REGS + IN_REGS + OUT_REGS + REST_REGS <= 5 * 96, "more registers than the block is launched with");
+constexpr int PARTS = 4;                 // threads that share a row of the state
+constexpr int MAIN = PARTS * 4, IN = MAIN, OUT = IN + 4, COPY = OUT + 4, ISSUE = COPY + 1;     // first warp of each role
+constexpr int THREADS = (COPY + 4) * 32; // seven warpgroups; launched with 72 registers a thread, 504 for one of each
+constexpr int MAIN_REGS = 80, IN_REGS = 64, OUT_REGS = 80, REST_REGS = 40;
+static_assert(PARTS * MAIN_REGS + IN_REGS + OUT_REGS + REST_REGS <= (PARTS + 3) * 72, "more registers than the block is launched with");
 constexpr int SQUARE = DeltaRecord::kSquare;
 // tensor memory columns
 constexpr uint32_t kX = 0, kY = 128, kAcc = 256, kAcc2 = 320, kNew = 384, kVal = 448;
@@ -95,15 +97,6 @@ template <int N> __device__ __forceinline__ void more_registers() { asm volatile
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 #define R4(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
 #define W4(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3])
-__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : R4(r, 0), R4(r, 4), R4(r, 8), R4(r, 12), R4(r, 16), R4(r, 20), R4(r, 24), R4(r, 28) : "r"(t) : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-                 "%15, %16};" ::"r"(t), W4(r, 0), W4(r, 4), W4(r, 8), W4(r, 12) : "memory");
-}
 __device__ __forceinline__ void tmem_ld16(uint32_t t, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
                  "[%16];" : R4(r, 0), R4(r, 4), R4(r, 8), R4(r, 12) : "r"(t) : "memory");
@@ -146,18 +139,18 @@ template <int COUNT>
 __device__ __forceinline__ void store_parts(uint32_t t, uint32_t lo_cols, const float2 (&x)[COUNT / 2], float f) {
     const float2 f2 = make_float2(f, f), minus = make_float2(-1.f, -1.f);
 #pragma unroll
-    for (int i = 0; i < COUNT / 2; i += 16) {
-        uint32_t hi[16], lo[16];
+    for (int i = 0; i < COUNT / 2; i += 8) {
+        uint32_t hi[8], lo[8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < 8; ++j) {
             const float2 v = __fmul2_rn(x[i + j], f2);
             const __half2 h = __float22half2_rn(v);
             const __half2 l = __float22half2_rn(__ffma2_rn(__half22float2(h), minus, v));
             hi[j] = *reinterpret_cast<const uint32_t*>(&h);
             lo[j] = *reinterpret_cast<const uint32_t*>(&l);
         }
-        tmem_st16(t + i, hi);
-        tmem_st16(t + lo_cols + i, lo);
+        tmem_st8(t + i, hi);
+        tmem_st8(t + lo_cols + i, lo);
     }
 }
 template <int COUNT>
@@ -201,15 +194,15 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full_a[2], full_b, full_c, full_e, empty_a[2], empty_b, empty_c, empty_e;
     __shared__ uint64_t s_ready, v_ready, v_done, n_ready, a_done, y_free, d_done, o_done, o_free, x_free, v_loaded, v_read;
-    __shared__ uint64_t pair_s[4], pair_n[4];
+    __shared__ uint64_t row_s[4], row_n[4];
     __shared__ uint32_t holder;
-    __shared__ float un_s[2][128], un_v[128], un_n[128], max_s[2][128], max_n[2][128];
+    __shared__ float un_s[2][128], un_v[128], un_n[128], max_s[PARTS][128], max_n[PARTS][128];
     __shared__ __align__(16) float betas[C];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const aussm_b200_delta_t& p = a.p;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int bh = blockIdx.x, b = bh / p.HV, h = bh % p.HV;
-    const int me = threadIdx.x & 127, v = blockIdx.y * 128 + me;      // row (value column) of the threads of warps 0-15
+    const int me = threadIdx.x & 127, v = blockIdx.y * 128 + me;      // row (value column) of all threads but the last warpgroup's
     const int width_all = a.transition ? p.DK : p.DV;                 // value columns (a transition: the state's own keys)
     const bool mine = v < width_all;
     const int seg = a.first_seg + (int)blockIdx.z, c0 = (BWD ? a.segs - 1 - seg : seg) * a.span;
@@ -222,32 +215,32 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         for (uint64_t* x : {&full_a[0], &full_a[1], &full_b, &full_c, &full_e, &empty_a[0], &empty_a[1], &empty_b, &empty_c,
                             &empty_e, &v_done, &a_done, &d_done, &o_done})
             mbar_init(x, 1);
-        for (uint64_t* x : {&s_ready, &n_ready, &y_free}) mbar_init(x, 256);
+        for (uint64_t* x : {&s_ready, &n_ready, &y_free}) mbar_init(x, PARTS * 128);
         for (uint64_t* x : {&v_ready, &o_free, &x_free, &v_loaded, &v_read}) mbar_init(x, 128);
         for (int i = 0; i < 4; ++i) {
-            mbar_init(&pair_s[i], 64);
-            mbar_init(&pair_n[i], 64);
+            mbar_init(&row_s[i], PARTS * 32);
+            mbar_init(&row_n[i], PARTS * 32);
         }
         fence_mbar_init();
         fence_proxy_async();
     }
-    if (warp == 17) tmem_alloc512(&holder);
+    if (warp == ISSUE) tmem_alloc512(&holder);
     tc_before();
     __syncthreads();
     tc_after();
     const uint32_t tm = holder, lanes = tm + ((uint32_t)((warp & 3) * 32) << 16);
 
-    if (warp < 8) {
-        // ---- the state: columns [half * HALF, half * HALF + HALF) of row `me` ------------------------------------------
+    if (warp < MAIN) {
+        // ---- the state: columns [part * COLS, part * COLS + COLS) of row `me` ------------------------------------------
         more_registers<MAIN_REGS>();
-        constexpr int HALF = KEY / 2;
-        const int half = warp >> 2;
-        const uint32_t sc = half * HALF;                              // first column in a float32 row
-        float2 s[HALF / 2];
+        constexpr int COLS = KEY / PARTS, NEWS = C / PARTS;          // columns of S, of V' of a thread
+        const int part = warp >> 2;
+        const uint32_t sc = part * COLS;                              // first column in a float32 row
+        float2 s[COLS / 2];
         const float* from = seg == 0 ? a.s0 : a.seg_in ? a.seg_in + seg * a.seg_stride : nullptr;
         if (from) from += (size_t)bh * p.DK * p.DV + v;
 #pragma unroll
-        for (int x = 0; x < HALF / 2; ++x) {
+        for (int x = 0; x < COLS / 2; ++x) {
             const int k0 = sc + 2 * x;
             s[x] = make_float2(0.f, 0.f);
             if (a.transition) s[x] = make_float2(k0 == me ? 1.f : 0.f, k0 + 1 == me ? 1.f : 0.f);
@@ -260,12 +253,12 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         auto add = [&](uint32_t t, float keep, float f) {
             const float2 k2 = make_float2(keep, keep), f2 = make_float2(f, f);
 #pragma unroll
-            for (int x = 0; x < HALF; x += 32) {
-                uint32_t r[32];
-                tmem_ld32(t + sc + x, r);
+            for (int x = 0; x < COLS; x += 16) {
+                uint32_t r[16];
+                tmem_ld16(t + sc + x, r);
                 tc_wait_ld();
 #pragma unroll
-                for (int y = 0; y < 16; ++y)
+                for (int y = 0; y < 8; ++y)
                     s[x / 2 + y] = __ffma2_rn(make_float2(__uint_as_float(r[2 * y]), __uint_as_float(r[2 * y + 1])), f2,
                                               __fmul2_rn(s[x / 2 + y], k2));
             }
@@ -275,40 +268,40 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             const float* head = reinterpret_cast<const float*>(record(i));
             const float un1 = head[BWD ? kUnKt : kUnW], un2 = head[BWD ? kUnP : kUnT], un3 = head[BWD ? kUnW : kUnKt],
                         unq = head[kUnQ], gamma = head[kGamma];
-            // one power of two for the whole row: the halves tell each other their maxima
-            max_s[half][me] = row_max(s);
-            arrive(&pair_s[warp & 3]);
-            if (!warp_wait(&pair_s[warp & 3], ph, a.status)) break;
-            const int es = part_exponent(fmaxf(max_s[0][me], max_s[1][me]));
+            // one power of two for the whole row: its threads tell each other their maxima
+            max_s[part][me] = row_max(s);
+            arrive(&row_s[warp & 3]);
+            if (!warp_wait(&row_s[warp & 3], ph, a.status)) break;
+            const int es = part_exponent(fmaxf(fmaxf(max_s[0][me], max_s[1][me]), fmaxf(max_s[2][me], max_s[3][me])));
             const float uns = pow2_float(-es);
-            store_parts<HALF>(X + half * (HALF / 2), KEY / 2, s, pow2_float(es));
-            if (half == 0) un_s[ph][me] = uns;
+            store_parts<COLS>(X + part * (COLS / 2), KEY / 2, s, pow2_float(es));
+            if (part == 0) un_s[ph][me] = uns;
             tc_wait_st();
             tc_before();
             arrive(&s_ready);
-            // V' (dV'), columns [32 half, 32 half + 32)
+            // V' (dV'), columns [NEWS part, NEWS part + NEWS)
             if (!warp_wait(&v_done, ph, a.status) || !warp_wait(&v_ready, ph, a.status)) break;
             tc_after();
             const float unv = un_v[me], f1 = (BWD ? uns : -uns) * un1, f2 = unv * un2;
-            float2 w[16];
+            float2 w[NEWS / 2];
             {
-                uint32_t r1[32], r2[32];
-                tmem_ld32(lanes + kAcc + half * 32, r1);
-                tmem_ld32(lanes + kAcc2 + half * 32, r2);
+                uint32_t r1[NEWS], r2[NEWS];
+                tmem_ld16(lanes + kAcc + part * NEWS, r1);
+                tmem_ld16(lanes + kAcc2 + part * NEWS, r2);
                 tc_wait_ld();
 #pragma unroll
-                for (int y = 0; y < 16; ++y)
+                for (int y = 0; y < NEWS / 2; ++y)
                     w[y] = __ffma2_rn(make_float2(__uint_as_float(r1[2 * y]), __uint_as_float(r1[2 * y + 1])), make_float2(f1, f1),
                                       __fmul2_rn(make_float2(__uint_as_float(r2[2 * y]), __uint_as_float(r2[2 * y + 1])), make_float2(f2, f2)));
             }
-            max_n[half][me] = row_max(w);
-            arrive(&pair_n[warp & 3]);
-            if (!warp_wait(&pair_n[warp & 3], ph, a.status)) break;
-            const int en = part_exponent(fmaxf(max_n[0][me], max_n[1][me]));
+            max_n[part][me] = row_max(w);
+            arrive(&row_n[warp & 3]);
+            if (!warp_wait(&row_n[warp & 3], ph, a.status)) break;
+            const int en = part_exponent(fmaxf(fmaxf(max_n[0][me], max_n[1][me]), fmaxf(max_n[2][me], max_n[3][me])));
             const float unn = pow2_float(-en);
             if (full && i && !warp_wait(&x_free, ph ^ 1, a.status)) break;      // the last V' has been taken out
-            store_parts<32>(lanes + kNew + half * 16, C / 2, w, pow2_float(en));
-            if (half == 0) un_n[me] = unn;
+            store_parts<NEWS>(lanes + kNew + part * (NEWS / 2), C / 2, w, pow2_float(en));
+            if (part == 0) un_n[me] = unn;
             tc_wait_st();
             tc_before();
             arrive(&n_ready);
@@ -328,13 +321,13 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             const int pitch = a.transition ? KEY : p.DV;
             to += (size_t)bh * (a.transition ? KEY : p.DK) * pitch + v;
 #pragma unroll
-            for (int x = 0; x < HALF / 2; ++x) {
+            for (int x = 0; x < COLS / 2; ++x) {
                 const int k0 = sc + 2 * x;
                 if (k0 < p.DK) to[(size_t)k0 * pitch] = s[x].x;
                 if (k0 + 1 < p.DK) to[(size_t)(k0 + 1) * pitch] = s[x].y;
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < OUT) {
         // ---- V (dO) in -------------------------------------------------------------------------------------------
         fewer_registers<IN_REGS>();
         const T* src = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + blockIdx.y * 128;
@@ -418,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             }
         }
         cp_async_wait<0>();
-    } else if (warp < 16) {
+    } else if (warp < COPY) {
         // ---- O (X), states and V' out ------------------------------------------------------------------------------
         more_registers<OUT_REGS>();
         T* dst = static_cast<T*>(a.out) + ((long long)b * p.L * p.HV + h) * p.DV + v;
@@ -445,34 +438,35 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             if (!warp_wait(&n_ready, ph, a.status) || !warp_wait(&o_done, ph, a.status)) break;
             tc_after();
             const float uns = un_s[ph][me], f1 = uns * unq, unn = un_n[me], f2 = unn * un2;
-            // all of it to registers first: the accumulators are wanted back
-            float y[C];
-#pragma unroll
+            T* to = dst + (long long)t0 * p.HV * p.DV;
+            float4* keep = reinterpret_cast<float4*>(a.rows) + at * (C / 4 * 128) + me;
+            const float4* be = reinterpret_cast<const float4*>(head + kBeta);
+#pragma unroll 1
             for (int t = 0; t < C; t += 16) {
                 uint32_t r1[16], r2[16];
+                float y[16];
                 if (!BWD) tmem_ld16(lanes + kAcc + t, r1);
                 tmem_ld16(lanes + kAcc2 + t, r2);
                 tc_wait_ld();
+                if (t + 16 == C) {               // the accumulators are wanted back
+                    tc_before();
+                    arrive(&o_free);
+                }
 #pragma unroll
                 for (int u = 0; u < 16; ++u)
-                    y[t + u] = BWD ? __uint_as_float(r2[u]) * f2 : fmaf(__uint_as_float(r1[u]), f1, __uint_as_float(r2[u]) * f2);
-            }
-            tc_before();
-            arrive(&o_free);
-            T* to = dst + (long long)t0 * p.HV * p.DV;
-            if (BWD && mine) {
-                float4* keep = reinterpret_cast<float4*>(a.rows) + at * (C / 4 * 128) + me;
-                const float4* be = reinterpret_cast<const float4*>(head + kBeta);
+                    y[u] = BWD ? __uint_as_float(r2[u]) * f2 : fmaf(__uint_as_float(r1[u]), f1, __uint_as_float(r2[u]) * f2);
+                if (BWD) {
 #pragma unroll
-                for (int t = 0; t < C; t += 4) {
-                    keep[t / 4 * 128] = make_float4(y[t], y[t + 1], y[t + 2], y[t + 3]);
-                    const float4 f = be[t / 4];
-                    y[t] *= f.x; y[t + 1] *= f.y; y[t + 2] *= f.z; y[t + 3] *= f.w;
+                    for (int u = 0; u < 16; u += 4) {
+                        if (mine) keep[(t + u) / 4 * 128] = make_float4(y[u], y[u + 1], y[u + 2], y[u + 3]);
+                        const float4 f = be[(t + u) / 4];
+                        y[u] *= f.x; y[u + 1] *= f.y; y[u + 2] *= f.z; y[u + 3] *= f.w;
+                    }
                 }
-            }
 #pragma unroll
-            for (int t = 0; t < C; ++t, to += out_step)
-                if (t < rows) *to = from_f32<T>(y[t]);
+                for (int u = 0; u < 16; ++u, to += out_step)
+                    if (t + u < rows) *to = from_f32<T>(y[u]);
+            }
             if (a.states) {
                 uint4* st = a.states + at * (KEY / 4 * 128 + 32);
                 dump(lanes + (ph ? kY : kX), KEY, st);
@@ -488,7 +482,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         }
     } else {
         fewer_registers<REST_REGS>();
-        if (warp == 16 && lane == 0) {
+        if (warp == COPY && lane == 0) {
             // ---- copies ------------------------------------------------------------------------------------------
             const int tile_a = BWD ? a.rec.kt() : a.rec.w(), square_a = BWD ? a.rec.p() : a.rec.t();
             const int tile_b = BWD ? a.rec.w() : a.rec.kt(), square_e = BWD ? a.rec.t() : a.rec.p();
@@ -525,7 +519,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 if (full || BWD) poll(&full_c, (done_b - 1) & 1, a.status);
                 if (full) poll(&full_e, (done_b - 1) & 1, a.status);
             }
-        } else if (warp == 17) {
+        } else if (warp == ISSUE) {
             // ---- MMAs --------------------------------------------------------------------------------------------
             const uint32_t base = smem_addr(sm), one = elect_one(), tm = __shfl_sync(0xffffffffu, holder, 0);
             auto wait = [&](uint64_t* bar, uint32_t ph) { return warp_wait(bar, ph, a.status); };
@@ -569,7 +563,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == 17) tmem_dealloc512(tm);
+    if (warp == ISSUE) tmem_dealloc512(tm);
 }
 
 // States at the segments' boundaries, from what each segment makes of a zero state and what it does to a state:
