@@ -182,8 +182,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* s
 template <typename T, int KEY>
 struct ScanSmem {
     static constexpr int kTile = KEY * 256;
-    // phase 1 operands twice (tile, square), then the two tiles and the square of the later phases, then V (dO)
-    static constexpr int kA = 0, kB = 2 * (kTile + SQUARE), kC = kB + kTile, kE = kC + kTile, kV = kE + SQUARE,
+    // A: the operands of phase 1 (tile, square), B and E: tile and square of the later phases, twice, C: Qt, then V (dO).
+    // A and C are wanted late after they are free again; B and E copied only then were waited for 1200 to 2200 cycles a chunk.
+    static constexpr int kA = 0, kB = kTile + SQUARE, kC = kB + 2 * kTile, kE = kC + kTile, kV = kE + 2 * SQUARE,
                          kBytes = kV + C * 128 * (int)sizeof(T) + 1024;
 };
 
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     using Smem = ScanSmem<T, KEY>;
     constexpr int TILE = Smem::kTile, LO = KEY * 128, SQ_LO = 8192;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t full_a[2], full_b, full_c, full_e, empty_a[2], empty_b, empty_c, empty_e;
+    __shared__ uint64_t full_a, full_b[2], full_c, full_e[2], empty_a, empty_b[2], empty_c, empty_e[2];
     __shared__ uint64_t s_ready, v_ready, v_done, n_ready, a_done, y_free, d_done, o_done, o_free, x_free, v_loaded, v_read;
     __shared__ uint64_t row_s[4], row_n[4];
     __shared__ uint32_t holder;
@@ -212,8 +213,8 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     auto record = [&](int i) { return a.records + ((size_t)bh * a.n + chunk_at(i)) * a.rec.bytes(); };
 
     if (threadIdx.x == 0) {
-        for (uint64_t* x : {&full_a[0], &full_a[1], &full_b, &full_c, &full_e, &empty_a[0], &empty_a[1], &empty_b, &empty_c,
-                            &empty_e, &v_done, &a_done, &d_done, &o_done})
+        for (uint64_t* x : {&full_a, &full_b[0], &full_b[1], &full_c, &full_e[0], &full_e[1], &empty_a, &empty_b[0], &empty_b[1],
+                            &empty_c, &empty_e[0], &empty_e[1], &v_done, &a_done, &d_done, &o_done})
             mbar_init(x, 1);
         for (uint64_t* x : {&s_ready, &n_ready, &y_free}) mbar_init(x, PARTS * 128);
         for (uint64_t* x : {&v_ready, &o_free, &x_free, &v_loaded, &v_read}) mbar_init(x, 128);
@@ -486,38 +487,36 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             // ---- copies ------------------------------------------------------------------------------------------
             const int tile_a = BWD ? a.rec.kt() : a.rec.w(), square_a = BWD ? a.rec.p() : a.rec.t();
             const int tile_b = BWD ? a.rec.w() : a.rec.kt(), square_e = BWD ? a.rec.t() : a.rec.p();
-            int done_a = 0, done_b = 0;
+            const bool c = full || BWD;                         // Qt: for O, or for the backward state
+            auto copy = [&](uint64_t* bar, int to, const uint8_t* from, int bytes) {
+                mbar_arrive_expect_tx(bar, bytes);
+                bulk_g2s(sm + to, from, bytes, bar);
+            };
+            int na = 0, nb = 0, nc = 0;                         // copies under way or done
             for (int i = 0; i < count; ++i) {
                 const uint8_t* rec = record(i);
                 const int st = i & 1;
-                if (i >= 2 && !poll(&empty_a[st], ((i >> 1) - 1) & 1, a.status)) break;
-                uint8_t* to = sm + Smem::kA + st * (TILE + SQUARE);
-                mbar_arrive_expect_tx(&full_a[st], TILE + SQUARE);
-                bulk_g2s(to, rec + tile_a, TILE, &full_a[st]);
-                bulk_g2s(to + TILE, rec + square_a, SQUARE, &full_a[st]);
-                done_a = i + 1;
-                const bool c = full || BWD;                     // Qt: for O, or for the backward state
-                if (i >= 1 && (!poll(&empty_b, (i - 1) & 1, a.status) || (c && !poll(&empty_c, (i - 1) & 1, a.status)) ||
-                               (full && !poll(&empty_e, (i - 1) & 1, a.status))))
-                    break;
-                mbar_arrive_expect_tx(&full_b, TILE);
-                bulk_g2s(sm + Smem::kB, rec + tile_b, TILE, &full_b);
+                if (i && !poll(&empty_a, (i - 1) & 1, a.status)) break;
+                mbar_arrive_expect_tx(&full_a, TILE + SQUARE);
+                bulk_g2s(sm + Smem::kA, rec + tile_a, TILE, &full_a);
+                bulk_g2s(sm + Smem::kA + TILE, rec + square_a, SQUARE, &full_a);
+                na = i + 1;
+                if (i >= 2 && (!poll(&empty_b[st], ((i >> 1) - 1) & 1, a.status) || (full && !poll(&empty_e[st], ((i >> 1) - 1) & 1, a.status)))) break;
+                copy(&full_b[st], Smem::kB + st * TILE, rec + tile_b, TILE);
+                if (full) copy(&full_e[st], Smem::kE + st * SQUARE, rec + square_e, SQUARE);
+                nb = i + 1;
                 if (c) {
-                    mbar_arrive_expect_tx(&full_c, TILE);
-                    bulk_g2s(sm + Smem::kC, rec + a.rec.q(), TILE, &full_c);
+                    if (i && !poll(&empty_c, (i - 1) & 1, a.status)) break;
+                    copy(&full_c, Smem::kC, rec + a.rec.q(), TILE);
+                    nc = i + 1;
                 }
-                if (full) {
-                    mbar_arrive_expect_tx(&full_e, SQUARE);
-                    bulk_g2s(sm + Smem::kE, rec + square_e, SQUARE, &full_e);
-                }
-                done_b = i + 1;
             }
             // no copy may be in flight when the block ends, also not when a wait ran out
-            for (int i = max(0, done_a - 2); i < done_a; ++i) poll(&full_a[i & 1], (i >> 1) & 1, a.status);
-            if (done_b) {
-                poll(&full_b, (done_b - 1) & 1, a.status);
-                if (full || BWD) poll(&full_c, (done_b - 1) & 1, a.status);
-                if (full) poll(&full_e, (done_b - 1) & 1, a.status);
+            if (na) poll(&full_a, (na - 1) & 1, a.status);
+            if (nc) poll(&full_c, (nc - 1) & 1, a.status);
+            for (int i = max(0, nb - 2); i < nb; ++i) {
+                poll(&full_b[i & 1], (i >> 1) & 1, a.status);
+                if (full) poll(&full_e[i & 1], (i >> 1) & 1, a.status);
             }
         } else if (warp == ISSUE) {
             // ---- MMAs --------------------------------------------------------------------------------------------
@@ -525,15 +524,15 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             auto wait = [&](uint64_t* bar, uint32_t ph) { return warp_wait(bar, ph, a.status); };
             for (int i = 0; i < count; ++i) {
                 const uint32_t ph = i & 1, X = tm + (ph ? kY : kX), Y = tm + (ph ? kX : kY);
-                const uint32_t ta = base + Smem::kA + ph * (TILE + SQUARE);
-                if (!wait(&full_a[ph], (i >> 1) & 1) || !wait(&v_ready, ph) || (full && i && !wait(&o_free, ph ^ 1))) break;
+                const uint32_t ta = base + Smem::kA, half = (i >> 1) & 1;
+                if (!wait(&full_a, ph) || !wait(&v_ready, ph) || (full && i && !wait(&o_free, ph ^ 1))) break;
                 tc_after();
                 product<C, C / 16, BWD>(tm + kAcc2, tm + kVal, ta + TILE, SQ_LO, one);       // no state in it
                 if (!wait(&s_ready, ph)) break;
                 tc_after();
                 product<C, KEY / 16, false>(tm + kAcc, X, ta, LO, one);
                 commit(&v_done, one);
-                commit(&empty_a[ph], one);
+                commit(&empty_a, one);
                 if (BWD) {
                     if (!wait(&full_c, ph) || (full && i && !wait(&x_free, ph ^ 1))) break;
                     product<KEY, C / 16, true>(Y, tm + kVal, base + Smem::kC, LO, one);
@@ -542,21 +541,21 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                     if (!wait(&y_free, ph)) break;
                 }
                 // Y held the parts of the state before this one: they have been taken out.  V' comes last.
-                if (!wait(&full_b, ph) || (full && (!wait(&full_e, ph) || (!BWD && !wait(&full_c, ph)) || (i && !wait(&x_free, ph ^ 1)))) ||
+                if (!wait(&full_b[ph], half) || (full && (!wait(&full_e[ph], half) || (!BWD && !wait(&full_c, ph)) || (i && !wait(&x_free, ph ^ 1)))) ||
                     !wait(&n_ready, ph))
                     break;
                 tc_after();
-                product<KEY, C / 16, true>(Y, tm + kNew, base + Smem::kB, LO, one);
+                product<KEY, C / 16, true>(Y, tm + kNew, base + Smem::kB + ph * TILE, LO, one);
                 commit(&d_done, one);
-                commit(&empty_b, one);
+                commit(&empty_b[ph], one);
                 if (!full) continue;
                 if (!BWD) {
                     product<C, KEY / 16, false>(tm + kAcc, X, base + Smem::kC, LO, one);
                     commit(&empty_c, one);
                 }
-                product<C, C / 16, BWD>(tm + kAcc2, tm + kNew, base + Smem::kE, SQ_LO, one);
+                product<C, C / 16, BWD>(tm + kAcc2, tm + kNew, base + Smem::kE + ph * SQUARE, SQ_LO, one);
                 commit(&o_done, one);
-                commit(&empty_e, one);
+                commit(&empty_e[ph], one);
             }
         }
     }
