@@ -87,11 +87,10 @@ __device__ __forceinline__ void commit(uint64_t* bar, uint32_t one) {
                  ::"r"(smem_addr(bar)), "r"(one) : "memory");
 }
 // A from tensor memory, B from shared memory
-template <bool ACCUMULATE>
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t one) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t one) {
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
                  "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "n"(ACCUMULATE ? 1 : 0), "r"(one) : "memory");
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
 }
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -123,14 +122,15 @@ template <int N, int STEPS, bool MN>
 __device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, int b_lo, uint32_t one) {
     constexpr uint32_t id = idesc(N, MN);
     constexpr uint32_t A_LO = STEPS * 8;
-    const uint64_t first = row_desc(b, MN ? 8192 : 16);
-#pragma unroll
+    uint64_t bh = row_desc(b, MN ? 8192 : 16);
+    const uint64_t lo = (uint32_t)(b_lo >> 4);
+#pragma unroll 1
     for (int k = 0; k < STEPS; ++k) {
-        const uint64_t bh = first + (uint32_t)((MN ? k * 2048 : (k >> 2) * 8192 + (k & 3) * 32) >> 4), bl = bh + (uint32_t)(b_lo >> 4);
-        if (k == 0) mma_ts<false>(d, a + A_LO, bh, id, one);
-        else mma_ts<true>(d, a + A_LO + k * 8, bh, id, one);
-        mma_ts<true>(d, a + k * 8, bl, id, one);
-        mma_ts<true>(d, a + k * 8, bh, id, one);
+        mma_ts(d, a + A_LO, bh, id, k > 0, one);
+        mma_ts(d, a, bh + lo, id, 1, one);
+        mma_ts(d, a, bh, id, 1, one);
+        a += 8;
+        bh += MN ? 2048 >> 4 : (k & 3) == 3 ? (8192 - 96) >> 4 : 32 >> 4;
     }
 }
 
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     __shared__ uint64_t s_ready, v_ready, v_done, n_ready, a_done, y_free, d_done, o_done, o_free, x_free, v_loaded, v_read;
     __shared__ uint64_t row_s[4], row_n[4];
     __shared__ uint32_t holder;
-    __shared__ float un_s[2][128], un_v[128], un_n[128], max_s[PARTS][128], max_n[PARTS][128];
+    __shared__ float un_s[2][128], un_v[2][128], un_n[128], max_s[PARTS][128], max_n[PARTS][128];
     __shared__ __align__(16) float betas[C];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const aussm_b200_delta_t& p = a.p;
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             // V' (dV'), columns [NEWS part, NEWS part + NEWS)
             if (!warp_wait(&v_done, ph, a.status) || !warp_wait(&v_ready, ph, a.status)) break;
             tc_after();
-            const float unv = un_v[me], f1 = (BWD ? uns : -uns) * un1, f2 = unv * un2;
+            const float unv = un_v[ph][me], f1 = (BWD ? uns : -uns) * un1, f2 = unv * un2;
             float2 w[NEWS / 2];
             {
                 uint32_t r1[NEWS], r2[NEWS];
@@ -357,12 +357,12 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             }
             cp_async_commit();
         };
-        // chunk i's row of this lane from shared memory to the parts in tensor memory; false: a wait ran out
-        auto hand_over = [&](int i) {
+        fetch(0);
+        for (int i = 0; i < count; ++i) {
             const int rows = me < width ? min(C, p.L - chunk_at(i) * C) : 0;
             cp_async_wait<0>();
             arrive(&v_loaded);
-            if (!warp_wait(&v_loaded, i & 1, a.status)) return false;
+            if (!warp_wait(&v_loaded, i & 1, a.status)) break;
             float m = 0.f;
 #pragma unroll 1
             for (int x = 0; x < C; x += 16)
@@ -373,6 +373,11 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 }
             const int e = part_exponent(m);
             const float scale = pow2_float(e);
+            // the products with chunk i - 1 are done: this one's parts go in
+            if (i) {
+                if (!warp_wait(BWD ? &a_done : &v_done, (i - 1) & 1, a.status)) break;
+                tc_after();
+            }
 #pragma unroll 1
             for (int x = 0; x < C; x += 16) {
                 uint32_t hi[8], lo[8];
@@ -390,21 +395,10 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 tmem_st8(lanes + kVal + x / 2, hi);
                 tmem_st8(lanes + kVal + C / 2 + x / 2, lo);
             }
-            un_v[me] = pow2_float(-e);
+            un_v[i & 1][me] = pow2_float(-e);
             tc_wait_st();
             tc_before();
             arrive(&v_ready);
-            return true;
-        };
-        fetch(0);
-        for (int i = 0; i < count; ++i) {
-            // the products with chunk i - 1 are done: this one's parts go in, and the next rows are on their way
-            if (i) {
-                const uint32_t ph = (i - 1) & 1;
-                if (!warp_wait(BWD ? &a_done : &v_done, ph, a.status) || !warp_wait(&n_ready, ph, a.status)) break;
-                tc_after();
-            }
-            if (!hand_over(i)) break;
             if (i + 1 < count) {
                 arrive(&v_read);
                 if (!warp_wait(&v_read, i & 1, a.status)) break;             // all lanes have read their rows
@@ -567,22 +561,21 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
 
 // States at the segments' boundaries, from what each segment makes of a zero state and what it does to a state:
 //     S_1 = N_0,   S_{z+1} = M_z S_z + N_z     (backward M^T of the mirrored segment),
-// S_{z+1} in the place of N_z.  A block owns 16 value columns of a head and keeps their states in shared memory, where the
-// next M is on its way (M is stored with KEY columns a row) while this one is worked on: a thread adds up rows r, r + 32, ..
-// of two columns in float32.
-constexpr int CHAIN_COLS = 16;
-template <int KEY>
+// S_{z+1} in the place of N_z.  A block owns CHAIN_COLS value columns of a head and keeps their states in shared memory, where the
+// next M is on its way (M is stored with KEY columns a row) while this one is worked on: a thread adds up some
+// rows of two columns in float32.
+template <int KEY, int CHAIN_COLS>
 struct ChainSmem {
     static constexpr int kPitch = KEY + 4;               // floats of a row of M: neighbouring rows in other banks
     static constexpr int kBytes = (2 * KEY * kPitch + KEY * CHAIN_COLS) * 4;
 };
-template <int KEY, bool BWD>
+template <int KEY, bool BWD, int CHAIN_COLS>
 __global__ void __launch_bounds__(256) delta_chain_kernel(const float* m, float* ends, int dk, int dv, int segs, size_t m_stride,
                                                           size_t end_stride) {
-    constexpr int PITCH = ChainSmem<KEY>::kPitch, ROWS = KEY / 32;
+    constexpr int PITCH = ChainSmem<KEY, CHAIN_COLS>::kPitch, LANES = CHAIN_COLS / 2, STEP = 256 / LANES, ROWS = KEY / STEP;
     extern __shared__ __align__(16) float chain[];
-    float* s = chain + 2 * KEY * PITCH;                  // [KEY][16]
-    const int bh = blockIdx.x, v0 = blockIdx.y * CHAIN_COLS, col = (threadIdx.x & 7) * 2, row = threadIdx.x >> 3;
+    float* s = chain + 2 * KEY * PITCH;                  // [KEY][CHAIN_COLS]
+    const int bh = blockIdx.x, v0 = blockIdx.y * CHAIN_COLS, col = threadIdx.x % LANES * 2, row = threadIdx.x / LANES;
     float* end = ends + (size_t)bh * dk * dv + v0 + col;
     const bool in0 = v0 + col < dv, in1 = v0 + col + 1 < dv;
     auto fetch = [&](int z) {
@@ -595,7 +588,7 @@ __global__ void __launch_bounds__(256) delta_chain_kernel(const float* m, float*
     fetch(1);
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const int x = row + 32 * i;
+        const int x = row + STEP * i;
         const bool there = x < dk;
         *reinterpret_cast<float2*>(s + x * CHAIN_COLS + col) =
             make_float2(there && in0 ? end[(size_t)x * dv] : 0.f, there && in1 ? end[(size_t)x * dv + 1] : 0.f);
@@ -605,33 +598,62 @@ __global__ void __launch_bounds__(256) delta_chain_kernel(const float* m, float*
         float2 acc[ROWS];
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            const int x = row + 32 * i;
+            const int x = row + STEP * i;
             acc[i] = make_float2(x < dk && in0 ? to[(size_t)x * dv] : 0.f, x < dk && in1 ? to[(size_t)x * dv + 1] : 0.f);
         }
         cp_async_wait<0>();
         __syncthreads();                                 // M and the states are there, the other M is free
         if (z + 1 < segs - 1) fetch(z + 1);
         const float* M = chain + (z & 1) * KEY * PITCH;
-#pragma unroll 8
-        for (int x = 0; x < dk; ++x) {
+#pragma unroll 2
+        for (int x = 0; x + 4 <= dk; x += 4) {
+            float w[ROWS][4];
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                if (BWD) {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) w[i][y] = M[(x + y) * PITCH + row + STEP * i];
+                } else {
+                    const float4 v = *reinterpret_cast<const float4*>(M + (row + STEP * i) * PITCH + x);
+                    w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const float2 f = *reinterpret_cast<const float2*>(s + (x + y) * CHAIN_COLS + col);
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) acc[i] = __ffma2_rn(make_float2(w[i][y], w[i][y]), f, acc[i]);
+            }
+        }
+        for (int x = dk & ~3; x < dk; ++x) {             // what is behind dk in M was never written
             const float2 f = *reinterpret_cast<const float2*>(s + x * CHAIN_COLS + col);
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
-                const float w = BWD ? M[x * PITCH + row + 32 * i] : M[(row + 32 * i) * PITCH + x];
-                acc[i].x = fmaf(w, f.x, acc[i].x);
-                acc[i].y = fmaf(w, f.y, acc[i].y);
+                const float w = BWD ? M[x * PITCH + row + STEP * i] : M[(row + STEP * i) * PITCH + x];
+                acc[i] = __ffma2_rn(make_float2(w, w), f, acc[i]);
             }
         }
         __syncthreads();                                 // the states have been read
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            const int x = row + 32 * i;
-            if (x >= dk) continue;                       // (M has no such rows)
+            const int x = row + STEP * i;
+            if (x >= dk) continue;
             *reinterpret_cast<float2*>(s + x * CHAIN_COLS + col) = acc[i];
             if (in0) to[(size_t)x * dv] = acc[i].x;
             if (in1) to[(size_t)x * dv + 1] = acc[i].y;
         }
     }
+}
+
+template <int KEY, bool BWD, int CHAIN_COLS>
+cudaError_t chain(const float* m, float* ends, int heads, int dk, int dv, int segs, cudaStream_t st) {
+    constexpr int smem = ChainSmem<KEY, CHAIN_COLS>::kBytes;
+    cudaError_t e = cudaFuncSetAttribute(delta_chain_kernel<KEY, BWD, CHAIN_COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    delta_chain_kernel<KEY, BWD, CHAIN_COLS><<<dim3(heads, (dv + CHAIN_COLS - 1) / CHAIN_COLS), 256, smem, st>>>(
+        m, ends, dk, dv, segs, (size_t)heads * KEY * KEY, (size_t)heads * dk * dv);
+    count_launch();
+    return cudaGetLastError();
 }
 
 template <typename T, int KEY, bool BWD>
@@ -655,11 +677,11 @@ cudaError_t scan(ScanParams a, const DeltaPlan& plan, float* m, float* ends, cud
         delta_scan_kernel<T, KEY, BWD><<<dim3(heads, plan.slices, segs - 1), THREADS, smem, st>>>(q);
         count_launch();
         if (segs > 2) {
-            e = cudaFuncSetAttribute(delta_chain_kernel<KEY, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChainSmem<KEY>::kBytes);
+            // 8 columns a block are quicker than 16 while each has an SM (4 heads of 128, 36 segments: 102 against 125 us,
+            // 32 heads, 4 segments: 29 against 18 us)
+            e = heads * ((a.p.DV + 7) / 8) <= 148 ? chain<KEY, BWD, 8>(m, ends, heads, a.p.DK, a.p.DV, segs, st)
+                                                  : chain<KEY, BWD, 16>(m, ends, heads, a.p.DK, a.p.DV, segs, st);
             if (e != cudaSuccess) return e;
-            delta_chain_kernel<KEY, BWD><<<dim3(heads, (a.p.DV + CHAIN_COLS - 1) / CHAIN_COLS), 256, ChainSmem<KEY>::kBytes, st>>>(
-                m, ends, a.p.DK, a.p.DV, segs, m_stride, end_stride);
-            count_launch();
         }
         a.seg_in = ends - end_stride;        // segment z starts from the state behind segment z - 1
         a.seg_stride = end_stride;

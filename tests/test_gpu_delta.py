@@ -331,7 +331,7 @@ def test_streams_and_graph_replay():
         torch.autograd.grad(alive.sum(), x["g"])
 
 
-@pytest.mark.parametrize("l,heads,dk,dv,rate", [(800, 1, 128, 128, 0.01), (1111, 3, 64, 64, 1e-3), (2500, 2, 72, 100, 0.1), (1030, 1, 128, 200, 1.0)])
+@pytest.mark.parametrize("l,heads,dk,dv,rate", [(800, 1, 128, 128, 0.01), (1111, 3, 64, 64, 1e-3), (2500, 2, 72, 100, 0.1), (1030, 1, 128, 200, 1.0), (1400, 1, 70, 33, 0.02)])
 def test_few_heads_in_segments(l, heads, dk, dv, rate):
     """Long sequences of few heads are cut along time: lengths that fill no segment, states that live through all of it."""
     compare(both(make(l, 1, l, heads, heads, dk, dv, rate=rate)))
