@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         const T* src = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + blockIdx.y * 128;
         T* tile = reinterpret_cast<T*>(sm + Smem::kV);
         const int width = a.transition ? 0 : min(128, p.DV - (int)blockIdx.y * 128);
-        // rows of chunk i to shared memory, [64][128]: 16-byte pieces in flight, or each lane its own column
+        // rows of chunk i to shared memory, [64][128]: 16-byte pieces in flight, or each lane its own column.  Columns
+        // behind the width stay the zeros of the start, rows behind the end are cleared: no selects in the conversions.
         auto fetch = [&](int i) {
             const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
             const T* from = src + (long long)t0 * a.v_stride[1];
@@ -355,23 +356,33 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
 #pragma unroll 4
                 for (int row = 0; row < rows; ++row) tile[row * 128 + me] = from[row * a.v_stride[1] + me];
             }
+            for (int row = rows; row < C; ++row) tile[row * 128 + me] = from_f32<T>(0.f);
             cp_async_commit();
         };
+        for (int row = 0; row < C; ++row) tile[row * 128 + me] = from_f32<T>(0.f);
+        arrive(&v_read);
+        if (warp_wait(&v_read, 0, a.status)) {
         fetch(0);
         for (int i = 0; i < count; ++i) {
-            const int rows = me < width ? min(C, p.L - chunk_at(i) * C) : 0;
             cp_async_wait<0>();
             arrive(&v_loaded);
             if (!warp_wait(&v_loaded, i & 1, a.status)) break;
-            float m = 0.f;
+            // two steps of this lane's column, times beta
+            auto pair = [&](int t) {
+                float2 f = make_float2(to_f32(tile[t * 128 + me]), to_f32(tile[(t + 1) * 128 + me]));
+                if (!BWD) f = __fmul2_rn(f, *reinterpret_cast<const float2*>(betas + t));
+                return f;
+            };
+            float m0 = 0.f, m1 = 0.f;
 #pragma unroll 1
             for (int x = 0; x < C; x += 16)
 #pragma unroll
-                for (int y = 0; y < 16; ++y) {
-                    const float f = to_f32(tile[(x + y) * 128 + me]) * (BWD ? 1.f : betas[x + y]);
-                    m = fmaxf(m, x + y < rows ? fabsf(f) : 0.f);
+                for (int y = 0; y < 16; y += 2) {
+                    const float2 f = pair(x + y);
+                    m0 = fmaxf(m0, fabsf(f.x));
+                    m1 = fmaxf(m1, fabsf(f.y));
                 }
-            const int e = part_exponent(m);
+            const int e = part_exponent(fmaxf(m0, m1));
             const float scale = pow2_float(e);
             // the products with chunk i - 1 are done: this one's parts go in
             if (i) {
@@ -380,20 +391,10 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             }
 #pragma unroll 1
             for (int x = 0; x < C; x += 16) {
-                uint32_t hi[8], lo[8];
+                float2 f[8];
 #pragma unroll
-                for (int y = 0; y < 8; ++y) {
-                    float f[2];
-#pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        const int t = x + 2 * y + z;
-                        const float g = to_f32(tile[t * 128 + me]) * (BWD ? 1.f : betas[t]);
-                        f[z] = t < rows ? g * scale : 0.f;
-                    }
-                    split2(f[0], f[1], hi[y], lo[y]);
-                }
-                tmem_st8(lanes + kVal + x / 2, hi);
-                tmem_st8(lanes + kVal + C / 2 + x / 2, lo);
+                for (int y = 0; y < 8; ++y) f[y] = pair(x + 2 * y);
+                store_parts<16>(lanes + kVal + x / 2, C / 2, f, scale);
             }
             un_v[i & 1][me] = pow2_float(-e);
             tc_wait_st();
@@ -401,9 +402,10 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             arrive(&v_ready);
             if (i + 1 < count) {
                 arrive(&v_read);
-                if (!warp_wait(&v_read, i & 1, a.status)) break;             // all lanes have read their rows
+                if (!warp_wait(&v_read, (i + 1) & 1, a.status)) break;       // all lanes have read their rows
                 fetch(i + 1);
             }
+        }
         }
         cp_async_wait<0>();
     } else if (warp < COPY) {
@@ -448,8 +450,12 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                     arrive(&o_free);
                 }
 #pragma unroll
-                for (int u = 0; u < 16; ++u)
-                    y[u] = BWD ? __uint_as_float(r2[u]) * f2 : fmaf(__uint_as_float(r1[u]), f1, __uint_as_float(r2[u]) * f2);
+                for (int u = 0; u < 16; u += 2) {
+                    const float2 v = __fmul2_rn(make_float2(__uint_as_float(r2[u]), __uint_as_float(r2[u + 1])), make_float2(f2, f2));
+                    const float2 w = BWD ? v : __ffma2_rn(make_float2(__uint_as_float(r1[u]), __uint_as_float(r1[u + 1])), make_float2(f1, f1), v);
+                    y[u] = w.x;
+                    y[u + 1] = w.y;
+                }
                 if (BWD) {
 #pragma unroll
                     for (int u = 0; u < 16; u += 4) {
@@ -458,9 +464,14 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                         y[u] *= f.x; y[u + 1] *= f.y; y[u + 2] *= f.z; y[u + 3] *= f.w;
                     }
                 }
+                if (t + 16 <= rows) {
 #pragma unroll
-                for (int u = 0; u < 16; ++u, to += out_step)
-                    if (t + u < rows) *to = from_f32<T>(y[u]);
+                    for (int u = 0; u < 16; ++u, to += out_step) *to = from_f32<T>(y[u]);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 16; ++u, to += out_step)
+                        if (t + u < rows) *to = from_f32<T>(y[u]);
+                }
             }
             if (a.states) {
                 uint4* st = a.states + at * (KEY / 4 * 128 + 32);
