@@ -142,6 +142,18 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
     const T* k = static_cast<const T*>(a.in.k) + b * p.k_stride[0] + t0 * p.k_stride[1] + hk * p.k_stride[2];
     auto record = [&](int h) { return a.records + (((size_t)b * p.HV + h) * a.n + c) * a.rec.bytes(); };
 
+    // warp 0 looks after the decays: two steps a lane, asked for a head ahead
+    double g0 = 0., g1 = 0.;
+    float b0 = 0.f, b1 = 0.f;
+    auto ask = [&](int h) {
+        const long long o = ((long long)b * p.L + t0 + 2 * lane) * p.HV + h;
+        g0 = 2 * lane < rows ? clamp_log_decay(a.in.g[o]) : 0.f;
+        g1 = 2 * lane + 1 < rows ? clamp_log_decay(a.in.g[o + p.HV]) : 0.f;
+        b0 = 2 * lane < rows ? a.in.beta[o] : 0.f;
+        b1 = 2 * lane + 1 < rows ? a.in.beta[o + p.HV] : 0.f;
+    };
+    if (warp == 0) ask(hk * r);
+
     // K and Q: 16-byte pieces of a tile, KEY / 32 of each per thread
     constexpr int PIECES = C * KEY / 8 / NT;
     int ek, eq;
@@ -213,12 +225,9 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
         float* head = reinterpret_cast<float*>(rec);
         __syncthreads();                       // the last value head's T beta e^G and vectors are read
         if (warp == 0) {
-            const long long o = ((long long)b * p.L + t0) * p.HV + h;
             const int i0 = 2 * lane, i1 = i0 + 1;
-            const double g0 = i0 < rows ? clamp_log_decay(a.in.g[o + (long long)i0 * p.HV]) : 0.f;
-            const double g1 = i1 < rows ? clamp_log_decay(a.in.g[o + (long long)i1 * p.HV]) : 0.f;
-            be[i0] = i0 < rows ? a.in.beta[o + (long long)i0 * p.HV] : 0.f;
-            be[i1] = i1 < rows ? a.in.beta[o + (long long)i1 * p.HV] : 0.f;
+            be[i0] = b0;
+            be[i1] = b1;
             double s = g0 + g1;
 #pragma unroll
             for (int m = 1; m < 32; m *= 2) {
@@ -245,6 +254,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 em = fmaxf(em, __shfl_xor_sync(0xffffffffu, em, m));
             }
             if (lane == 0) { red[48] = um; red[49] = em; }
+            if (h + 1 < hk * r + r) ask(h + 1);
         }
         __syncthreads();
         // A to shared memory, P kept in the fragments
@@ -269,7 +279,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
 #pragma unroll
             for (int x = 0; x < PIECES; ++x) {
                 const int piece = tid + x * NT, row = piece / (KEY / 8), at = panel_at(row, piece % (KEY / 8) * 8);
-                float f[8];
+                float f[8];                      // (reading K and Q again takes longer: 509 against 462 us)
                 join8(kr + at, kr + LO + at, until[row], f);
                 put8(rec + a.rec.kt() + at, LO, f, s);
                 join8(qr + at, qr + LO + at, since[row], f);

@@ -8,16 +8,19 @@
 // product is converted by the thread that owns the row and goes back as the next product's A without leaving the lane.
 // A row's FP16 parts are scaled by a power of two of the row's own: no reduction between threads.
 //
-// Warps 0-15 own the state, four threads a row, each a quarter of its columns (the chain: convert S, product, convert V',
-// product, add); warps 16-19 bring V (dO) in, a chunk ahead, through shared memory; warps 20-23 take everything out (O or X;
-// the parts of S and V' that a backward pass reads, as they lie in tensor memory); warp 24 copies the records' tiles (bulk
-// copies), warp 25 issues the MMAs (26 and 27 fill their warpgroup, which hands its registers to the others).  Tensor memory, 512
+// Warps 0-7 own the state, two threads a row, each half of its columns (the chain: convert S, product, convert V',
+// product, add); warps 8-11 bring V (dO) in, a chunk ahead, through shared memory; warps 12-15 take everything out (O or X;
+// the parts of S and V' that a backward pass reads, as they lie in tensor memory); warp 16 copies the records' tiles (bulk
+// copies), warp 17 issues the MMAs (18 and 19 fill their warpgroup, which hands its registers to the others).  Tensor memory, 512
 // columns: [X | Y] take turns as the parts of S and as the product that updates it, two accumulators of 64 columns, the
 // parts of V' and of V.  Every wait is bounded: one that runs out sets the status word and the block ends.
 //
 // The roles walk different code, chunk after chunk, out of one instruction cache: with every loop unrolled the issue of 36
 // MMAs took 4700 cycles instead of 1700.  Only what must be (registers that are indexed) is unrolled, and the state's
-// conversions, the longest straight line, are cut into quarters that run side by side.
+// conversions, the longest straight line, are cut into halves that run side by side (quarters take as long).
+//
+// What bounds it: the instructions that turn float32 rows into FP16 parts and back, 5400 an SM quarter and chunk at 0.45 a
+// cycle (the tensor core is busy 27 % of the time, DRAM 30 %).  A chunk takes 4.4 us (8000 cycles; its MMAs alone 4000).
 #include "common.cuh"
 #include "delta.cuh"
 #include "host_common.cuh"
@@ -26,11 +29,14 @@ namespace aussm {
 namespace {
 
 constexpr int C = kDeltaChunk;
-constexpr int PARTS = 4;                 // threads that share a row of the state
+constexpr int PARTS = 2;                 // threads that share a row of the state
 constexpr int MAIN = PARTS * 4, IN = MAIN, OUT = IN + 4, COPY = OUT + 4, ISSUE = COPY + 1;     // first warp of each role
-constexpr int THREADS = (COPY + 4) * 32; // seven warpgroups; launched with 72 registers a thread, 504 for one of each
-constexpr int MAIN_REGS = 80, IN_REGS = 64, OUT_REGS = 80, REST_REGS = 40;
-static_assert(PARTS * MAIN_REGS + IN_REGS + OUT_REGS + REST_REGS <= (PARTS + 3) * 72, "more registers than the block is launched with");
+constexpr int THREADS = (COPY + 4) * 32; // five warpgroups; launched with 96 registers a thread, 480 for one of each
+constexpr int LAUNCHED = 96, MAIN_REGS = 136, IN_REGS = 64, OUT_REGS = 104, REST_REGS = 40;
+static_assert(PARTS * MAIN_REGS + IN_REGS + OUT_REGS + REST_REGS <= (PARTS + 3) * LAUNCHED, "more registers than the block is launched with");
+static_assert(THREADS * LAUNCHED <= 65536 && THREADS * (LAUNCHED + 8) > 65536, "what the compiler takes for the block");
+static_assert(MAIN_REGS >= LAUNCHED && OUT_REGS >= LAUNCHED && IN_REGS <= LAUNCHED && REST_REGS <= LAUNCHED,
+              "a warpgroup asks for more than it has, or gives some of it back");
 constexpr int SQUARE = DeltaRecord::kSquare;
 // tensor memory columns
 constexpr uint32_t kX = 0, kY = 128, kAcc = 256, kAcc2 = 320, kNew = 384, kVal = 448;
@@ -250,6 +256,12 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 if (k0 + 1 < p.DK) s[x].y = from[(size_t)(k0 + 1) * p.DV];
             }
         }
+        auto all_max = [&](const float (&m)[PARTS][128]) {
+            float r = m[0][me];
+#pragma unroll
+            for (int i = 1; i < PARTS; ++i) r = fmaxf(r, m[i][me]);
+            return r;
+        };
         // s = s * keep + r * f over the columns of a product
         auto add = [&](uint32_t t, float keep, float f) {
             const float2 k2 = make_float2(keep, keep), f2 = make_float2(f, f);
@@ -273,7 +285,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             max_s[part][me] = row_max(s);
             arrive(&row_s[warp & 3]);
             if (!warp_wait(&row_s[warp & 3], ph, a.status)) break;
-            const int es = part_exponent(fmaxf(fmaxf(max_s[0][me], max_s[1][me]), fmaxf(max_s[2][me], max_s[3][me])));
+            const int es = part_exponent(all_max(max_s));
             const float uns = pow2_float(-es);
             store_parts<COLS>(X + part * (COLS / 2), KEY / 2, s, pow2_float(es));
             if (part == 0) un_s[ph][me] = uns;
@@ -285,20 +297,21 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             tc_after();
             const float unv = un_v[ph][me], f1 = (BWD ? uns : -uns) * un1, f2 = unv * un2;
             float2 w[NEWS / 2];
-            {
-                uint32_t r1[NEWS], r2[NEWS];
-                tmem_ld16(lanes + kAcc + part * NEWS, r1);
-                tmem_ld16(lanes + kAcc2 + part * NEWS, r2);
+#pragma unroll
+            for (int x = 0; x < NEWS; x += 16) {
+                uint32_t r1[16], r2[16];
+                tmem_ld16(lanes + kAcc + part * NEWS + x, r1);
+                tmem_ld16(lanes + kAcc2 + part * NEWS + x, r2);
                 tc_wait_ld();
 #pragma unroll
-                for (int y = 0; y < NEWS / 2; ++y)
-                    w[y] = __ffma2_rn(make_float2(__uint_as_float(r1[2 * y]), __uint_as_float(r1[2 * y + 1])), make_float2(f1, f1),
-                                      __fmul2_rn(make_float2(__uint_as_float(r2[2 * y]), __uint_as_float(r2[2 * y + 1])), make_float2(f2, f2)));
+                for (int y = 0; y < 8; ++y)
+                    w[x / 2 + y] = __ffma2_rn(make_float2(__uint_as_float(r1[2 * y]), __uint_as_float(r1[2 * y + 1])), make_float2(f1, f1),
+                                              __fmul2_rn(make_float2(__uint_as_float(r2[2 * y]), __uint_as_float(r2[2 * y + 1])), make_float2(f2, f2)));
             }
             max_n[part][me] = row_max(w);
             arrive(&row_n[warp & 3]);
             if (!warp_wait(&row_n[warp & 3], ph, a.status)) break;
-            const int en = part_exponent(fmaxf(fmaxf(max_n[0][me], max_n[1][me]), fmaxf(max_n[2][me], max_n[3][me])));
+            const int en = part_exponent(all_max(max_n));
             const float unn = pow2_float(-en);
             if (full && i && !warp_wait(&x_free, ph ^ 1, a.status)) break;      // the last V' has been taken out
             store_parts<NEWS>(lanes + kNew + part * (NEWS / 2), C / 2, w, pow2_float(en));
