@@ -82,7 +82,15 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             const int row = tid >> 3, col = (tid & 7) * 8, dv = tid & 63, grp = tid >> 6, l = (v0 & 64) + dv;
             const size_t piece = at * a.slices + (v0 >> 7);
             const bool there = dv < cols;
-            float f[3][8], s[KEY / 64][8], d[KEY / 64][8], m[5] = {};
+            float shrink[5];
+            auto unit = [&](int y, float m) {            // exponent of operand y, and what its sums so far shrink by
+                const int now = min(e[y], part_exponent(m));
+                shrink[y] = v0 ? pow2_float(max(-126, now - e[y])) : 0.f;
+                e[y] = now;
+            };
+            const int pt = panel_at(dv, 8 * grp);
+            {
+            float f[3][8], s[KEY / 64][8], m[4] = {};
             if (row < rows) load8(go + row * p.go_stride[1] + v0, col, cols, a.vec_go, f[0]); else zero8(f[0]);
             auto parts = [&](const uint8_t* base, int groups, int g8, float (&o)[8]) {
                 const uint8_t* x = base + ((size_t)g8 * 128 + l) * 16;
@@ -100,37 +108,21 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             }
 #pragma unroll
             for (int y = 0; y < KEY / 64; ++y) {
-                if (there) {
-                    parts(a.states + piece * DeltaPlan::state_bytes(KEY), KEY / 8, grp + 8 * y, s[y]);
-                    parts(a.dstates + piece * DeltaPlan::state_bytes(KEY), KEY / 8, grp + 8 * y, d[y]);
-                } else {
-                    zero8(s[y]);
-                    zero8(d[y]);
-                }
+                if (there) parts(a.states + piece * DeltaPlan::state_bytes(KEY), KEY / 8, grp + 8 * y, s[y]);
+                else zero8(s[y]);
                 m[3] = max8(s[y], m[3]);
-                m[4] = max8(d[y], m[4]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) dots = fmaf(s[y][i], d[y][i], dots);
             }
 #pragma unroll
             for (int y = 0; y < 3; ++y) m[y] = max8(f[y], 0.f);
             block_max<WARPS>(m, red);
-            float shrink[5];
 #pragma unroll
-            for (int y = 0; y < 5; ++y) {
-                const int now = min(e[y], part_exponent(m[y]));
-                shrink[y] = v0 ? pow2_float(max(-126, now - e[y])) : 0.f;
-                e[y] = now;
-            }
-            const int pt = panel_at(dv, 8 * grp);
+            for (int y = 0; y < 4; ++y) unit(y, m[y]);
             put8(sm + Smem::kGo + panel_at(row, col), SQ_LO, f[0], pow2_float(e[0]));
             put8(sm + Smem::kX + pt, SQ_LO, f[1], pow2_float(e[1]));
             put8(sm + Smem::kNew + pt, SQ_LO, f[2], pow2_float(e[2]));
 #pragma unroll
-            for (int y = 0; y < KEY / 64; ++y) {
-                const int ps = panel_at(dv, 8 * grp + 64 * y);
-                put8(sm + Smem::kS + ps, ST_LO, s[y], pow2_float(e[3]));
-                put8(sm + Smem::kDs + ps, ST_LO, d[y], pow2_float(e[4]));
+            for (int y = 0; y < KEY / 64; ++y)
+                put8(sm + Smem::kS + panel_at(dv, 8 * grp + 64 * y), ST_LO, s[y], pow2_float(e[3]));
             }
             if (v0) {                                    // the sums so far, in the new unit
 #pragma unroll
@@ -143,10 +135,25 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                     for (int i = 0; i < 4; ++i) {
                         dqt[y][i] *= shrink[0] * shrink[3];
                         zz[y][i] *= shrink[1] * shrink[3];
-                        dkt[y][i] *= shrink[2] * shrink[4];
                     }
             }
             __syncthreads();
+            // dS is asked for here and taken up behind the products without it
+            uint4 raw_d[KEY / 64][2];
+            float un_d = 0.f;
+            if (there) {
+                const uint8_t* base_d = a.dstates + piece * DeltaPlan::state_bytes(KEY);
+                un_d = reinterpret_cast<const float*>(base_d + (size_t)KEY * 512)[l];
+#pragma unroll
+                for (int y = 0; y < KEY / 64; ++y) {
+                    const uint8_t* x = base_d + ((size_t)(grp + 8 * y) * 128 + l) * 16;
+                    raw_d[y][0] = *reinterpret_cast<const uint4*>(x);
+                    raw_d[y][1] = *reinterpret_cast<const uint4*>(x + (size_t)KEY * 256);
+                }
+            } else {
+#pragma unroll
+                for (int y = 0; y < KEY / 64; ++y) raw_d[y][0] = raw_d[y][1] = make_uint4(0, 0, 0, 0);
+            }
             if (dv < rows) {                             // X.V of step dv over the columns of group grp
                 float w[8], sum = 0.f;
                 load8(v + dv * p.v_stride[1] + v0, 8 * grp, cols, a.vec_v, w);
@@ -196,6 +203,39 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                         mma16816(zz[2 * x + y], xh, bh[2 * y], bh[2 * y + 1]);
                     }
                 }
+            }
+            {
+                float d[KEY / 64][8], m[1] = {};
+#pragma unroll
+                for (int y = 0; y < KEY / 64; ++y) {
+                    join8(reinterpret_cast<const uint8_t*>(&raw_d[y][0]), reinterpret_cast<const uint8_t*>(&raw_d[y][1]), un_d, d[y]);
+                    m[0] = max8(d[y], m[0]);
+                }
+                block_max<WARPS>(m, red + 4 * WARPS);
+                unit(4, m[0]);
+                const float un_s = pow2_float(-e[3]);
+#pragma unroll
+                for (int y = 0; y < KEY / 64; ++y) {
+                    const int ps = panel_at(dv, 8 * grp + 64 * y);
+                    float v8[8];                         // S of the same places
+                    put8(sm + Smem::kDs + ps, ST_LO, d[y], pow2_float(e[4]));
+                    join8(sm + Smem::kS + ps, sm + Smem::kS + ST_LO + ps, un_s, v8);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dots = fmaf(v8[i], d[y][i], dots);
+                }
+                if (v0) {
+#pragma unroll
+                    for (int y = 0; y < NW; ++y)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) dkt[y][i] *= shrink[2] * shrink[4];
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k0 = 0; k0 < VS; k0 += 16) {
+                if (k0 >= cols) break;
+                uint32_t gh[4], gl[4], bh[4], bl[4];
+                const int fx = frag_at(k0, rb * 16);
                 ldmatrix4_trans(gh, base + Smem::kNew + fx);
                 ldmatrix4_trans(gl, base + Smem::kNew + SQ_LO + fx);
 #pragma unroll
@@ -269,6 +309,46 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                 }
             }
         }
+        // the terms with states: dQt and dKt - beta Gamma Z (they take the places of dqt and dkt), their products with Q and K
+        {
+            const float fq = pow2_float(-e[0]) * pow2_float(-e[3]), fz = pow2_float(-e[1]) * pow2_float(-e[3]), fk = pow2_float(-e[2]) * pow2_float(-e[4]);
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const int i = rb * 16 + g + 8 * z;
+                const float since = expf(ghi[i] + glo[i]), until = expf((ghi[C - 1] - ghi[i]) + (glo[C - 1] - glo[i]));
+                float sumq = 0.f, sumz = 0.f, sumk = 0.f;
+#pragma unroll
+                for (int y = 0; y < NW; ++y) {
+                    const int col = cq * (KEY / 4) + 8 * y + 2 * t, pa = panel_at(i, col);
+                    const float2 kh = __half22float2(*reinterpret_cast<const __half2*>(sm + Smem::kK + pa)),
+                                 kl = __half22float2(*reinterpret_cast<const __half2*>(sm + Smem::kK + ST_LO + pa)),
+                                 qh = __half22float2(*reinterpret_cast<const __half2*>(sm + Smem::kQ + pa)),
+                                 ql = __half22float2(*reinterpret_cast<const __half2*>(sm + Smem::kQ + ST_LO + pa));
+                    const float kv[2] = {(kh.x + kl.x) * unk, (kh.y + kl.y) * unk}, qv[2] = {(qh.x + ql.x) * unq, (qh.y + ql.y) * unq};
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const float dqv = p.scale * since * (dqt[y][2 * z + w] * fq), zv = since * (zz[y][2 * z + w] * fz),
+                                    dkv = until * (dkt[y][2 * z + w] * fk);
+                        sumq = fmaf(dqv, qv[w], sumq);
+                        sumz = fmaf(zv, kv[w], sumz);
+                        sumk = fmaf(dkv, kv[w], sumk);
+                        dqt[y][2 * z + w] = dqv;
+                        dkt[y][2 * z + w] = dkv - be[i] * zv;
+                    }
+                }
+#pragma unroll
+                for (int mm = 1; mm < 4; mm *= 2) {
+                    sumq += __shfl_xor_sync(0xffffffffu, sumq, mm);
+                    sumz += __shfl_xor_sync(0xffffffffu, sumz, mm);
+                    sumk += __shfl_xor_sync(0xffffffffu, sumk, mm);
+                }
+                if (t == 0) {
+                    rowa[cq * 64 + i] = sumq - be[i] * sumz;
+                    rowz[cq * 64 + i] = -sumz;
+                    rowk[cq * 64 + i] = sumk;
+                }
+            }
+        }
         // E1 = scale D dO V'^T (gradient of Q K^T), E = -beta D X V'^T (gradient of K K^T), F = their part in G_i - G_j
         float m[2] = {}, bsum[2] = {};                   // dbeta of rows g and g + 8: sum of -D X V'^T K K^T
         {
@@ -305,6 +385,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         for (int z = 0; z < 2; ++z) {
             bsum[z] += __shfl_xor_sync(0xffffffffu, bsum[z], 1);
             bsum[z] += __shfl_xor_sync(0xffffffffu, bsum[z], 2);
+            if (t == 0) rowz[cq * 64 + rb * 16 + g + 8 * z] += bsum[z];
         }
         block_max<WARPS>(m, red + 2 * WARPS);
         const int e1 = part_exponent(m[0]), e2 = part_exponent(m[1]);
@@ -382,41 +463,17 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         }
         {
             const float f1 = pow2_float(-e1), f2 = pow2_float(-e2);
-            const float fq = pow2_float(-e[0]) * pow2_float(-e[3]), fz = pow2_float(-e[1]) * pow2_float(-e[3]), fk = pow2_float(-e[2]) * pow2_float(-e[4]);
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
                 const int i = rb * 16 + g + 8 * z;
-                const float since = expf(ghi[i] + glo[i]), until = expf((ghi[C - 1] - ghi[i]) + (glo[C - 1] - glo[i]));
-                float sumq = 0.f, sumz = 0.f, sumk = 0.f;
 #pragma unroll
                 for (int y = 0; y < NW; ++y) {
-                    const int col = cq * (KEY / 4) + 8 * y + 2 * t, pa = panel_at(i, col);
-                    const float2 kh = __half22float2(*reinterpret_cast<const __half2*>(sm + Smem::kK + pa)),
-                                 kl = __half22float2(*reinterpret_cast<const __half2*>(sm + Smem::kK + ST_LO + pa)),
-                                 qh = __half22float2(*reinterpret_cast<const __half2*>(sm + Smem::kQ + pa)),
-                                 ql = __half22float2(*reinterpret_cast<const __half2*>(sm + Smem::kQ + ST_LO + pa));
-                    const float kv[2] = {(kh.x + kl.x) * unk, (kh.y + kl.y) * unk}, qv[2] = {(qh.x + ql.x) * unq, (qh.y + ql.y) * unq};
+                    const int col = cq * (KEY / 4) + 8 * y + 2 * t;
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
-                        const float dqv = p.scale * since * (dqt[y][2 * z + w] * fq), zv = since * (zz[y][2 * z + w] * fz),
-                                    dkv = until * (dkt[y][2 * z + w] * fk);
-                        sumq = fmaf(dqv, qv[w], sumq);
-                        sumz = fmaf(zv, kv[w], sumz);
-                        sumk = fmaf(dkv, kv[w], sumk);
-                        accq[i * KEY + col + w] += fmaf(sq[y][2 * z + w] * f1, unk, dqv);
-                        acck[i * KEY + col + w] += sk[y][2 * z + w] * f1 * unq + se[y][2 * z + w] * f2 * unk + dkv - be[i] * zv;
+                        accq[i * KEY + col + w] += fmaf(sq[y][2 * z + w] * f1, unk, dqt[y][2 * z + w]);
+                        acck[i * KEY + col + w] += sk[y][2 * z + w] * f1 * unq + se[y][2 * z + w] * f2 * unk + dkt[y][2 * z + w];
                     }
-                }
-#pragma unroll
-                for (int mm = 1; mm < 4; mm *= 2) {
-                    sumq += __shfl_xor_sync(0xffffffffu, sumq, mm);
-                    sumz += __shfl_xor_sync(0xffffffffu, sumz, mm);
-                    sumk += __shfl_xor_sync(0xffffffffu, sumk, mm);
-                }
-                if (t == 0) {
-                    rowa[cq * 64 + i] = sumq - be[i] * sumz;
-                    rowz[cq * 64 + i] = bsum[z] - sumz;
-                    rowk[cq * 64 + i] = sumk;
                 }
             }
         }
