@@ -64,7 +64,7 @@ __host__ __device__ __forceinline__ float pow2_float(int k) {
 // exponent k of the scale 2^k for a tile whose largest magnitude is m
 __device__ __forceinline__ int part_exponent(float m) {
     const int e = (int)((__float_as_uint(m) >> 23) & 0xffu) - 127;
-    return max(-100, min(100, 13 - e));
+    return max(-115, min(115, 13 - e));                  // the whole range of float32
 }
 // hi and lo parts of two values that are scaled already, packed
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {

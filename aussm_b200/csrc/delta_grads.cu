@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
 
         // ---- products over the value columns -------------------------------------------------------------------
         float dp[2][4] = {}, xn[2][4] = {}, dqt[NW][4] = {}, zz[NW][4] = {}, dkt[NW][4] = {};
-        int e[5] = {100, 100, 100, 100, 100};            // exponents of dO, X, V', S, dS
+        int e[5] = {115, 115, 115, 115, 115};            // exponents of dO, X, V', S, dS
         float dotv = 0.f, dots = 0.f;
         for (int v0 = 0; v0 < DV; v0 += VS) {
             const int cols = DV - v0;

@@ -273,7 +273,8 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 }
         }
         // Kt and Qt from the parts of K and Q; their largest magnitudes are at most these
-        const int et = part_exponent(red[48] * pow2_float(14 - ek)), eqt = part_exponent(red[49] * pow2_float(14 - eq));
+        const int et = part_exponent(red[48] * pow2_float(min(127, 14 - ek))),
+                  eqt = part_exponent(red[49] * pow2_float(min(127, 14 - eq)));
         {
             const float s = unk * pow2_float(et), sq = unq * pow2_float(eqt);
 #pragma unroll

@@ -284,7 +284,7 @@ struct Walk {
 template <typename T, int VEC, int G, int UPL, bool BWD>
 __global__ void __launch_bounds__(NT, BWD ? 2 : 3) rotate_kernel(const RotateParams a) {
     const int lane = threadIdx.x % G;
-    const unsigned first = (blockIdx.x * NT + threadIdx.x) / G, stride = gridDim.x * (NT / G);
+    const unsigned first = blockIdx.x * (NT / G) + threadIdx.x / G, stride = gridDim.x * (NT / G);
     Walk<T, VEC, G, UPL, BWD> q, k;
     if (BWD) {
 #pragma unroll

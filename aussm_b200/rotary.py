@@ -137,6 +137,8 @@ def qk_norm_rotate(q: Tensor, k: Tensor, frequencies: Optional[Tensor] = None, p
     n, stride = 0, 0
     if frequencies is not None:
         n = frequencies.numel()
+        if frequencies.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("qk_norm_rotate is not differentiable in the frequencies: detach them")
         if 2 * n > d:
             raise RuntimeError(f"{n} frequencies for heads of {d} elements: at most {d // 2}")
         frequencies = _typed("frequencies", frequencies, torch.float64, (n,), dev).contiguous()

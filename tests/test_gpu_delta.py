@@ -129,6 +129,19 @@ def test_scale_and_large_values():
     compare(both(d, scale=1e-3))
 
 
+@pytest.mark.parametrize("size", [1e36, 1e-30])
+def test_ends_of_the_range(size):
+    """Values and states near the ends of float32 (the gradients of q, k, g and beta, products of two of them, do not fit)."""
+    d = make(14, 1, 100, 1, 1, 64, 64)
+    d["v"] *= size
+    d["state"] *= size
+    o, s = gated_delta_rule(*(d[n] for n in NAMES[:5]), initial_state=d["state"], return_final_state=True)
+    y = {n: t.double() for n, t in d.items()}
+    o64, s64 = gated_delta_ref(*(y[n] for n in NAMES[:5]), initial_state=y["state"])
+    for got, truth in ((o, o64), (s, s64)):
+        close("scaled", (got.double() / size).float(), truth / size, FWD)
+
+
 def test_a_nan_stays_in_its_value_column():
     d = make(17, 1, 130, 1, 1, 64, 64)
     clean, cs = gated_delta_rule(*(d[n] for n in NAMES[:5]), return_final_state=True)

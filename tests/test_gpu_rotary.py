@@ -135,6 +135,7 @@ def test_empty_graph_and_refusals():
            lambda: qk_norm_rotate(q, k[:, :2], f), lambda: qk_norm_rotate(q, k[..., :16], f), lambda: qk_norm_rotate(q, k, f.float()),
            lambda: qk_norm_rotate(q, k, torch.ones(17, device="cuda", dtype=torch.float64)), lambda: qk_norm_rotate(q, k, f.cpu()),
            lambda: qk_norm_rotate(q, k, f, x["positions"].int()), lambda: qk_norm_rotate(q, k, f, x["positions"][:, :3]),
+           lambda: qk_norm_rotate(q, k, f.clone().requires_grad_()),
            lambda: qk_norm_rotate(q, k, f, norm="layer"), lambda: qk_norm_rotate(q, k, f, q_weight=w.detach()[:5]),
            lambda: qk_norm_rotate(q[0], k[0], f), lambda: qk_norm_rotate(torch.zeros(1, 1, 1, 257, device="cuda"), torch.zeros(1, 1, 1, 257, device="cuda")),
            lambda: torch.func.vmap(lambda a: qk_norm_rotate(a, k, f)[0])(q[None])]
