@@ -16,7 +16,10 @@ DeltaPlan delta_plan(const aussm_b200_delta_t& p) {
     d.rec.key = p.DK <= 64 ? 64 : 128;
     d.slices = (p.DV + 127) / 128;
     const size_t pieces = d.heads * d.slices;
-    // A block of the recurrences takes an SM.
+    // A block of the recurrences takes an SM; a segment costs a second pass (a third forward) over its chunks and a share of
+    // the chain.  One sequence of 4096 steps, heads of 128, forward / training, in segments and whole: 16 heads 213 against
+    // 331 / 671 against 1021 us, 32 heads 358 against 402 / 1217 against 1417 us, 48 heads 490 against 474 / 1747 against
+    // 1797 us; 64 heads in two segments 540 against 546 / 2185 against 2190 us.  So: from a third of the SMs on, whole.
     const long long blocks = (long long)p.B * p.HV * d.slices;
     long long segs = 1;
     if (blocks * 3 <= 148) {

@@ -5,6 +5,9 @@
 // FP16 parts with mma.sync (two blocks an SM, 8 warps each, warp = 16 rows x half of the columns), skipping the 16 x 16
 // blocks above the diagonal.  Differences of the sums of g are taken from pairs of floats: sums reach thousands, and
 // e^(G_i - G_j) has to be right to 24 bits where G_i - G_j is small.
+//
+// What bounds it: 3900 instructions a warp at 0.41 a cycle and SM quarter, barriers and shared memory between them.  2048
+// chunk heads of 128: 144 us, 268 MB of records written (1.9 TB/s); 8192 that share 4096 key heads: 462 us.
 #include "delta_tiles.cuh"
 #include "host_common.cuh"
 
