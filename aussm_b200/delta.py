@@ -21,7 +21,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .ops import _PLAIN, _eager, _ptr, _workspace
+from .ops import _PLAIN, _eager, _poll_status, _ptr, _workspace
 
 __all__ = ["gated_delta_rule", "gated_delta_step", "MAX_KEY", "MAX_VALUE"]
 
@@ -121,6 +121,7 @@ def _forward(p, q, k, v, g, beta, state, want_state, train):
                                       _ptr(room) if train else None, size if train else 0, None if train else _ptr(room),
                                       0 if train else size, _raw_stream(q.device))
     _lib.check(rc, "gated_delta_rule")
+    _poll_status("gated_delta_rule", q.device)
     return o, last, room if train else None
 
 
@@ -161,6 +162,7 @@ class _GatedDelta(torch.autograd.Function):
                                           keep.numel(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dg), _ptr(dbeta), _ptr(ds0),
                                           _ptr(ws), ws.numel(), _raw_stream(q.device))
         _lib.check(rc, "gated_delta_rule backward")
+        _poll_status("gated_delta_rule backward", q.device)
         return dq, dk, dv, dg, dbeta, ds0, None, None
 
 
@@ -216,4 +218,6 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
         rc = _lib.load().aussm_b200_delta_step(p, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(out),
                                                _ptr(o), _raw_stream(q.device))
     _lib.check(rc, "gated_delta_step")
+    if not out.is_inference():                          # written in place: a graph that has saved it must not use it
+        torch.autograd.graph.increment_version(out)
     return o

@@ -415,3 +415,29 @@ def test_models_with_delta_layers():
     out = clf(ids, torch.tensor([70, 33], device="cuda"))
     assert out.shape == (2, 3) and torch.isfinite(out).all()
     assert aussm_b200.device_status() == 0
+
+
+def test_status_word_is_polled(monkeypatch):
+    seen = []
+    monkeypatch.setattr("aussm_b200.ops.check_device_status", True)
+    monkeypatch.setattr("aussm_b200.ops.device_status", lambda device=None: seen.append(device) or 0)
+    d = make(1, 1, 70, 1, 1, 8, 8)
+    q = d["q"].requires_grad_()
+    gated_delta_rule(q, d["k"], d["v"], d["g"], d["beta"]).sum().backward()
+    assert seen == [q.device] * 2
+    monkeypatch.setattr("aussm_b200.ops.device_status", lambda device=None: 1)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="gave up"):
+        gated_delta_rule(q, d["k"], d["v"], d["g"], d["beta"])
+
+
+def test_step_counts_as_a_change_in_place():
+    d = make(2, 2, 1, 1, 2, 16, 16)
+    w = torch.ones((), device="cuda", requires_grad=True)
+    kept = (w * d["state"]).sum()                       # saves the state for w's gradient
+    gated_delta_step(*(d[n] for n in NAMES))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
+    with torch.inference_mode():                        # states made there have no count
+        x = {n: t.clone() for n, t in d.items()}
+        other = gated_delta_step(*(x[n] for n in NAMES))
+    assert torch.equal(other, gated_delta_step(*(d[n] for n in NAMES)))

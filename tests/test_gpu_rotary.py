@@ -153,3 +153,11 @@ def test_empty_graph_and_refusals():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y[0], ref[0]) and torch.equal(y[1], ref[1]) and torch.equal(gw, gref)
+
+
+def test_differentiable_once():
+    q, k = (torch.randn(1, 5, 2, 8, device="cuda").requires_grad_() for _ in range(2))
+    yq, yk = qk_norm_rotate(q, k)
+    gq, = torch.autograd.grad(yq.sum() + yk.sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(gq.sum(), q)
