@@ -51,6 +51,13 @@ def _typed(name: str, t: Tensor, dtype, shape, device) -> Tensor:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
     if tuple(t.shape) != tuple(shape):
         raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return _plain(t)
+
+
+def _plain(t: Tensor) -> Tensor:
+    """``t`` with unit stride along its last axis and its sign in memory (parts of conjugate tensors have it in a flag)."""
+    if t.is_neg():
+        t = t.resolve_neg()
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
@@ -147,13 +154,13 @@ class _GatedDelta(torch.autograd.Function):
         if ctx.has_state and ctx.needs_input_grad[5]:
             ds0 = torch.empty(p.B, p.HV, p.DK, p.DV, device=q.device, dtype=torch.float32)
         if glast is not None:
-            glast = glast.contiguous()
+            glast = _plain(glast).contiguous()
         if keep is None:                                # no steps
             if ds0 is not None:
                 ds0.zero_() if glast is None else ds0.copy_(glast)
             return dq, dk, dv, dg, dbeta, ds0, None, None
         go = torch.zeros(v.shape, device=v.device, dtype=v.dtype) if go is None else go
-        go = go if go.stride(-1) == 1 or go.shape[-1] == 1 else go.contiguous()
+        go = _plain(go)
         p.go_stride = _strides(go)
         lib = _lib.load()
         with _on(q.device):
@@ -203,7 +210,7 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     p, q, k, v, g, beta = _check(q, k, v, g, beta, scale)
     out = state if new_state is None else new_state
     state = _state("state", state, p, q.device)
-    if not out.is_contiguous() or tuple(out.shape) != tuple(state.shape) or out.dtype != torch.float32 or out.device != q.device:
+    if not out.is_contiguous() or out.is_neg() or tuple(out.shape) != tuple(state.shape) or out.dtype != torch.float32 or out.device != q.device:
         raise RuntimeError(f"the state that takes the result must be contiguous float32 {tuple(state.shape)} on {q.device}")
     if new_state is not None and state.numel():
         lo, hi, size = sorted((state.data_ptr(), out.data_ptr())) + [4 * state.numel()]

@@ -16,7 +16,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .delta import _DTYPES, _on, _raw_stream, _refuse_traced, _strides, _typed
+from .delta import _DTYPES, _on, _plain, _raw_stream, _refuse_traced, _strides, _typed
 from .ops import _ptr, _workspace
 
 __all__ = ["qk_norm_rotate", "rotary_frequencies", "MAX_HEAD"]
@@ -39,6 +39,8 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] =
         raise RuntimeError(f"dim must be even and positive, got {dim}")
     if factor <= 0 or base <= 0:
         raise RuntimeError("base and factor must be positive")
+    if not turns[0] < turns[1]:
+        raise RuntimeError(f"turns must be two rising numbers, got {turns}")
     i = torch.arange(0, dim, 2, device=device, dtype=torch.float64) / dim
     magnitude = 1.0
     if scaling == "base" and dim > 2:
@@ -91,7 +93,7 @@ class _NormRotate(torch.autograd.Function):
         dkw = torch.empty_like(k_weight) if ctx.needs_input_grad[3] else None
         if not (p.B and p.L):
             return dq, dk, None if dqw is None else dqw.zero_(), None if dkw is None else dkw.zero_(), None, None, None
-        gq, gk = (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (gq, gk))
+        gq, gk = _plain(gq), _plain(gk)
         p.gq_stride, p.gk_stride = _strides(gq), _strides(gk)
         lib = _lib.load()
         with _on(q.device):

@@ -128,3 +128,34 @@ def test_block_in_the_models(monkeypatch):
     for bad in (dict(d_model=30, n_heads=4), dict(d_model=512, n_heads=2), dict(d_model=32, rotary_dim=3), dict(d_model=32, n_heads=2, rotary_dim=18)):
         with pytest.raises(ValueError):
             models.GatedDeltaBlock(**bad)
+
+
+def test_block_reads_a_prompt_in_pieces(monkeypatch):
+    models = _with_oracle(monkeypatch)
+    called = []
+
+    def rule(q, k, v, g, beta, initial_state=None, return_final_state=False):
+        called.append(q.shape[1])
+        o, s = gated_delta_ref(q, k, v, g, beta, initial_state=initial_state)
+        return (o, s) if return_final_state else o
+
+    monkeypatch.setattr(models.delta, "gated_delta_rule", rule)
+    torch.manual_seed(1)
+    block = models.GatedDeltaBlock(32, n_heads=2, rotary_dim=8, bias=True).double()
+    x = torch.randn(2, 60, 32, dtype=torch.float64)
+    whole = block(x)
+    cache = block.init_cache(2, dtype=torch.float64)
+    cache["state"] = cache["state"].double()
+    cuts = [0, 37, 38, 40, 43, 60]
+    pieces = torch.cat([block.step(x[:, a:b], cache) for a, b in zip(cuts, cuts[1:])], 1)
+    # The gates are cast to float32: a product summed in another order (1e-16 off) may round to its neighbour, one step of
+    # 2^-23 relative.  |a| < 4 moves softplus(a + dt) and so g by at most 4 * 2^-23 of itself (softplus' <= softplus for
+    # arguments below 0.5, and the step sizes start at 0.1 or less), the state, in which a decay of g lasts 1 / |g| steps,
+    # by as much of itself, beta by 2^-23: 6e-7 of o, and as much again through the norm of the head and its product.
+    assert torch.allclose(pieces, whole, rtol=0, atol=2e-6 * float(whole.detach().abs().max()))
+    assert int(cache["position"]) == 60 and called == [60, 37, 17]
+
+
+def test_stretch_wants_rising_turns():
+    with pytest.raises(RuntimeError, match="rising"):
+        rotary_frequencies(8, scaling="ramp", factor=2.0, turns=(4.0, 4.0))

@@ -441,3 +441,59 @@ def test_step_counts_as_a_change_in_place():
         x = {n: t.clone() for n, t in d.items()}
         other = gated_delta_step(*(x[n] for n in NAMES))
     assert torch.equal(other, gated_delta_step(*(d[n] for n in NAMES)))
+
+
+def test_signs_kept_in_a_flag():
+    """Parts of conjugate tensors carry their sign in a flag, as inputs and as gradients."""
+    d = make(3, 2, 70, 1, 2, 16, 8)
+    flagged = lambda t: torch.complex(torch.zeros_like(t), -t).conj().imag
+    x = {n: flagged(t) for n, t in d.items()}
+    assert all(t.is_neg() for t in x.values())
+    a, b = gated_delta_rule(*(d[n] for n in NAMES[:5]), initial_state=d["state"]), gated_delta_rule(
+        *(x[n] for n in NAMES[:5]), initial_state=x["state"])
+    assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="takes the result"):
+        gated_delta_step(*(x[n][:, :1] for n in NAMES[:5]), x["state"])
+    new = torch.empty_like(d["state"])
+    assert torch.equal(gated_delta_step(*(x[n][:, :1] for n in NAMES[:5]), x["state"], new_state=new),
+                       gated_delta_step(*(d[n][:, :1] for n in NAMES[:5]), d["state"].clone()))
+    v = d["v"].requires_grad_()
+    o, s = gated_delta_rule(d["q"], d["k"], v, d["g"], d["beta"], return_final_state=True)
+    go, gs = torch.randn_like(o), torch.randn_like(s)
+    assert torch.equal(torch.autograd.grad([o, s], v, [go, gs], retain_graph=True)[0],
+                       torch.autograd.grad([o, s], v, [flagged(go), flagged(gs)])[0])
+
+
+@pytest.mark.parametrize("rotary_dim", [0, 32])
+def test_block_captured_step_and_prompt(rotary_dim):
+    """A prompt in one piece, then single tokens from a captured and replayed step, against whole sequences."""
+    from aussm_b200 import models
+    torch.manual_seed(4)
+    block = models.GatedDeltaBlock(128, n_heads=2, rotary_dim=rotary_dim).cuda()
+    x = torch.randn(2, 90, 128, device="cuda")
+    static = torch.empty(2, 1, 128, device="cuda")
+    with torch.no_grad():
+        whole = block(x)
+        cache = block.init_cache(2, device="cuda")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            block.step(static.zero_(), cache)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = block.step(static, cache)
+        for t in cache.values():
+            t.zero_()
+        got = [block.step(x[:, :70], cache), block.step(x[:, 70:73], cache)]
+        for t in range(73, 90):
+            static.copy_(x[:, t:t + 1])
+            graph.replay()
+            got.append(y.clone())
+    assert int(cache["position"]) == 90
+    # both sides are within the block's tolerance of the exact values
+    close("pieces", torch.cat(got, 1), whole, 8 * FWD)
+    if rotary_dim:
+        fresh = models.GatedDeltaBlock(128, n_heads=2, rotary_dim=rotary_dim).cuda()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()), pytest.raises(RuntimeError, match="before it is captured"):
+            fresh._frequencies(x.device)

@@ -161,3 +161,13 @@ def test_differentiable_once():
     gq, = torch.autograd.grad(yq.sum() + yk.sum(), q, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(gq.sum(), q)
+
+
+def test_gradients_with_their_sign_in_a_flag():
+    q, k = (torch.randn(1, 5, 2, 8, device="cuda").requires_grad_() for _ in range(2))
+    y = qk_norm_rotate(q, k)
+    g = [torch.randn_like(t) for t in y]
+    flagged = [torch.complex(torch.zeros_like(t), -t).conj().imag for t in g]
+    assert all(t.is_neg() for t in flagged)
+    for a, b in zip(torch.autograd.grad(y, [q, k], g, retain_graph=True), torch.autograd.grad(y, [q, k], flagged)):
+        assert torch.equal(a, b)
