@@ -232,7 +232,7 @@ class GatedDeltaBlock(nn.Module):
 
     def forward(self, x):
         d = self.d_model
-        if x.is_cuda and x.dtype == torch.float32 and self.conv1d.kernel_size[0] <= 4:
+        if x.is_cuda and x.dtype == torch.float32 and self.conv1d.kernel_size[0] <= 4 and not torch.is_autocast_enabled("cuda"):
             w, bias = self.in_proj.weight, self.in_proj.bias
             xs = stages.project_tokens(w[:3 * d], x)                         # (b, 3d, l): the convolution's layout
             xs = xs if bias is None else xs + bias[:3 * d, None]
@@ -244,10 +244,12 @@ class GatedDeltaBlock(nn.Module):
         q, k, v, g, beta = self._inputs(x, conv, None)
         return self._output(delta.gated_delta_rule(q, k, v, g, beta), z)
 
-    def init_cache(self, batch: int, device=None, dtype=torch.float32):
+    def init_cache(self, batch: int, device=None, dtype=None):
         """What ``step`` carries from token to token: the state (float32), the convolution's last inputs, the position (all
-        on the device: a captured step moves on when it is replayed)."""
+        on the device: a captured step moves on when it is replayed).  Device and type default to the block's."""
         h, w = self.n_heads, self.d_head
+        device = self.conv1d.weight.device if device is None else device
+        dtype = self.conv1d.weight.dtype if dtype is None else dtype
         return dict(state=torch.zeros(batch, h, w, w, device=device, dtype=torch.float32),
                     position=torch.zeros(1, device=device, dtype=torch.int64),
                     conv=torch.zeros(batch, self.conv1d.kernel_size[0] - 1, 3 * self.d_model, device=device, dtype=dtype))
@@ -262,7 +264,7 @@ class GatedDeltaBlock(nn.Module):
         if l == 1:
             conv = torch.einsum("bkc,ck->bc", window, w[:, 0])[:, None]
             conv = conv if bias is None else conv + bias
-        elif x.is_cuda and x.dtype == torch.float32 and w.shape[2] <= 4:
+        elif x.is_cuda and window.dtype == w.dtype == torch.float32 and w.shape[2] <= 4:
             conv = stages.causal_conv_bias(window.transpose(1, 2), w, bias).transpose(1, 2)[:, w.shape[2] - 1:]
         else:
             conv = _causal_depthwise_conv(self.conv1d, window)[:, w.shape[2] - 1:]

@@ -497,3 +497,35 @@ def test_block_captured_step_and_prompt(rotary_dim):
         fresh = models.GatedDeltaBlock(128, n_heads=2, rotary_dim=rotary_dim).cuda()
         with torch.cuda.graph(torch.cuda.CUDAGraph()), pytest.raises(RuntimeError, match="before it is captured"):
             fresh._frequencies(x.device)
+
+
+def test_block_in_sixteen_bits():
+    """The cache follows the block's type; both ways through the block agree to bfloat16's roundings."""
+    from aussm_b200 import models
+    torch.manual_seed(6)
+    block = models.GatedDeltaBlock(64, n_heads=2, rotary_dim=16).cuda().bfloat16()
+    x = torch.randn(2, 30, 64, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        whole, cache = block(x), block.init_cache(2)
+        got = torch.cat([block.step(x[:, a:b], cache) for a, b in ((0, 20), (20, 21), (21, 30))], 1)
+    assert cache["conv"].dtype == torch.bfloat16 and cache["state"].dtype == torch.float32 and cache["state"].is_cuda
+    # In the worst case each of a dozen roundings of 2^-8 stays, for both sides, in the same direction: 24 * 2^-8 of the
+    # largest element; a step that took a wrong position, input or state is off by the size of the result.
+    assert got.dtype == torch.bfloat16
+    assert float((got.float() - whole.float()).abs().max()) <= 24 * 2 ** -8 * float(whole.float().abs().max())
+
+
+def test_block_under_autocast():
+    from aussm_b200 import models
+    torch.manual_seed(7)
+    block = models.GatedDeltaBlock(64, n_heads=2).cuda()
+    x = torch.randn(2, 70, 64, device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = block(x)
+        with torch.no_grad():
+            cache = block.init_cache(2)
+            steps = torch.cat([block.step(x[:, a:b], cache) for a, b in ((0, 40), (40, 41), (41, 70))], 1)
+    y.float().square().mean().backward()
+    # as in bfloat16 altogether, see above
+    assert float((steps.float() - y.detach().float()).abs().max()) <= 24 * 2 ** -8 * float(y.detach().float().abs().max())
+    assert torch.isfinite(y).all() and all(torch.isfinite(p.grad).all() for p in block.parameters())
