@@ -31,7 +31,9 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 def _refuse_traced(what: str, *tensors) -> None:
     """A kernel that writes through raw pointers is invisible to tracers and function transforms: refuse them."""
-    plain = all(t is None or type(t) in _PLAIN for t in tensors)
+    plain = True
+    for t in tensors:
+        plain = plain and (t is None or type(t) in _PLAIN)
     if plain and _eager():
         return
     from torch.fx.experimental.proxy_tensor import get_proxy_mode
@@ -43,6 +45,9 @@ def _refuse_traced(what: str, *tensors) -> None:
 
 def _typed(name: str, t: Tensor, dtype, shape, device) -> Tensor:
     """``t`` checked, with unit stride along its last axis (a copy only where it has not)."""
+    if (type(t) in _PLAIN and t.device == device and t.dtype is dtype and t.shape == shape and t.stride(-1) == 1
+            and not t.is_neg() and t.is_cuda):
+        return t                                        # as most are: short calls are bound by the host
     if not isinstance(t, Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor (there is no CPU implementation of this operator)")
     if t.device != device:
