@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     constexpr int TILE = Smem::kTile, LO = KEY * 128, SQ_LO = 8192;
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full_a, full_b[2], full_c, full_e[2], empty_a, empty_b[2], empty_c, empty_e[2];
-    __shared__ uint64_t s_ready, v_ready, v_done, n_ready, a_done, y_free, d_done, o_done, o_free, x_free, v_loaded, v_read;
+    __shared__ uint64_t s_ready, v_ready[2], v_done, n_ready, a_done, y_free, d_done, o_done, o_free, x_free, v_loaded, v_read;
     __shared__ uint64_t row_s[4], row_n[4];
     __shared__ uint32_t holder;
     __shared__ float un_s[2][128], un_v[2][128], un_n[128], max_s[PARTS][128], max_n[PARTS][128];
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                             &empty_c, &empty_e[0], &empty_e[1], &v_done, &a_done, &d_done, &o_done})
             mbar_init(x, 1);
         for (uint64_t* x : {&s_ready, &n_ready, &y_free}) mbar_init(x, PARTS * 128);
-        for (uint64_t* x : {&v_ready, &o_free, &x_free, &v_loaded, &v_read}) mbar_init(x, 128);
+        for (uint64_t* x : {&v_ready[0], &v_ready[1], &o_free, &x_free, &v_loaded, &v_read}) mbar_init(x, 128);
         for (int i = 0; i < 4; ++i) {
             mbar_init(&row_s[i], PARTS * 32);
             mbar_init(&row_n[i], PARTS * 32);
@@ -292,8 +292,9 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             tc_wait_st();
             tc_before();
             arrive(&s_ready);
-            // V' (dV'), columns [NEWS part, NEWS part + NEWS)
-            if (!warp_wait(&v_done, ph, a.status) || !warp_wait(&v_ready, ph, a.status)) break;
+            // V' (dV'), columns [NEWS part, NEWS part + NEWS).  v_ready has a barrier for each of two chunks: the next V may
+            // be in before a warp that saw v_done has come to this wait, and a single one would be two phases on by then.
+            if (!warp_wait(&v_done, ph, a.status) || !warp_wait(&v_ready[ph], (i >> 1) & 1, a.status)) break;
             tc_after();
             const float unv = un_v[ph][me], f1 = (BWD ? uns : -uns) * un1, f2 = unv * un2;
             float2 w[NEWS / 2];
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             un_v[i & 1][me] = pow2_float(-e);
             tc_wait_st();
             tc_before();
-            arrive(&v_ready);
+            arrive(&v_ready[i & 1]);
             if (i + 1 < count) {
                 arrive(&v_read);
                 if (!warp_wait(&v_read, (i + 1) & 1, a.status)) break;       // all lanes have read their rows
@@ -543,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             for (int i = 0; i < count; ++i) {
                 const uint32_t ph = i & 1, X = tm + (ph ? kY : kX), Y = tm + (ph ? kX : kY);
                 const uint32_t ta = base + Smem::kA, half = (i >> 1) & 1;
-                if (!wait(&full_a, ph) || !wait(&v_ready, ph) || (full && i && !wait(&o_free, ph ^ 1))) break;
+                if (!wait(&full_a, ph) || !wait(&v_ready[ph], half) || (full && i && !wait(&o_free, ph ^ 1))) break;
                 tc_after();
                 product<C, C / 16, BWD>(tm + kAcc2, tm + kVal, ta + TILE, SQ_LO, one);       // no state in it
                 if (!wait(&s_ready, ph)) break;
