@@ -66,6 +66,11 @@ __device__ __forceinline__ int part_exponent(float m) {
     const int e = (int)((__float_as_uint(m) >> 23) & 0xffu) - 127;
     return max(-115, min(115, 13 - e));                  // the whole range of float32
 }
+// The same from the largest of the values' ranks: unsigned numbers in the order of the magnitudes, with what is not finite
+// below zero.  An infinity would set a scale that turns every finite element of its tile into zero; so it sets none, and
+// stays an infinity (and its lo part a NaN) in the conversion.
+__device__ __forceinline__ uint32_t rank_of(float x) { return (__float_as_uint(x) << 1) + 0x01000000u; }
+__device__ __forceinline__ int rank_exponent(uint32_t r) { return max(-115, min(115, 13 + 128 - (int)(r >> 24))); }
 // hi and lo parts of two values that are scaled already, packed
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(a, b);

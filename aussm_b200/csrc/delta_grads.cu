@@ -57,7 +57,8 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
     float* vec = reinterpret_cast<float*>(sm + Smem::kVec);
     float *ghi = vec, *glo = vec + 64, *be = vec + 128, *rowa = vec + 192 /* (4, 64) */, *rowk = vec + 448 /* (4, 64) */,
           *rowz = vec + 704 /* (4, 64) */;
-    __shared__ float red[6 * WARPS], xv[8][C], ssum[WARPS], am[C], kkt[C];
+    __shared__ uint32_t red[6 * WARPS];
+    __shared__ float xv[8][C], ssum[WARPS], am[C], kkt[C];
     const aussm_b200_delta_t& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int rb = warp & 3, cq = warp >> 2;             // 16 rows, a quarter of the columns
@@ -86,14 +87,15 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             const size_t piece = at * a.slices + (v0 >> 7);
             const bool there = dv < cols;
             float shrink[5];
-            auto unit = [&](int y, float m) {            // exponent of operand y, and what its sums so far shrink by
-                const int now = min(e[y], part_exponent(m));
+            auto unit = [&](int y, uint32_t m) {            // exponent of operand y, and what its sums so far shrink by
+                const int now = min(e[y], rank_exponent(m));
                 shrink[y] = v0 ? pow2_float(max(-126, now - e[y])) : 0.f;
                 e[y] = now;
             };
             const int pt = panel_at(dv, 8 * grp);
             {
-            float f[3][8], s[KEY / 64][8], m[4] = {};
+            float f[3][8], s[KEY / 64][8];
+            uint32_t m[4] = {};
             if (row < rows) load8(go + row * p.go_stride[1] + v0, col, cols, a.vec_go, f[0]); else zero8(f[0]);
             auto parts = [&](const uint8_t* base, int groups, int g8, float (&o)[8]) {
                 const uint8_t* x = base + ((size_t)g8 * 128 + l) * 16;
@@ -116,7 +118,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                 m[3] = max8(s[y], m[3]);
             }
 #pragma unroll
-            for (int y = 0; y < 3; ++y) m[y] = max8(f[y], 0.f);
+            for (int y = 0; y < 3; ++y) m[y] = max8(f[y], 0u);
             block_max<WARPS>(m, red);
 #pragma unroll
             for (int y = 0; y < 4; ++y) unit(y, m[y]);
@@ -208,7 +210,8 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                 }
             }
             {
-                float d[KEY / 64][8], m[1] = {};
+                float d[KEY / 64][8];
+                uint32_t m[1] = {};
 #pragma unroll
                 for (int y = 0; y < KEY / 64; ++y) {
                     join8(reinterpret_cast<const uint8_t*>(&raw_d[y][0]), reinterpret_cast<const uint8_t*>(&raw_d[y][1]), un_d, d[y]);
@@ -268,7 +271,8 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             constexpr int PIECES = C * KEY / 8 / NT;
             const T* q = static_cast<const T*>(a.in.q) + b * p.q_stride[0] + t0 * p.q_stride[1] + hk * p.q_stride[2];
             const T* k = static_cast<const T*>(a.in.k) + b * p.k_stride[0] + t0 * p.k_stride[1] + hk * p.k_stride[2];
-            float fk[PIECES][8], fq[PIECES][8], m[2] = {};
+            float fk[PIECES][8], fq[PIECES][8];
+            uint32_t m[2] = {};
 #pragma unroll
             for (int y = 0; y < PIECES; ++y) {
                 const int piece = tid + y * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8;
@@ -283,8 +287,8 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                 m[1] = max8(fq[y], m[1]);
             }
             block_max<WARPS>(m, red);
-            ek = part_exponent(m[0]);
-            eq = part_exponent(m[1]);
+            ek = rank_exponent(m[0]);
+            eq = rank_exponent(m[1]);
 #pragma unroll
             for (int y = 0; y < PIECES; ++y) {
                 const int piece = tid + y * NT, pk = panel_at(piece / (KEY / 8), piece % (KEY / 8) * 8);
@@ -353,7 +357,8 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             }
         }
         // E1 = scale D dO V'^T (gradient of Q K^T), E = -beta D X V'^T (gradient of K K^T), F = their part in G_i - G_j
-        float m[2] = {}, bsum[2] = {};                   // dbeta of rows g and g + 8: sum of -D X V'^T K K^T
+        uint32_t m[2] = {};
+        float bsum[2] = {};                   // dbeta of rows g and g + 8: sum of -D X V'^T K K^T
         {
             const uint8_t* pt = reinterpret_cast<const uint8_t*>(head) + a.rec.p();
             const float unp = head[kUnP], fp = pow2_float(-e[0]) * pow2_float(-e[2]), fx = pow2_float(-e[1]) * pow2_float(-e[2]);
@@ -379,8 +384,8 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                         F[i * FP + j + w] = below ? fmaf(dpv, pv[w], be[i] * mx * kkv) : 0.f;
                         dp[y][2 * z + w] = p.scale * d * dpv;
                         xn[y][2 * z + w] = be[i] * mx;
-                        m[0] = fmaxf(m[0], fabsf(dp[y][2 * z + w]));
-                        m[1] = fmaxf(m[1], fabsf(xn[y][2 * z + w]));
+                        m[0] = max(m[0], rank_of(dp[y][2 * z + w]));
+                        m[1] = max(m[1], rank_of(xn[y][2 * z + w]));
                     }
                 }
         }
@@ -391,7 +396,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             if (t == 0) rowz[cq * 64 + rb * 16 + g + 8 * z] += bsum[z];
         }
         block_max<WARPS>(m, red + 2 * WARPS);
-        const int e1 = part_exponent(m[0]), e2 = part_exponent(m[1]);
+        const int e1 = rank_exponent(m[0]), e2 = rank_exponent(m[1]);
         {
             const float s1 = pow2_float(e1), s2 = pow2_float(e2);
 #pragma unroll

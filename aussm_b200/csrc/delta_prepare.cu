@@ -125,7 +125,7 @@ __device__ __forceinline__ void invert(float* A, float* tmp) {
 template <int KEY>
 struct PrepareSmem {
     static constexpr int kTile = KEY * 256;
-    static constexpr int kBytes = 2 * kTile + DeltaRecord::kSquare + C * PITCH * 4 + 64 * 34 * 4 + 6 * C * 4 + 64 * 4;
+    static constexpr int kBytes = 2 * kTile + DeltaRecord::kSquare + C * PITCH * 4 + 64 * 34 * 4 + 6 * C * 4 + 4 * 4 + 32 * 4;
 };
 
 template <typename T, int KEY>
@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
     uint8_t *kr = sm, *qr = sm + Smem::kTile;
     uint8_t* tr = qr + Smem::kTile;                                   // T beta e^G
     float* A = reinterpret_cast<float*>(tr + DeltaRecord::kSquare);
-    float *tmp = A + C * PITCH, *ghi = tmp + 64 * 34, *glo = ghi + C, *be = glo + C, *until = be + C, *left = until + C, *since = left + C, *red = since + C;
+    float *tmp = A + C * PITCH, *ghi = tmp + 64 * 34, *glo = ghi + C, *be = glo + C, *until = be + C, *left = until + C, *since = left + C, *bound = since + C;
+    uint32_t* red = reinterpret_cast<uint32_t*>(bound + 4);
     constexpr int LO = KEY * 128;                                     // lo panels behind the hi panels
     const aussm_b200_delta_t& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -161,7 +162,8 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
     constexpr int PIECES = C * KEY / 8 / NT;
     int ek, eq;
     {
-        float fk[PIECES][8], fq[PIECES][8], m[2] = {};
+        float fk[PIECES][8], fq[PIECES][8];
+        uint32_t m[2] = {};
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
             const int piece = tid + x * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8;
@@ -176,8 +178,8 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) { m[0] = max8(fk[x], m[0]); m[1] = max8(fq[x], m[1]); }
         block_max<8>(m, red);
-        ek = part_exponent(m[0]);
-        eq = part_exponent(m[1]);
+        ek = rank_exponent(m[0]);
+        eq = rank_exponent(m[1]);
         const float sk = pow2_float(ek), sq = pow2_float(eq);
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
@@ -250,18 +252,20 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             head[kGHi + i0] = h0; head[kGHi + i1] = h1;
             head[kGLo + i0] = glo[i0]; head[kGLo + i1] = glo[i1];
             if (lane == 31) head[kGamma] = e1;
-            float um = fmaxf(u0, u1), em = fabsf(p.scale) * fmaxf(e0, e1);
+            auto finite = [](float x) { return x <= 3.402823466e38f ? x : 0.f; };
+            float um = fmaxf(finite(u0), finite(u1)), em = fabsf(p.scale) * fmaxf(finite(e0), finite(e1));
 #pragma unroll
             for (int m = 16; m; m >>= 1) {
                 um = fmaxf(um, __shfl_xor_sync(0xffffffffu, um, m));
                 em = fmaxf(em, __shfl_xor_sync(0xffffffffu, em, m));
             }
-            if (lane == 0) { red[48] = um; red[49] = em; }
+            if (lane == 0) { bound[0] = um; bound[1] = em; }
             if (h + 1 < hk * r + r) ask(h + 1);
         }
         __syncthreads();
         // A to shared memory, P kept in the fragments
-        float pr[4][4], m[3] = {};
+        float pr[4][4];
+        uint32_t m[3] = {};
         {
             const int i0 = rb * 16 + (lane >> 2);
 #pragma unroll
@@ -272,12 +276,12 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                     const float d = j <= i ? expf((ghi[i] - ghi[j]) + (glo[i] - glo[j])) : 0.f;
                     A[i * PITCH + j] = j < i ? be[i] * d * (kk[x][y] * unk * unk) : 0.f;
                     pr[x][y] = j <= i ? p.scale * d * (qk[x][y] * unk * unq) : 0.f;
-                    m[0] = fmaxf(m[0], fabsf(pr[x][y]));
+                    m[0] = max(m[0], rank_of(pr[x][y]));
                 }
         }
         // Kt and Qt from the parts of K and Q; their largest magnitudes are at most these
-        const int et = part_exponent(red[48] * pow2_float(min(127, 14 - ek))),
-                  eqt = part_exponent(red[49] * pow2_float(min(127, 14 - eq)));
+        const int et = part_exponent(bound[0] * pow2_float(min(127, 14 - ek))),
+                  eqt = part_exponent(bound[1] * pow2_float(min(127, 14 - eq)));
         {
             const float s = unk * pow2_float(et), sq = unq * pow2_float(eqt);
 #pragma unroll
@@ -304,12 +308,12 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                m[1] = fmaxf(m[1], fabsf(ft[x][i]));
-                m[2] = fmaxf(m[2], fabsf(ft[x][i] * left[col + i]));
+                m[1] = max(m[1], rank_of(ft[x][i]));
+                m[2] = max(m[2], rank_of(ft[x][i] * left[col + i]));
             }
         }
         block_max<8>(m, red);
-        const int ep = part_exponent(m[0]), ett = part_exponent(m[1]), el = part_exponent(m[2]);
+        const int ep = rank_exponent(m[0]), ett = rank_exponent(m[1]), el = rank_exponent(m[2]);
         store_fragments(rec + a.rec.p(), 8192, rb * 16, half * 32, pr, pow2_float(ep));
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -346,17 +350,17 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 }
             }
         }
-        float mw[1] = {};
+        uint32_t mw[1] = {};
         const float unw = pow2_float(-el) * unk;
 #pragma unroll
         for (int x = 0; x < TILES; ++x)
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
                 w[x][y] *= unw;
-                mw[0] = fmaxf(mw[0], fabsf(w[x][y]));
+                mw[0] = max(mw[0], rank_of(w[x][y]));
             }
         block_max<8>(mw, red + 24);
-        const int ew = part_exponent(mw[0]);
+        const int ew = rank_exponent(mw[0]);
 #pragma unroll
         for (int x = 0; x < TILES / 4; ++x) {
             float f[4][4];

@@ -70,9 +70,9 @@ __device__ __forceinline__ void zero8(float (&f)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = 0.f;
 }
-__device__ __forceinline__ float max8(const float (&f)[8], float m) {
+__device__ __forceinline__ uint32_t max8(const float (&f)[8], uint32_t m) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
+    for (int i = 0; i < 8; ++i) m = max(m, rank_of(f[i]));
     return m;
 }
 __device__ __forceinline__ void split8(const float (&f)[8], float s, uint4& hi, uint4& lo) {
@@ -100,22 +100,20 @@ __device__ __forceinline__ void join8(const uint8_t* hi, const uint8_t* lo, floa
     }
 }
 
-// maxima of N values over the block of WARPS warps; `buf` has N * WARPS floats and is free again after the next barrier
+// maxima of N ranks over the block of WARPS warps; `buf` has N * WARPS words and is free again after the next barrier
 template <int WARPS, int N>
-__device__ __forceinline__ void block_max(float (&v)[N], float* buf) {
+__device__ __forceinline__ void block_max(uint32_t (&v)[N], uint32_t* buf) {
 #pragma unroll
-    for (int m = 16; m; m >>= 1)
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = fmaxf(v[i], __shfl_xor_sync(0xffffffffu, v[i], m));
+    for (int i = 0; i < N; ++i) v[i] = __reduce_max_sync(0xffffffffu, v[i]);
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
         for (int i = 0; i < N; ++i) buf[i * WARPS + (threadIdx.x >> 5)] = v[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        v[i] = 0.f;
+        v[i] = 0;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) v[i] = fmaxf(v[i], buf[i * WARPS + w]);
+        for (int w = 0; w < WARPS; ++w) v[i] = max(v[i], buf[i * WARPS + w]);
     }
 }
 

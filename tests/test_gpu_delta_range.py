@@ -1,0 +1,123 @@
+"""Gated delta rule with single entries far out of the range of the others, infinite or NaN, step by step against the
+recurrence in float64.
+
+Tolerances.  What a query or its gradient of the output touches is its own row of each product, so the output of step t is
+off by at most FWD (see test_gpu_delta.py: 8 products of 2^-21, sqrt(128) between a sum of magnitudes and its result) of
+|q_t| times the largest o / |q| of the head, whatever the other queries hold, and its gradient dq_t by BWD of |go_t| times the
+largest dq / |go|.  Sums over the steps of a chunk (64) are rounded to the largest of their terms: a large value shows in the
+other outputs of its value column and chunk, by FWD of itself, and nowhere else.
+"""
+import math
+
+import pytest
+import torch
+
+import aussm_b200
+from aussm_b200.delta import gated_delta_rule, gated_delta_step
+from oracle.delta import gated_delta_ref
+from tests.test_gpu_delta import BWD, FWD, NAMES, make
+
+pytestmark = pytest.mark.gpu
+CHUNK = 64
+
+
+def run(d, go=None, fn=gated_delta_rule, dtype=None):
+    """Output, final state and (with go) the gradients."""
+    x = {n: (t if dtype is None else t.to(dtype)).detach().clone().requires_grad_(go is not None) for n, t in d.items()}
+    kw = dict(return_final_state=True) if fn is gated_delta_rule else {}
+    o, s = fn(*(x[n] for n in NAMES[:5]), initial_state=x["state"], **kw)
+    grads = None if go is None else dict(zip(x, torch.autograd.grad(o, list(x.values()), go.to(o.dtype))))
+    return o.detach(), s.detach(), grads
+
+
+def truth(d, go=None):
+    return run(d, go, gated_delta_ref, torch.float64)
+
+
+def go_like(d, seed=5):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(d["v"].shape, device="cuda", generator=gen).to(d["v"].dtype)
+
+
+def by_rows(name, got, want, size, tol, steps=None):
+    """|got - want| of every step within tol of `size` (b, l, heads) times the head's largest |want| / size, and half a step
+    of the type; on `steps` (b, l), default all."""
+    want = want.double()
+    size = size.double()[..., None]
+    there = torch.ones(want.shape[:2], dtype=torch.bool, device=want.device) if steps is None else steps
+    ratio = torch.where(there[:, :, None, None] & (size > 0), want.abs() / size.clamp(min=1e-300), 0)
+    most = ratio.amax((1, 3), keepdim=True)
+    half = torch.finfo(got.dtype).eps / 2 if got.dtype != torch.float32 else 0.0
+    # results below the normal numbers of their type are rounded to its smallest step
+    allowed = tol * size * most + half * want.abs() + torch.finfo(got.dtype).tiny
+    err = (got.double() - want).abs()[there]
+    assert torch.isfinite(got[there]).all(), name
+    assert (err <= allowed.expand(want.shape)[there]).all(), f"{name}: {float((err / allowed.expand(want.shape)[there]).max()):.3g} times the tolerance"
+
+
+def wide(d, n):
+    """(b, l, hk) -> (b, l, hv)"""
+    return n.repeat_interleave(d["v"].shape[2] // n.shape[2], 2)
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_an_infinite_query_stays_with_its_step(bad, dtype):
+    d = make(63, 1, 150, 1, 2, 64, 64, dtype)
+    clean = {n: t.clone() for n, t in d.items()}
+    d["q"][0, 77, 0, 3] = bad
+    go = go_like(d)
+    (o, s, g), (o64, s64, g64) = run(d, go), truth(clean, go)
+    others = torch.ones(1, 150, dtype=torch.bool, device="cuda")
+    others[0, 77] = False
+    assert not torch.isfinite(o[0, 77]).any()
+    by_rows("o", o, o64, wide(d, clean["q"].double().norm(dim=-1)), FWD, others)
+    assert float((s - s64).abs().max()) <= FWD * float(s64.abs().max())
+    by_rows("grad q", g["q"], g64["q"], torch.ones_like(g["q"][..., 0]), BWD)      # none of them sees a query
+    for n in ("k", "v", "g", "beta"):                            # the next chunk does not see it, this one may not hide it
+        a, b, half = g[n].double(), g64[n], torch.finfo(g[n].dtype).eps / 2
+        most = float(b.abs().max())
+        assert ((a - b).abs()[:, 128:] <= BWD * most + half * b.abs()[:, 128:]).all(), n
+        assert (((a - b).abs() <= BWD * most + half * b.abs()) | ~torch.isfinite(a))[:, 78:].all(), n
+    assert not torch.isfinite(g["v"][0, :78]).any() and not torch.isfinite(g["k"][0, :78]).any()
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_an_outlying_gradient_stays_with_its_step(bad):
+    """One step of the gradient of o: the other steps' dq do not see it."""
+    d = make(64, 1, 150, 1, 1, 64, 80)
+    go = go_like(d)
+    clean = go.clone()
+    if math.isfinite(bad):
+        go[0, 30] *= bad
+    else:
+        go[0, 30, 0, 5] = bad
+    _, _, g = run(d, go)
+    _, _, g64 = truth(d, clean)
+    others = torch.ones(1, 150, dtype=torch.bool, device="cuda")
+    others[0, 30] = False
+    by_rows("grad q", g["q"], g64["q"], torch.ones_like(g["q"][..., 0]), BWD, others)
+    if math.isfinite(bad):
+        by_rows("grad q", g["q"] / bad, g64["q"], torch.ones_like(g["q"][..., 0]), BWD, ~others)
+    for n in ("k", "v", "g", "beta"):
+        assert float((g[n][:, 64:] - g64[n][:, 64:]).abs().max()) <= BWD * float(g64[n].abs().max()), n
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("name", ["v", "k", "beta", "g"])
+def test_what_is_not_finite_is_never_hidden(name, bad):
+    """From its step on nothing that depends on it is finite; before it, a step of its chunk is right or not finite, and a
+    step of an earlier chunk is right."""
+    d = make(68, 1, 200, 1, 1, 64, 64)
+    clean = truth(d)[0]
+    d[name][(0, 90, 0, 5)[:d[name].dim()]] = bad
+    o, s, _ = run(d)
+    err = (o - clean).abs()
+    tol = FWD * float(clean.abs().max())
+    assert (err[:, :64] <= tol).all()
+    assert ((err <= tol) | ~torch.isfinite(o))[:, :90].all()
+    cols = [5] if name == "v" else list(range(64))
+    assert not torch.isfinite(o[0, 91:, 0, cols]).any() and not torch.isfinite(s[0, 0, :, cols]).all(0).any()
+    if name == "v":
+        rest = [c for c in range(64) if c != 5]
+        assert (err[..., rest] <= tol).all()
