@@ -32,22 +32,26 @@ constexpr int kDeltaChunk = 64;
 // from shared memory: panels of 64 columns (64 rows of 128 bytes, 16-byte pieces swizzled by the row), the hi panels
 // and then the lo panels.  Rows of 128 bytes serve as K-major and as MN-major operands alike.
 //
+// Queries differ in size, and no output has a share in another's query: rows of Q are brought to one size by a power of two
+// of their own, r_i, before anything else (Q / r in P and Qt).  O's rows are multiplied with r_i when they leave, dO's rows
+// with r_i when they come in as the operand of P and Qt.
+//
 // Per chunk and value head one record of such tiles (`key` = DK rounded up to 64 or 128):
 struct DeltaRecord {
     int key;                                            // columns of W, Kt, Q
-    static constexpr int kHead = 1024;                  // bytes of the header
+    static constexpr int kHead = 1536;                  // bytes of the header
     static constexpr int kSquare = 16384;               // bytes of a 64 x 64 tile, hi and lo
     __host__ __device__ int tile() const { return key * 256; }
     __host__ __device__ int w() const { return kHead; }                             // W = T beta e^G K
     __host__ __device__ int kt() const { return kHead + tile(); }                   // Kt = e^(G_C - G) K
-    __host__ __device__ int q() const { return kHead + 2 * tile(); }                // Qt = scale e^G Q
+    __host__ __device__ int q() const { return kHead + 2 * tile(); }                // Qt = scale e^G Q / r
     __host__ __device__ int t() const { return kHead + 3 * tile(); }                // T = (I + A)^-1
-    __host__ __device__ int p() const { return kHead + 3 * tile() + kSquare; }      // P
+    __host__ __device__ int p() const { return kHead + 3 * tile() + kSquare; }      // P / r
     __host__ __device__ int bytes() const { return kHead + 3 * tile() + 2 * kSquare; }
 };
 // header, in floats: what a stored part is to be multiplied with (1 / S) ...
 enum : int { kUnW = 0, kUnKt = 1, kUnQ = 2, kUnT = 3, kUnP = 4, kGamma = 5 /* e^(G_C) */,
-             kBeta = 16 /* 64 */, kGHi = 80, kGLo = 144 /* G_i = hi + lo, 64 each */ };
+             kBeta = 16 /* 64 */, kGHi = 80, kGLo = 144 /* G_i = hi + lo, 64 each */, kRow = 208 /* r, 64 */ };
 
 // byte offset of element (row, col) in the hi panels of a tile
 __host__ __device__ __forceinline__ int panel_at(int row, int col) {

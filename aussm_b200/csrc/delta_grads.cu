@@ -58,7 +58,9 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
     float *ghi = vec, *glo = vec + 64, *be = vec + 128, *rowa = vec + 192 /* (4, 64) */, *rowk = vec + 448 /* (4, 64) */,
           *rowz = vec + 704 /* (4, 64) */;
     __shared__ uint32_t red[6 * WARPS];
-    __shared__ float xv[8][C], ssum[WARPS], am[C], kkt[C];
+    __shared__ uint32_t e1max[4][C];
+    __shared__ int eo[C], eqs[C];                        // exponents of the rows of dO, of Q
+    __shared__ float go_shrink[C], xv[8][C], ssum[WARPS], am[C], kkt[C];
     const aussm_b200_delta_t& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int rb = warp & 3, cq = warp >> 2;             // 16 rows, a quarter of the columns
@@ -78,7 +80,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
 
         // ---- products over the value columns -------------------------------------------------------------------
         float dp[2][4] = {}, xn[2][4] = {}, dqt[NW][4] = {}, zz[NW][4] = {}, dkt[NW][4] = {};
-        int e[5] = {115, 115, 115, 115, 115};            // exponents of dO, X, V', S, dS
+        int e[5] = {115, 115, 115, 115, 115};            // exponents of dO (this thread's row), X, V', S, dS
         float dotv = 0.f, dots = 0.f;
         for (int v0 = 0; v0 < DV; v0 += VS) {
             const int cols = DV - v0;
@@ -95,7 +97,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             const int pt = panel_at(dv, 8 * grp);
             {
             float f[3][8], s[KEY / 64][8];
-            uint32_t m[4] = {};
+            uint32_t m[3] = {};
             if (row < rows) load8(go + row * p.go_stride[1] + v0, col, cols, a.vec_go, f[0]); else zero8(f[0]);
             auto parts = [&](const uint8_t* base, int groups, int g8, float (&o)[8]) {
                 const uint8_t* x = base + ((size_t)g8 * 128 + l) * 16;
@@ -115,13 +117,15 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             for (int y = 0; y < KEY / 64; ++y) {
                 if (there) parts(a.states + piece * DeltaPlan::state_bytes(KEY), KEY / 8, grp + 8 * y, s[y]);
                 else zero8(s[y]);
-                m[3] = max8(s[y], m[3]);
+                m[2] = max8(s[y], m[2]);
             }
 #pragma unroll
-            for (int y = 0; y < 3; ++y) m[y] = max8(f[y], 0u);
+            for (int y = 0; y < 2; ++y) m[y] = max8(f[1 + y], 0u);
+            unit(0, row_max<8>(max8(f[0], 0u)));         // a row of dO meets no other: it has an exponent of its own
+            if (col == 0) { eo[row] = e[0]; go_shrink[row] = shrink[0]; }
             block_max<WARPS>(m, red);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) unit(y, m[y]);
+            for (int y = 0; y < 3; ++y) unit(1 + y, m[y]);
             put8(sm + Smem::kGo + panel_at(row, col), SQ_LO, f[0], pow2_float(e[0]));
             put8(sm + Smem::kX + pt, SQ_LO, f[1], pow2_float(e[1]));
             put8(sm + Smem::kNew + pt, SQ_LO, f[2], pow2_float(e[2]));
@@ -130,15 +134,16 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                 put8(sm + Smem::kS + panel_at(dv, 8 * grp + 64 * y), ST_LO, s[y], pow2_float(e[3]));
             }
             if (v0) {                                    // the sums so far, in the new unit
+                const float go_row[2] = {go_shrink[rb * 16 + g], go_shrink[rb * 16 + g + 8]};
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { dp[y][i] *= shrink[0] * shrink[2]; xn[y][i] *= shrink[1] * shrink[2]; }
+                    for (int i = 0; i < 4; ++i) { dp[y][i] *= go_row[i >> 1] * shrink[2]; xn[y][i] *= shrink[1] * shrink[2]; }
 #pragma unroll
                 for (int y = 0; y < NW; ++y)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        dqt[y][i] *= shrink[0] * shrink[3];
+                        dqt[y][i] *= go_row[i >> 1] * shrink[3];
                         zz[y][i] *= shrink[1] * shrink[3];
                     }
             }
@@ -266,13 +271,13 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         if (lane == 0) ssum[warp] = dots;
 
         // ---- K, Q; K K^T ----------------------------------------------------------------------------------------
-        int ek, eq;
+        int ek;
         {
             constexpr int PIECES = C * KEY / 8 / NT;
             const T* q = static_cast<const T*>(a.in.q) + b * p.q_stride[0] + t0 * p.q_stride[1] + hk * p.q_stride[2];
             const T* k = static_cast<const T*>(a.in.k) + b * p.k_stride[0] + t0 * p.k_stride[1] + hk * p.k_stride[2];
             float fk[PIECES][8], fq[PIECES][8];
-            uint32_t m[2] = {};
+            uint32_t m[1] = {}, mq[PIECES];
 #pragma unroll
             for (int y = 0; y < PIECES; ++y) {
                 const int piece = tid + y * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8;
@@ -284,20 +289,20 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                     zero8(fq[y]);
                 }
                 m[0] = max8(fk[y], m[0]);
-                m[1] = max8(fq[y], m[1]);
+                mq[y] = row_max<KEY / 8>(max8(fq[y], 0u));
             }
             block_max<WARPS>(m, red);
             ek = rank_exponent(m[0]);
-            eq = rank_exponent(m[1]);
 #pragma unroll
             for (int y = 0; y < PIECES; ++y) {
-                const int piece = tid + y * NT, pk = panel_at(piece / (KEY / 8), piece % (KEY / 8) * 8);
+                const int piece = tid + y * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8, pk = panel_at(row, col), eq = rank_exponent(mq[y]);
                 put8(sm + Smem::kK + pk, ST_LO, fk[y], pow2_float(ek));
                 put8(sm + Smem::kQ + pk, ST_LO, fq[y], pow2_float(eq));
+                if (col == 0) eqs[row] = eq;
             }
         }
         __syncthreads();
-        const float unk = pow2_float(-ek), unq = pow2_float(-eq);
+        const float unk = pow2_float(-ek);
         float kk[2][4] = {};
         if (cq <= rb) {
 #pragma unroll
@@ -318,11 +323,12 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         }
         // the terms with states: dQt and dKt - beta Gamma Z (they take the places of dqt and dkt), their products with Q and K
         {
-            const float fq = pow2_float(-e[0]) * pow2_float(-e[3]), fz = pow2_float(-e[1]) * pow2_float(-e[3]), fk = pow2_float(-e[2]) * pow2_float(-e[4]);
+            const float fz = pow2_float(-e[1]) * pow2_float(-e[3]), fk = pow2_float(-e[2]) * pow2_float(-e[4]);
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
                 const int i = rb * 16 + g + 8 * z;
                 const float since = expf(ghi[i] + glo[i]), until = expf((ghi[C - 1] - ghi[i]) + (glo[C - 1] - glo[i]));
+                const float fq = pow2_float(-eo[i]) * pow2_float(-e[3]), unq = pow2_float(-eqs[i]);
                 float sumq = 0.f, sumz = 0.f, sumk = 0.f;
 #pragma unroll
                 for (int y = 0; y < NW; ++y) {
@@ -357,23 +363,24 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             }
         }
         // E1 = scale D dO V'^T (gradient of Q K^T), E = -beta D X V'^T (gradient of K K^T), F = their part in G_i - G_j
-        uint32_t m[2] = {};
+        uint32_t m[1] = {}, mrow[2] = {};
         float bsum[2] = {};                   // dbeta of rows g and g + 8: sum of -D X V'^T K K^T
         {
             const uint8_t* pt = reinterpret_cast<const uint8_t*>(head) + a.rec.p();
-            const float unp = head[kUnP], fp = pow2_float(-e[0]) * pow2_float(-e[2]), fx = pow2_float(-e[1]) * pow2_float(-e[2]);
+            const float unp = head[kUnP], fx = pow2_float(-e[1]) * pow2_float(-e[2]);
 #pragma unroll
             for (int y = 0; y < 2; ++y)
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
                     const int i = rb * 16 + g + 8 * z, j = cq * 16 + 8 * y + 2 * t;
                     const int pa = panel_at(i, j);
+                    const float fp = pow2_float(-eo[i]) * pow2_float(-e[2]), unit_q = pow2_float(13 - eqs[i]);     // r_i
                     float2 ph = make_float2(0.f, 0.f), pl = ph;
                     if (cq <= rb) {
                         ph = __half22float2(*reinterpret_cast<const __half2*>(pt + pa));
                         pl = __half22float2(*reinterpret_cast<const __half2*>(pt + 8192 + pa));
                     }
-                    const float pv[2] = {(ph.x + pl.x) * unp, (ph.y + pl.y) * unp};
+                    const float pv[2] = {(ph.x + pl.x) * unp * unit_q, (ph.y + pl.y) * unp * unit_q};
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
                         const bool in = j + w <= i, below = j + w < i;
@@ -384,8 +391,8 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                         F[i * FP + j + w] = below ? fmaf(dpv, pv[w], be[i] * mx * kkv) : 0.f;
                         dp[y][2 * z + w] = p.scale * d * dpv;
                         xn[y][2 * z + w] = be[i] * mx;
-                        m[0] = max(m[0], rank_of(dp[y][2 * z + w]));
-                        m[1] = max(m[1], rank_of(xn[y][2 * z + w]));
+                        mrow[z] = max(mrow[z], rank_of(dp[y][2 * z + w]));
+                        m[0] = max(m[0], rank_of(xn[y][2 * z + w]));
                     }
                 }
         }
@@ -393,19 +400,42 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         for (int z = 0; z < 2; ++z) {
             bsum[z] += __shfl_xor_sync(0xffffffffu, bsum[z], 1);
             bsum[z] += __shfl_xor_sync(0xffffffffu, bsum[z], 2);
-            if (t == 0) rowz[cq * 64 + rb * 16 + g + 8 * z] += bsum[z];
+            mrow[z] = row_max<4>(mrow[z]);
+            if (t == 0) {
+                rowz[cq * 64 + rb * 16 + g + 8 * z] += bsum[z];
+                e1max[cq][rb * 16 + g + 8 * z] = mrow[z];
+            }
         }
         block_max<WARPS>(m, red + 2 * WARPS);
-        const int e1 = rank_exponent(m[0]), e2 = rank_exponent(m[1]);
+        // E1's rows have exponents e1 of their own in E1 K, where they meet no other; in E1^T Q the rows of Q make up for them,
+        // as q 2^(-e1 - top) with the largest of these in the usual range.  Rows 2^24 below that one add nothing.
+        const int e2 = rank_exponent(m[0]);
+        auto e1_of = [&](int i) { return rank_exponent(max(max(e1max[0][i], e1max[1][i]), max(e1max[2][i], e1max[3][i]))); };
+        const int e1[2] = {e1_of(rb * 16 + g), e1_of(rb * 16 + g + 8)};
+        const int top = __reduce_max_sync(0xffffffffu, max(-e1_of(lane) - eqs[lane], -e1_of(lane + 32) - eqs[lane + 32]));
+#pragma unroll
+        for (int y = 0; y < C * KEY / 8 / NT; ++y) {
+            const int piece = tid + y * NT, row = piece / (KEY / 8), down = -e1_of(row) - eqs[row] - top;
+            const __half2 f = __float2half2_rn(down < -24 ? 0.f : pow2_float(down));
+#pragma unroll
+            for (int lo = 0; lo <= ST_LO; lo += ST_LO) {
+                uint4* at_q = reinterpret_cast<uint4*>(sm + Smem::kQ + lo + panel_at(row, piece % (KEY / 8) * 8));
+                uint4 x = *at_q;
+                __half2* h2 = reinterpret_cast<__half2*>(&x);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h2[i] = __hmul2(h2[i], f);
+                *at_q = x;
+            }
+        }
         {
-            const float s1 = pow2_float(e1), s2 = pow2_float(e2);
+            const float s1[2] = {pow2_float(e1[0]), pow2_float(e1[1])}, s2 = pow2_float(e2);
 #pragma unroll
             for (int y = 0; y < 2; ++y)
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
                     const int i = rb * 16 + g + 8 * z, j = cq * 16 + 8 * y + 2 * t, pa = panel_at(i, j);
                     uint32_t hi, lo;
-                    split2(dp[y][2 * z] * s1, dp[y][2 * z + 1] * s1, hi, lo);
+                    split2(dp[y][2 * z] * s1[z], dp[y][2 * z + 1] * s1[z], hi, lo);
                     *reinterpret_cast<uint32_t*>(sm + Smem::kE1 + pa) = hi;
                     *reinterpret_cast<uint32_t*>(sm + Smem::kE1 + SQ_LO + pa) = lo;
                     // E + E^T: the strictly lower triangle and its mirror image (the diagonal is zero)
@@ -470,17 +500,18 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             }
         }
         {
-            const float f1 = pow2_float(-e1), f2 = pow2_float(-e2);
+            const float f2 = pow2_float(-e2), fk = pow2_float(top >> 1), fk2 = pow2_float(top - (top >> 1));
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
                 const int i = rb * 16 + g + 8 * z;
+                const float f1 = pow2_float(-e1[z]);
 #pragma unroll
                 for (int y = 0; y < NW; ++y) {
                     const int col = cq * (KEY / 4) + 8 * y + 2 * t;
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
                         accq[i * KEY + col + w] += fmaf(sq[y][2 * z + w] * f1, unk, dqt[y][2 * z + w]);
-                        acck[i * KEY + col + w] += sk[y][2 * z + w] * f1 * unq + se[y][2 * z + w] * f2 * unk + dkt[y][2 * z + w];
+                        acck[i * KEY + col + w] += sk[y][2 * z + w] * fk * fk2 + se[y][2 * z + w] * f2 * unk + dkt[y][2 * z + w];
                     }
                 }
             }

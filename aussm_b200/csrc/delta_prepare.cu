@@ -125,7 +125,7 @@ __device__ __forceinline__ void invert(float* A, float* tmp) {
 template <int KEY>
 struct PrepareSmem {
     static constexpr int kTile = KEY * 256;
-    static constexpr int kBytes = 2 * kTile + DeltaRecord::kSquare + C * PITCH * 4 + 64 * 34 * 4 + 6 * C * 4 + 4 * 4 + 32 * 4;
+    static constexpr int kBytes = 2 * kTile + DeltaRecord::kSquare + C * PITCH * 4 + 64 * 34 * 4 + 7 * C * 4 + 4 * 4 + 32 * 4;
 };
 
 template <typename T, int KEY>
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
     uint8_t *kr = sm, *qr = sm + Smem::kTile;
     uint8_t* tr = qr + Smem::kTile;                                   // T beta e^G
     float* A = reinterpret_cast<float*>(tr + DeltaRecord::kSquare);
-    float *tmp = A + C * PITCH, *ghi = tmp + 64 * 34, *glo = ghi + C, *be = glo + C, *until = be + C, *left = until + C, *since = left + C, *bound = since + C;
+    float *tmp = A + C * PITCH, *ghi = tmp + 64 * 34, *glo = ghi + C, *be = glo + C, *until = be + C, *left = until + C, *since = left + C, *unit = since + C, *bound = unit + C;
     uint32_t* red = reinterpret_cast<uint32_t*>(bound + 4);
     constexpr int LO = KEY * 128;                                     // lo panels behind the hi panels
     const aussm_b200_delta_t& p = a.p;
@@ -160,10 +160,10 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
 
     // K and Q: 16-byte pieces of a tile, KEY / 32 of each per thread
     constexpr int PIECES = C * KEY / 8 / NT;
-    int ek, eq;
+    int ek;
     {
         float fk[PIECES][8], fq[PIECES][8];
-        uint32_t m[2] = {};
+        uint32_t m[1] = {}, mq[PIECES];
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
             const int piece = tid + x * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8;
@@ -176,16 +176,17 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             }
         }
 #pragma unroll
-        for (int x = 0; x < PIECES; ++x) { m[0] = max8(fk[x], m[0]); m[1] = max8(fq[x], m[1]); }
+        for (int x = 0; x < PIECES; ++x) { m[0] = max8(fk[x], m[0]); mq[x] = row_max<KEY / 8>(max8(fq[x], 0u)); }
         block_max<8>(m, red);
         ek = rank_exponent(m[0]);
-        eq = rank_exponent(m[1]);
-        const float sk = pow2_float(ek), sq = pow2_float(eq);
+        const float sk = pow2_float(ek);
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
             const int piece = tid + x * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8, at = panel_at(row, col);
+            const int eq = rank_exponent(mq[x]);
             put8(kr + at, LO, fk[x], sk);
-            put8(qr + at, LO, fq[x], sq);
+            put8(qr + at, LO, fq[x], pow2_float(eq));              // 2^13 Q / r
+            if (col == 0) unit[row] = pow2_float(13 - eq);
         }
     }
     __syncthreads();
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             }
         }
     }
-    const float unk = pow2_float(-ek), unq = pow2_float(-eq);
+    const float unk = pow2_float(-ek), unq = pow2_float(-13);
 
     for (int h = hk * r; h < hk * r + r; ++h) {
         uint8_t* rec = record(h);
@@ -251,6 +252,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             head[kBeta + i0] = be[i0]; head[kBeta + i1] = be[i1];
             head[kGHi + i0] = h0; head[kGHi + i1] = h1;
             head[kGLo + i0] = glo[i0]; head[kGLo + i1] = glo[i1];
+            head[kRow + i0] = unit[i0]; head[kRow + i1] = unit[i1];
             if (lane == 31) head[kGamma] = e1;
             auto finite = [](float x) { return x <= 3.402823466e38f ? x : 0.f; };
             float um = fmaxf(finite(u0), finite(u1)), em = fabsf(p.scale) * fmaxf(finite(e0), finite(e1));
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
         }
         // Kt and Qt from the parts of K and Q; their largest magnitudes are at most these
         const int et = part_exponent(bound[0] * pow2_float(min(127, 14 - ek))),
-                  eqt = part_exponent(bound[1] * pow2_float(min(127, 14 - eq)));
+                  eqt = part_exponent(bound[1] * 2.f);
         {
             const float s = unk * pow2_float(et), sq = unq * pow2_float(eqt);
 #pragma unroll

@@ -204,7 +204,10 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     __shared__ uint64_t row_s[4], row_n[4];
     __shared__ uint32_t holder;
     __shared__ float un_s[2][128], un_v[2][128], un_n[128], max_s[PARTS][128], max_n[PARTS][128];
-    __shared__ __align__(16) float betas[C];
+    // Factors of the steps: V comes in times beta and O goes out times r, dO comes in times r and dV goes out times beta.  Those
+    // of the way out are copied with the ones of the way in, and chunk i + 4 is asked for when v_done (a_done) of i + 2 is
+    // seen, which the issuing warp commits after x_free of i: four of them.
+    __shared__ __align__(16) float factors[C], out_factors[4][C];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const aussm_b200_delta_t& p = a.p;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -353,7 +356,11 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
         auto fetch = [&](int i) {
             const int t0 = chunk_at(i) * C, rows = min(C, p.L - t0);
             const T* from = src + (long long)t0 * a.v_stride[1];
-            if (me < C / 4) cp_async16(betas + 4 * me, reinterpret_cast<const float*>(record(i)) + kBeta + 4 * me);
+            if (me < C / 2) {
+                const int x = me % (C / 4) * 4;
+                const bool out = me >= C / 4;
+                cp_async16((out ? out_factors[i & 3] : factors) + x, reinterpret_cast<const float*>(record(i)) + (out != BWD ? kRow : kBeta) + x);
+            }
             if (a.vec_v) {
                 constexpr int E = 16 / (int)sizeof(T), PIECES = 128 / E, ROWS = 128 / PIECES;      // rows an instruction
                 int row = me / PIECES;
@@ -381,11 +388,10 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             cp_async_wait<0>();
             arrive(&v_loaded);
             if (!warp_wait(&v_loaded, i & 1, a.status)) break;
-            // two steps of this lane's column, times beta
+            // two steps of this lane's column, times their factors
             auto pair = [&](int t) {
-                float2 f = make_float2(to_f32(tile[t * 128 + me]), to_f32(tile[(t + 1) * 128 + me]));
-                if (!BWD) f = __fmul2_rn(f, *reinterpret_cast<const float2*>(betas + t));
-                return f;
+                return __fmul2_rn(make_float2(to_f32(tile[t * 128 + me]), to_f32(tile[(t + 1) * 128 + me])),
+                                  *reinterpret_cast<const float2*>(factors + t));
             };
             float m0 = 0.f, m1 = 0.f;
 #pragma unroll 1
@@ -451,7 +457,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             const float uns = un_s[ph][me], f1 = uns * unq, unn = un_n[me], f2 = unn * un2;
             T* to = dst + (long long)t0 * p.HV * p.DV;
             float4* keep = reinterpret_cast<float4*>(a.rows) + at * (C / 4 * 128) + me;
-            const float4* be = reinterpret_cast<const float4*>(head + kBeta);
+            const float4* out_factor = reinterpret_cast<const float4*>(out_factors[i & 3]);
 #pragma unroll 1
             for (int t = 0; t < C; t += 16) {
                 uint32_t r1[16], r2[16];
@@ -470,13 +476,11 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                     y[u] = w.x;
                     y[u + 1] = w.y;
                 }
-                if (BWD) {
 #pragma unroll
-                    for (int u = 0; u < 16; u += 4) {
-                        if (mine) keep[(t + u) / 4 * 128] = make_float4(y[u], y[u + 1], y[u + 2], y[u + 3]);
-                        const float4 f = be[(t + u) / 4];
-                        y[u] *= f.x; y[u + 1] *= f.y; y[u + 2] *= f.z; y[u + 3] *= f.w;
-                    }
+                for (int u = 0; u < 16; u += 4) {
+                    if (BWD && mine) keep[(t + u) / 4 * 128] = make_float4(y[u], y[u + 1], y[u + 2], y[u + 3]);
+                    const float4 f = out_factor[(t + u) / 4];
+                    y[u] *= f.x; y[u + 1] *= f.y; y[u + 2] *= f.z; y[u + 3] *= f.w;
                 }
                 if (t + 16 <= rows) {
 #pragma unroll

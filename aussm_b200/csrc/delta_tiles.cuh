@@ -100,6 +100,14 @@ __device__ __forceinline__ void join8(const uint8_t* hi, const uint8_t* lo, floa
     }
 }
 
+// maximum over LANES neighbouring lanes
+template <int LANES>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+#pragma unroll
+    for (int m = 1; m < LANES; m *= 2) v = max(v, __shfl_xor_sync(0xffffffffu, v, m));
+    return v;
+}
+
 // maxima of N ranks over the block of WARPS warps; `buf` has N * WARPS words and is free again after the next barrier
 template <int WARPS, int N>
 __device__ __forceinline__ void block_max(uint32_t (&v)[N], uint32_t* buf) {

@@ -116,6 +116,18 @@ def test_nobody_is_overtaken(backward, full):
     assert not late, late
 
 
+@pytest.mark.parametrize("backward", [False, True])
+def test_factors_stay_until_the_results_are_out(backward):
+    """The warps that bring V in fetch the factors of the results of chunk i + 1 when they have handed on chunk i, into one of
+    four buffers: not before chunk i - 3 is out."""
+    progs = programs(backward, True)
+    for at, (kind, b, c) in enumerate(progs["out"]):
+        if (kind, b) == ("a", "x_free") and c + 3 < CHUNKS:
+            handed_on = furthest(progs, "out", at)[1]["v_ready"]
+            assert c + 3 not in handed_on, c
+            assert backward or c + 2 in handed_on, c                         # three buffers would not do
+
+
 def test_the_kernel_waits_by_slots():
     """A barrier of two phases is named with its slot wherever it is used."""
     text = open(SOURCE).read()

@@ -60,6 +60,37 @@ def wide(d, n):
     return n.repeat_interleave(d["v"].shape[2] // n.shape[2], 2)
 
 
+@pytest.mark.parametrize("size", [1e-12, 1e3, 1e6, 1e9, 1e12, 1e30])
+@pytest.mark.parametrize("l,hk,hv,dk,dv", [(70, 2, 4, 64, 48), (200, 1, 1, 128, 100), (1100, 1, 2, 72, 64)])
+def test_a_query_of_another_size(size, l, hk, hv, dk, dv):
+    d = make(61, 1, l, hk, hv, dk, dv)
+    for t in (0, 21, l - 1):
+        d["q"][:, t, 0] *= size
+    d["q"][:, 40, 0, 1:] = 0
+    d["q"][:, 40, 0, 0] = size                                   # a single element
+    go = go_like(d)
+    (o, s, g), (o64, s64, g64) = run(d, go if size < 1e20 else None), truth(d, go if size < 1e20 else None)
+    by_rows("o", o, o64, wide(d, d["q"].double().norm(dim=-1)), FWD)
+    assert float((s - s64).abs().max()) <= FWD * float(s64.abs().max())
+    if g is None:
+        return
+    by_rows("grad q", g["q"], g64["q"], torch.ones_like(g["q"][..., 0]), BWD)
+    # the other gradients are sums over later queries: chunk by chunk within BWD of the chunk's largest
+    for n in ("k", "v", "g", "beta"):
+        for c in range(0, l, CHUNK):
+            a, b = g[n][:, c:c + CHUNK].double(), g64[n][:, c:c + CHUNK]
+            assert float((a - b).abs().max()) <= BWD * float(b.abs().max()), (n, c)
+    assert aussm_b200.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 1e9), (torch.float16, 6e4)])
+def test_a_query_of_another_size_in_16_bits(dtype, size):
+    d = make(62, 2, 150, 2, 2, 64, 64, dtype)
+    d["q"][0, 90, 1] *= size
+    o, _, _ = run(d)
+    by_rows("o", o, truth(d)[0], wide(d, d["q"].double().norm(dim=-1)), FWD)
+
+
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_an_infinite_query_stays_with_its_step(bad, dtype):
@@ -82,7 +113,7 @@ def test_an_infinite_query_stays_with_its_step(bad, dtype):
     assert not torch.isfinite(g["v"][0, :78]).any() and not torch.isfinite(g["k"][0, :78]).any()
 
 
-@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("bad", [math.inf, math.nan, 1e9])
 def test_an_outlying_gradient_stays_with_its_step(bad):
     """One step of the gradient of o: the other steps' dq do not see it."""
     d = make(64, 1, 150, 1, 1, 64, 80)
