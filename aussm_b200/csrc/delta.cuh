@@ -35,6 +35,11 @@ constexpr int kDeltaChunk = 64;
 // Queries differ in size, and no output has a share in another's query: rows of Q are brought to one size by a power of two
 // of their own, r_i, before anything else (Q / r in P and Qt).  O's rows are multiplied with r_i when they leave, dO's rows
 // with r_i when they come in as the operand of P and Qt.
+// Keys above 1 would have their share of a tile's scale even where beta is zero (a padded step: unwritten memory may lie
+// there).  Their rows are divided by a power of two kappa_i >= 1 that brings them into 1..2 (unit keys: 1): with k^ = k /
+// kappa, beta^ = beta kappa^2 and v^ = v / kappa the rule is the same, S and O are the same and V'^ = kappa V', X^ = X / kappa.
+// K, beta and V' stand for these in all tiles and kernels; beta^ v^ = (beta kappa) v, dv = (beta kappa) X^, dk = dk^ / kappa,
+// dbeta = kappa^2 dbeta^.
 //
 // Per chunk and value head one record of such tiles (`key` = DK rounded up to 64 or 128):
 struct DeltaRecord {
@@ -51,7 +56,8 @@ struct DeltaRecord {
 };
 // header, in floats: what a stored part is to be multiplied with (1 / S) ...
 enum : int { kUnW = 0, kUnKt = 1, kUnQ = 2, kUnT = 3, kUnP = 4, kGamma = 5 /* e^(G_C) */,
-             kBeta = 16 /* 64 */, kGHi = 80, kGLo = 144 /* G_i = hi + lo, 64 each */, kRow = 208 /* r, 64 */ };
+             kBeta = 16 /* beta kappa, 64 */, kGHi = 80, kGLo = 144 /* G_i = hi + lo, 64 each */, kRow = 208 /* r, 64 */,
+             kKey = 272 /* kappa, 64 */ };
 
 // byte offset of element (row, col) in the hi panels of a tile
 __host__ __device__ __forceinline__ int panel_at(int row, int col) {
@@ -65,6 +71,8 @@ __host__ __device__ __forceinline__ float pow2_float(int k) {
     return 0.f;
 #endif
 }
+// 1 / x for a power of two x from 2^-126 to 2^126
+__device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 // exponent k of the scale 2^k for a tile whose largest magnitude is m
 __device__ __forceinline__ int part_exponent(float m) {
     const int e = (int)((__float_as_uint(m) >> 23) & 0xffu) - 127;
@@ -75,6 +83,10 @@ __device__ __forceinline__ int part_exponent(float m) {
 // stays an infinity (and its lo part a NaN) in the conversion.
 __device__ __forceinline__ uint32_t rank_of(float x) { return (__float_as_uint(x) << 1) + 0x01000000u; }
 __device__ __forceinline__ int rank_exponent(uint32_t r) { return max(-115, min(115, 13 + 128 - (int)(r >> 24))); }
+// exponent of kappa for a row of keys, and the rank of what is left of x behind the division
+__device__ __forceinline__ int key_exponent(uint32_t r) { return max(0, min(126, (int)(r >> 24) - 128)); }
+__device__ __forceinline__ int key_exponent_of(float kappa) { return (int)(__float_as_uint(kappa) >> 23) - 127; }
+__device__ __forceinline__ uint32_t rank_less(uint32_t r, int c) { return r - min(r, (uint32_t)c << 24); }
 // hi and lo parts of two values that are scaled already, packed
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(a, b);

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
     __shared__ uint32_t red[6 * WARPS];
     __shared__ uint32_t e1max[4][C];
     __shared__ int eo[C], eqs[C];                        // exponents of the rows of dO, of Q
-    __shared__ float go_shrink[C], xv[8][C], ssum[WARPS], am[C], kkt[C];
+    __shared__ float kappa[C], go_shrink[C], xv[8][C], ssum[WARPS], am[C], kkt[C];
     const aussm_b200_delta_t& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int rb = warp & 3, cq = warp >> 2;             // 16 rows, a quarter of the columns
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         const T* go = static_cast<const T*>(a.go) + b * p.go_stride[0] + t0 * p.go_stride[1] + h * p.go_stride[2];
         const T* v = static_cast<const T*>(a.in.v) + b * p.v_stride[0] + t0 * p.v_stride[1] + h * p.v_stride[2];
         __syncthreads();                                 // the last head is done with shared memory
-        if (tid < C) { ghi[tid] = head[kGHi + tid]; glo[tid] = head[kGLo + tid]; be[tid] = head[kBeta + tid]; }
+        if (tid < C) { ghi[tid] = head[kGHi + tid]; glo[tid] = head[kGLo + tid]; kappa[tid] = head[kKey + tid]; be[tid] = head[kBeta + tid] * kappa[tid]; }
 
         // ---- products over the value columns -------------------------------------------------------------------
         float dp[2][4] = {}, xn[2][4] = {}, dqt[NW][4] = {}, zz[NW][4] = {}, dkt[NW][4] = {};
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                     zero8(fk[y]);
                     zero8(fq[y]);
                 }
-                m[0] = max8(fk[y], m[0]);
+                m[0] = max(m[0], rank_less(max8(fk[y], 0u), key_exponent_of(kappa[row])));
                 mq[y] = row_max<KEY / 8>(max8(fq[y], 0u));
             }
             block_max<WARPS>(m, red);
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
 #pragma unroll
             for (int y = 0; y < PIECES; ++y) {
                 const int piece = tid + y * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8, pk = panel_at(row, col), eq = rank_exponent(mq[y]);
-                put8(sm + Smem::kK + pk, ST_LO, fk[y], pow2_float(ek));
+                put8(sm + Smem::kK + pk, ST_LO, fk[y], pow2_float(ek) * pow2_inverse(kappa[row]));
                 put8(sm + Smem::kQ + pk, ST_LO, fq[y], pow2_float(eq));
                 if (col == 0) eqs[row] = eq;
             }
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
 #pragma unroll
             for (int w = 0; w < 8; ++w) dotx += xv[w][tid];
             if (tid < rows)
-                a.dbeta[o + (long long)tid * p.HV] = dotx + ((rowz[tid] + rowz[64 + tid]) + (rowz[128 + tid] + rowz[192 + tid]));
+                a.dbeta[o + (long long)tid * p.HV] = kappa[tid] * dotx + kappa[tid] * kappa[tid] * ((rowz[tid] + rowz[64 + tid]) + (rowz[128 + tid] + rowz[192 + tid]));
         }
         const int i = tid >> 3, seg = tid & 7;           // eight threads a row: sums of F up to and with each column
         {
@@ -568,10 +568,11 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
     const long long step = (long long)p.HK * p.DK;
     for (int e = tid; e < rows * KEY / 4; e += NT) {
         const int row = e / (KEY / 4), col = e % (KEY / 4) * 4;
+        const float of_key = pow2_inverse(kappa[row]);
         if (a.vec_out) {
             struct alignas(4 * sizeof(T)) Raw { T v[4]; } x, y;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) { x.v[w] = from_f32<T>(accq[row * KEY + col + w]); y.v[w] = from_f32<T>(acck[row * KEY + col + w]); }
+            for (int w = 0; w < 4; ++w) { x.v[w] = from_f32<T>(accq[row * KEY + col + w]); y.v[w] = from_f32<T>(acck[row * KEY + col + w] * of_key); }
             if (col < p.DK) {
                 *reinterpret_cast<Raw*>(dq + row * step + col) = x;
                 *reinterpret_cast<Raw*>(dk + row * step + col) = y;
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             for (int w = 0; w < 4; ++w)
                 if (col + w < p.DK) {
                     dq[row * step + col + w] = from_f32<T>(accq[row * KEY + col + w]);
-                    dk[row * step + col + w] = from_f32<T>(acck[row * KEY + col + w]);
+                    dk[row * step + col + w] = from_f32<T>(acck[row * KEY + col + w] * of_key);
                 }
         }
     }

@@ -125,7 +125,7 @@ __device__ __forceinline__ void invert(float* A, float* tmp) {
 template <int KEY>
 struct PrepareSmem {
     static constexpr int kTile = KEY * 256;
-    static constexpr int kBytes = 2 * kTile + DeltaRecord::kSquare + C * PITCH * 4 + 64 * 34 * 4 + 7 * C * 4 + 4 * 4 + 32 * 4;
+    static constexpr int kBytes = 2 * kTile + DeltaRecord::kSquare + C * PITCH * 4 + 64 * 34 * 4 + 8 * C * 4 + 4 * 4 + 32 * 4;
 };
 
 template <typename T, int KEY>
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
     uint8_t *kr = sm, *qr = sm + Smem::kTile;
     uint8_t* tr = qr + Smem::kTile;                                   // T beta e^G
     float* A = reinterpret_cast<float*>(tr + DeltaRecord::kSquare);
-    float *tmp = A + C * PITCH, *ghi = tmp + 64 * 34, *glo = ghi + C, *be = glo + C, *until = be + C, *left = until + C, *since = left + C, *unit = since + C, *bound = unit + C;
+    float *tmp = A + C * PITCH, *ghi = tmp + 64 * 34, *glo = ghi + C, *be = glo + C, *until = be + C, *left = until + C, *since = left + C, *unit = since + C, *kappa = unit + C, *bound = kappa + C;
     uint32_t* red = reinterpret_cast<uint32_t*>(bound + 4);
     constexpr int LO = KEY * 128;                                     // lo panels behind the hi panels
     const aussm_b200_delta_t& p = a.p;
@@ -164,6 +164,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
     {
         float fk[PIECES][8], fq[PIECES][8];
         uint32_t m[1] = {}, mq[PIECES];
+        int ck[PIECES];                    // exponents of kappa
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
             const int piece = tid + x * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8;
@@ -176,17 +177,24 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             }
         }
 #pragma unroll
-        for (int x = 0; x < PIECES; ++x) { m[0] = max8(fk[x], m[0]); mq[x] = row_max<KEY / 8>(max8(fq[x], 0u)); }
+        for (int x = 0; x < PIECES; ++x) {
+            const uint32_t mk = row_max<KEY / 8>(max8(fk[x], 0u));
+            ck[x] = key_exponent(mk);
+            m[0] = max(m[0], rank_less(mk, ck[x]));
+            mq[x] = row_max<KEY / 8>(max8(fq[x], 0u));
+        }
         block_max<8>(m, red);
         ek = rank_exponent(m[0]);
-        const float sk = pow2_float(ek);
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
             const int piece = tid + x * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8, at = panel_at(row, col);
             const int eq = rank_exponent(mq[x]);
-            put8(kr + at, LO, fk[x], sk);
+            put8(kr + at, LO, fk[x], pow2_float(ek - ck[x]));      // (12 or 13 less 126 at least: kappa > 1 leaves K / kappa >= 1)
             put8(qr + at, LO, fq[x], pow2_float(eq));              // 2^13 Q / r
-            if (col == 0) unit[row] = pow2_float(13 - eq);
+            if (col == 0) {
+                unit[row] = pow2_float(13 - eq);
+                kappa[row] = pow2_float(ck[x]);
+            }
         }
     }
     __syncthreads();
@@ -232,8 +240,9 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
         __syncthreads();                       // the last value head's T beta e^G and vectors are read
         if (warp == 0) {
             const int i0 = 2 * lane, i1 = i0 + 1;
-            be[i0] = b0;
-            be[i1] = b1;
+            b0 *= kappa[i0]; b1 *= kappa[i1];
+            be[i0] = b0 * kappa[i0];
+            be[i1] = b1 * kappa[i1];
             double s = g0 + g1;
 #pragma unroll
             for (int m = 1; m < 32; m *= 2) {
@@ -249,7 +258,8 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             const float e0 = expf((float)before), e1 = expf((float)s);
             left[i0] = be[i0] * e0; left[i1] = be[i1] * e1;                 // what T's columns are multiplied with for W
             since[i0] = p.scale * e0; since[i1] = p.scale * e1;
-            head[kBeta + i0] = be[i0]; head[kBeta + i1] = be[i1];
+            head[kBeta + i0] = b0; head[kBeta + i1] = b1;
+            head[kKey + i0] = kappa[i0]; head[kKey + i1] = kappa[i1];
             head[kGHi + i0] = h0; head[kGHi + i1] = h1;
             head[kGLo + i0] = glo[i0]; head[kGLo + i1] = glo[i1];
             head[kRow + i0] = unit[i0]; head[kRow + i1] = unit[i1];

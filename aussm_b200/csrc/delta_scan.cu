@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     __shared__ uint64_t row_s[4], row_n[4];
     __shared__ uint32_t holder;
     __shared__ float un_s[2][128], un_v[2][128], un_n[128], max_s[PARTS][128], max_n[PARTS][128];
-    // Factors of the steps: V comes in times beta and O goes out times r, dO comes in times r and dV goes out times beta.  Those
+    // Factors of the steps: V comes in times beta kappa and O goes out times r, dO times r and dV times beta kappa.  Those
     // of the way out are copied with the ones of the way in, and chunk i + 4 is asked for when v_done (a_done) of i + 2 is
     // seen, which the issuing warp commits after x_free of i: four of them.
     __shared__ __align__(16) float factors[C], out_factors[4][C];

@@ -134,6 +134,52 @@ def test_an_outlying_gradient_stays_with_its_step(bad):
         assert float((g[n][:, 64:] - g64[n][:, 64:]).abs().max()) <= BWD * float(g64[n].abs().max()), n
 
 
+@pytest.mark.parametrize("l,hk,hv,dk,dv", [(150, 1, 2, 64, 64), (1100, 1, 1, 128, 128), (40, 1, 1, 16, 130)])
+@pytest.mark.parametrize("size", [1e4, 1e9, 1e18])
+def test_padded_keys_of_any_size(size, l, hk, hv, dk, dv):
+    """g = beta = 0 leaves the state alone whatever k and v hold, and the gradients of the other steps with it."""
+    d = make(65, 2, l, hk, hv, dk, dv)
+    pad = slice(20, 33)
+    for n in ("g", "beta"):
+        d[n][0, pad] = 0
+    d["k"][0, pad] *= size
+    d["v"][0, pad] *= size
+    go = go_like(d)
+    (o, s, g), (o64, s64, g64) = run(d, go), truth(d, go)
+    by_rows("o", o, o64, wide(d, d["q"].double().norm(dim=-1)), FWD)
+    assert float((s - s64).abs().max()) <= FWD * float(s64.abs().max())
+    real = torch.ones(2, l, dtype=torch.bool, device="cuda")
+    real[0, pad] = False
+    for n in NAMES:
+        a, b = g[n].double(), g64[n]
+        if n != "state":
+            assert (a[~real] == 0).all() or n in ("q", "g", "beta"), n
+            a, b = a[real], b[real]
+        assert float((a - b).abs().max()) <= BWD * float(b.abs().max()), n
+    # of a padded step itself: beta's gradient is a product of its key and value, as large as they are
+    a, b = g["beta"][~real].double(), g64["beta"][~real]
+    assert float((a - b).abs().max()) <= BWD * float(b.abs().max())
+
+
+@pytest.mark.parametrize("l,hk,hv,dk,dv", [(150, 1, 2, 64, 64), (1100, 1, 1, 128, 128)])
+def test_keys_of_all_sizes(l, hk, hv, dk, dv):
+    """With keys times s, values times s and step sizes over s^2 the rule is the same: dk and dv shrink by s, dbeta grows by s^2.
+    Powers of two are exact, so the results are held to the recurrence of the unit keys; what is left of a row behind the
+    division is 1..2 at its largest element, 1 to 4 times a unit key here: four times the usual bounds for the neighbours."""
+    d = make(69, 1, l, hk, hv, dk, dv)
+    gen = torch.Generator().manual_seed(3)
+    s = 2.0 ** torch.randint(3, 30, (1, l, hk, 1), generator=gen).cuda()
+    s[:, ::3] = 1.0
+    big = dict(d, k=d["k"] * s, v=d["v"] * wide(d, s), beta=d["beta"] / wide(d, s)[..., 0] ** 2)
+    go = go_like(d)
+    (o, last, g), (o64, s64, g64) = run(big, go), truth(d, go)
+    g = dict(g, k=g["k"] * s, v=g["v"] * wide(d, s), beta=g["beta"] / wide(d, s)[..., 0] ** 2)
+    by_rows("o", o, o64, wide(d, d["q"].double().norm(dim=-1)), 4 * FWD)
+    assert float((last - s64).abs().max()) <= 4 * FWD * float(s64.abs().max())
+    for n in NAMES:
+        assert float((g[n] - g64[n]).abs().max()) <= 4 * BWD * float(g64[n].abs().max()), n
+
+
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
 @pytest.mark.parametrize("name", ["v", "k", "beta", "g"])
 def test_what_is_not_finite_is_never_hidden(name, bad):
