@@ -57,7 +57,8 @@ struct DeltaRecord {
 // header, in floats: what a stored part is to be multiplied with (1 / S) ...
 enum : int { kUnW = 0, kUnKt = 1, kUnQ = 2, kUnT = 3, kUnP = 4, kGamma = 5 /* e^(G_C) */,
              kBeta = 16 /* beta kappa, 64 */, kGHi = 80, kGLo = 144 /* G_i = hi + lo, 64 each */, kRow = 208 /* r, 64 */,
-             kKey = 272 /* kappa, 64 */ };
+             kKey = 272 /* kappa, 64 */,
+             kIdle = 6 /* 2 words: bit i of the first is set when beta of step 2 i is zero, of the second 2 i + 1 */ };
 
 // byte offset of element (row, col) in the hi panels of a tile
 __host__ __device__ __forceinline__ int panel_at(int row, int col) {
@@ -100,6 +101,10 @@ struct DeltaInputs {
     const void *q, *k, *v;
     const float *g, *beta;
 };
+
+// Keys and values of a step with beta = 0 (padding: unwritten memory may lie there) count as zero where they are not finite:
+// they are multiplied with zeros only, which would make NaN of them.
+__device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) <= 3.402823466e38f ? x : 0.f; }
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }

@@ -165,12 +165,21 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                 for (int y = 0; y < KEY / 64; ++y) raw_d[y][0] = raw_d[y][1] = make_uint4(0, 0, 0, 0);
             }
             if (dv < rows) {                             // X.V of step dv over the columns of group grp
-                float w[8], sum = 0.f;
+                float w[8];
                 load8(v + dv * p.v_stride[1] + v0, 8 * grp, cols, a.vec_v, w);
+                auto dot = [&]() {
+                    float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint8_t* x = sm + Smem::kX + panel_at(8 * grp + i, dv);
-                    sum = fmaf(__half2float(*reinterpret_cast<const __half*>(x)) + __half2float(*reinterpret_cast<const __half*>(x + SQ_LO)), w[i], sum);
+                    for (int i = 0; i < 8; ++i) {
+                        const uint8_t* x = sm + Smem::kX + panel_at(8 * grp + i, dv);
+                        sum = fmaf(__half2float(*reinterpret_cast<const __half*>(x)) + __half2float(*reinterpret_cast<const __half*>(x + SQ_LO)), w[i], sum);
+                    }
+                    return sum;
+                };
+                float sum = dot();
+                if (be[dv] == 0.f && rank_of(sum) < 0x01000000u) {
+                    keep_finite8(w);
+                    sum = dot();
                 }
                 dotv = fmaf(sum, pow2_float(-e[1]), dotv);
             }
@@ -283,6 +292,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
                 const int piece = tid + y * NT, row = piece / (KEY / 8), col = piece % (KEY / 8) * 8;
                 if (row < rows) {
                     load8(k + row * p.k_stride[1], col, p.DK, a.vec_k, fk[y]);
+                    if (!finite8(fk[y]) && all_idle(a.in.beta + ((long long)b * p.L + t0 + row) * p.HV + hk * r, r)) keep_finite8(fk[y]);
                     load8(q + row * p.q_stride[1], col, p.DK, a.vec_q, fq[y]);
                 } else {
                     zero8(fk[y]);

@@ -176,6 +176,12 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 zero8(fq[x]);
             }
         }
+        // (asking for beta of every row beforehand takes 2 % longer)
+#pragma unroll
+        for (int x = 0; x < PIECES; ++x) {
+            const int row = (tid + x * NT) / (KEY / 8);
+            if (!finite8(fk[x]) && row < rows && all_idle(a.in.beta + ((long long)b * p.L + t0 + row) * p.HV + hk * r, r)) keep_finite8(fk[x]);
+        }
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
             const uint32_t mk = row_max<KEY / 8>(max8(fk[x], 0u));
@@ -259,13 +265,17 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
             left[i0] = be[i0] * e0; left[i1] = be[i1] * e1;                 // what T's columns are multiplied with for W
             since[i0] = p.scale * e0; since[i1] = p.scale * e1;
             head[kBeta + i0] = b0; head[kBeta + i1] = b1;
-            head[kKey + i0] = kappa[i0]; head[kKey + i1] = kappa[i1];
             head[kGHi + i0] = h0; head[kGHi + i1] = h1;
             head[kGLo + i0] = glo[i0]; head[kGLo + i1] = glo[i1];
             head[kRow + i0] = unit[i0]; head[kRow + i1] = unit[i1];
+            head[kKey + i0] = kappa[i0]; head[kKey + i1] = kappa[i1];
             if (lane == 31) head[kGamma] = e1;
-            auto finite = [](float x) { return x <= 3.402823466e38f ? x : 0.f; };
-            float um = fmaxf(finite(u0), finite(u1)), em = fabsf(p.scale) * fmaxf(finite(e0), finite(e1));
+            const uint32_t even = __ballot_sync(0xffffffffu, i0 < rows && b0 == 0.f), odd = __ballot_sync(0xffffffffu, i1 < rows && b1 == 0.f);
+            if (lane == 0) {
+                head[kIdle] = __uint_as_float(even);
+                head[kIdle + 1] = __uint_as_float(odd);
+            }
+            float um = fmaxf(finite_or_zero(u0), finite_or_zero(u1)), em = fabsf(p.scale) * fmaxf(finite_or_zero(e0), finite_or_zero(e1));
 #pragma unroll
             for (int m = 16; m; m >>= 1) {
                 um = fmaxf(um, __shfl_xor_sync(0xffffffffu, um, m));

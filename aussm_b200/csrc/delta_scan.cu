@@ -208,6 +208,7 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
     // of the way out are copied with the ones of the way in, and chunk i + 4 is asked for when v_done (a_done) of i + 2 is
     // seen, which the issuing warp commits after x_free of i: four of them.
     __shared__ __align__(16) float factors[C], out_factors[4][C];
+    __shared__ __align__(16) uint32_t idle[4];                        // [2], [3]: steps without a step size, from the header
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const aussm_b200_delta_t& p = a.p;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -361,6 +362,8 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
                 const bool out = me >= C / 4;
                 cp_async16((out ? out_factors[i & 3] : factors) + x, reinterpret_cast<const float*>(record(i)) + (out != BWD ? kRow : kBeta) + x);
             }
+            static_assert(kIdle == 6, "the second half of 16 bytes of the header");
+            if (!BWD && me == C / 2) cp_async16(idle, reinterpret_cast<const float*>(record(i)) + 4);
             if (a.vec_v) {
                 constexpr int E = 16 / (int)sizeof(T), PIECES = 128 / E, ROWS = 128 / PIECES;      // rows an instruction
                 int row = me / PIECES;
@@ -388,6 +391,10 @@ __global__ void __launch_bounds__(THREADS, 1) delta_scan_kernel(const ScanParams
             cp_async_wait<0>();
             arrive(&v_loaded);
             if (!warp_wait(&v_loaded, i & 1, a.status)) break;
+            if (!BWD)                             // values that count as zero: each lane clears its column
+#pragma unroll 1
+                for (int z = 0; z < 2; ++z)
+                    for (uint32_t m = idle[2 + z]; m; m &= m - 1) tile[(2 * (__ffs(m) - 1) + z) * 128 + me] = from_f32<T>(0.f);
             // two steps of this lane's column, times their factors
             auto pair = [&](int t) {
                 return __fmul2_rn(make_float2(to_f32(tile[t * 128 + me]), to_f32(tile[(t + 1) * 128 + me])),

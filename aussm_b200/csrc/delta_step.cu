@@ -58,17 +58,18 @@ __global__ void __launch_bounds__(NT) delta_step_kernel(const StepParams a) {
     const T* v = static_cast<const T*>(a.in.v) + b * p.v_stride[0] + h * p.v_stride[2];
     for (int t = 0; t < p.L; ++t) {
         const int buf = t & 1;
+        const long long gh = ((long long)b * p.L + t) * p.HV + h;
+        const float decay = expf(a.in.g[gh]), beta = a.in.beta[gh];
+        auto taken = [&](float x) { return beta == 0.f ? finite_or_zero(x) : x; };         // a key or value
         if (threadIdx.x < AUSSM_MAX_DELTA_KEY)
-            ks[buf][threadIdx.x] = threadIdx.x < p.DK ? to_f32(k[t * p.k_stride[1] + threadIdx.x]) : 0.f;
+            ks[buf][threadIdx.x] = threadIdx.x < p.DK ? taken(to_f32(k[t * p.k_stride[1] + threadIdx.x])) : 0.f;
         else if (threadIdx.x < 2 * AUSSM_MAX_DELTA_KEY) {
             const int x = threadIdx.x - AUSSM_MAX_DELTA_KEY;
             qs[buf][x] = x < p.DK ? to_f32(q[t * p.q_stride[1] + x]) : 0.f;
         }
-        const long long gh = ((long long)b * p.L + t) * p.HV + h;
-        const float decay = expf(a.in.g[gh]), beta = a.in.beta[gh];
         float val[VEC];
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) val[c] = mine ? to_f32(v[t * p.v_stride[1] + col + c]) : 0.f;
+        for (int c = 0; c < VEC; ++c) val[c] = mine ? taken(to_f32(v[t * p.v_stride[1] + col + c])) : 0.f;
         __syncthreads();
         float pk[VEC] = {}, pq[VEC] = {}, kq = 0.f;
 #pragma unroll

@@ -44,6 +44,23 @@ __device__ __forceinline__ int frag_bt(int krow, int ncol) {
     return panel_at(krow + (lane & 15), ncol + (lane >> 4) * 8);
 }
 
+// whether beta of a step is zero for all `heads` value heads that share a key head
+__device__ __forceinline__ bool all_idle(const float* beta, int heads) {
+    bool idle = true;
+    for (int h = 0; h < heads; ++h) idle = idle && beta[h] == 0.f;
+    return idle;
+}
+__device__ __forceinline__ bool finite8(const float (&f)[8]) {
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) all = all && rank_of(f[i]) >= 0x01000000u;
+    return all;
+}
+__device__ __forceinline__ void keep_finite8(float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = finite_or_zero(f[i]);
+}
+
 // eight consecutive elements of a row, zeros from `cols` on
 template <typename T>
 __device__ __forceinline__ void load8(const T* row, int c, int cols, bool vec, float (&f)[8]) {

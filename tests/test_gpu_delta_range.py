@@ -181,6 +181,53 @@ def test_keys_of_all_sizes(l, hk, hv, dk, dv):
 
 
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_padded_steps_of_anything(bad, dtype):
+    """Unwritten memory in the keys and values of padded steps, in sequences and in single steps."""
+    d = make(66, 2, 150, 1, 2, 64, 64, dtype)
+    clean = {n: t.clone() for n, t in d.items()}
+    pad = torch.zeros(2, 150, dtype=torch.bool, device="cuda")
+    pad[0, 100:], pad[1, :7], pad[1, 70] = True, True, True
+    for x in (d, clean):
+        x["g"][pad] = 0
+        x["beta"][pad] = 0
+    d["k"][pad], d["v"][pad] = bad, bad
+    clean["k"][pad], clean["v"][pad] = 0, 0
+    go = go_like(d)
+    go[pad] = 0
+    (o, s, g), (o64, s64, g64) = run(d, go), truth(clean, go)
+    by_rows("o", o, o64, wide(d, d["q"].double().norm(dim=-1)), FWD)
+    assert float((s - s64).abs().max()) <= FWD * float(s64.abs().max())
+    for n in NAMES[:5]:
+        a, b = g[n][~pad].double(), g64[n][~pad]
+        assert ((a - b).abs() <= BWD * float(b.abs().max()) + torch.finfo(g[n].dtype).eps / 2 * b.abs()).all(), n
+    assert float((g["state"] - g64["state"]).abs().max()) <= BWD * float(g64["state"].abs().max())
+    assert (g["k"][pad] == 0).all() and (g["v"][pad] == 0).all()
+    state = clean["state"].clone()
+    for t in range(100, 104):
+        y = gated_delta_step(*(d[n][:1, t:t + 1] for n in NAMES[:5]), state[:1])
+        assert torch.isfinite(y).all()
+    assert torch.equal(state, clean["state"])
+
+
+@pytest.mark.parametrize("size", [1e6, 1e12])
+def test_a_large_value_shows_in_its_column_and_chunk(size):
+    d = make(67, 1, 200, 1, 1, 64, 64)
+    d["v"][0, 90, 0, 11] *= size
+    put = float(d["beta"][0, 90, 0] * d["v"][0, 90, 0, 11].abs())       # into the state; sqrt(dk) less into an output
+    (o, s, _), (o64, s64, _) = run(d), truth(d)
+    err = (o - o64).abs()[0, :, 0]
+    rest = [c for c in range(64) if c != 11]
+    assert float(err[:, rest].max()) <= FWD * float(o64[..., rest].abs().max())
+    assert float(err[:64, 11].max()) <= FWD * float(o64[:, :64, 0, 11].abs().max())
+    # The state behind the chunk is e^G S + sum_j Kt_j V'_j, whose terms are rounded by 2^-21 of the largest |Kt_j| (at most a
+    # unit key) times the largest |V'_j| (the value put in): a decay that follows the value in its chunk does not shrink that
+    # error.  Here it shrinks the result to 6e-14 of the value, so the bound is on the value, not on what is left of it.
+    assert float(err[64:, 11].max()) <= FWD * put / 8
+    assert float((s - s64).abs()[..., 11].max()) <= FWD * put
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
 @pytest.mark.parametrize("name", ["v", "k", "beta", "g"])
 def test_what_is_not_finite_is_never_hidden(name, bad):
     """From its step on nothing that depends on it is finite; before it, a step of its chunk is right or not finite, and a
