@@ -214,7 +214,11 @@ class GatedDeltaBlock(nn.Module):
         if device not in self._angles:       # float64 whatever type the module is cast to
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("GatedDeltaBlock: call the block once before it is captured into a graph")
-            self._angles[device] = rotary.rotary_frequencies(self.rotary_dim, self.rotary_base, device=device)[0]
+            with torch.inference_mode(False):    # kept for training too, whoever calls first ..
+                kept = rotary.rotary_frequencies(self.rotary_dim, self.rotary_base, device=device)[0]
+            if device.type == "cuda":            # .. and for every stream
+                torch.cuda.current_stream(device).synchronize()
+            self._angles[device] = kept
         return self._angles[device]
 
     def _inputs(self, x, conv, positions):

@@ -156,6 +156,28 @@ def test_block_reads_a_prompt_in_pieces(monkeypatch):
     assert int(cache["position"]) == 60 and called == [60, 37, 17]
 
 
+def test_the_blocks_frequencies_serve_training_after_inference():
+    from aussm_b200 import models
+    block = models.GatedDeltaBlock(32, n_heads=2, rotary_dim=8)
+    with torch.inference_mode():
+        first = block._frequencies(torch.device("cpu"))
+    assert block._frequencies(torch.device("cpu")) is first and not first.is_inference()
+
+    class Keep(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, f):
+            ctx.save_for_backward(x, f)
+            return x * f.sum()
+
+        @staticmethod
+        def backward(ctx, g):
+            return g * ctx.saved_tensors[1].sum(), None
+
+    x = torch.ones(3, dtype=torch.float64, requires_grad=True)
+    Keep.apply(x, first).sum().backward()
+    assert torch.equal(x.grad, first.sum().expand(3))
+
+
 def test_stretch_wants_rising_turns():
     with pytest.raises(RuntimeError, match="rising"):
         rotary_frequencies(8, scaling="ramp", factor=2.0, turns=(4.0, 4.0))
