@@ -33,8 +33,7 @@ int delta_check(const char* who, const aussm_b200_delta_t* p) {
         return AUSSM_EINVAL;
     }
     // grids are built from the number of chunks and heads
-    const long long chunks = (p->L + kDeltaChunk - 1) / kDeltaChunk;
-    if ((long long)p->B * p->HV * chunks > 0x3fffffffLL) {
+    if ((long long)p->B * p->HV > 0x3fffffffLL / delta_chunks(p->L)) {
         set_error("%s: B*HV*L/%d exceeds 2^30", who, kDeltaChunk);
         return AUSSM_EINVAL;
     }

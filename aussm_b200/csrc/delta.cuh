@@ -24,6 +24,7 @@
 namespace aussm {
 
 constexpr int kDeltaChunk = 64;
+inline int delta_chunks(int steps) { return steps / kDeltaChunk + (steps % kDeltaChunk != 0); }      // L + 63 need not fit
 
 // ---- operand tiles -----------------------------------------------------------------------------------------------
 // Products run on FP16 parts: with S the power of two that brings a tile's largest magnitude to 2^13..2^14,

@@ -9,9 +9,8 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 }  // namespace
 
 DeltaPlan delta_plan(const aussm_b200_delta_t& p) {
-    constexpr int C = kDeltaChunk;
     DeltaPlan d;
-    d.n = (p.L + C - 1) / C;
+    d.n = delta_chunks(p.L);
     d.heads = (size_t)p.B * p.HV * d.n;
     d.rec.key = p.DK <= 64 ? 64 : 128;
     d.slices = (p.DV + 127) / 128;

@@ -99,6 +99,8 @@ def _check(q, k, v, g, beta, scale):
         raise RuntimeError("q, k and v must be (batch, length, heads, width)")
     b, l, hk, dk = q.shape
     hv, dv = v.shape[2:]
+    if (b | l | hk | hv) >> 31:
+        raise RuntimeError(f"batch {b}, length {l}, heads {hk} and {hv}: sizes below 2^31 are supported")
     if hk == 0 or hv == 0 or hv % hk:
         raise RuntimeError(f"the {hv} value heads must be a multiple of the {hk} key heads")
     if not (1 <= dk <= MAX_KEY and 1 <= dv <= MAX_VALUE):

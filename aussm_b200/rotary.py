@@ -129,6 +129,8 @@ def qk_norm_rotate(q: Tensor, k: Tensor, frequencies: Optional[Tensor] = None, p
     if norm not in _NORMS:
         raise RuntimeError(f'norm must be "rms", "l2" or None, got {norm!r}')
     b, l, hq, d = q.shape
+    if (b | l | hq | k.shape[2]) >> 31:
+        raise RuntimeError(f"batch {b}, length {l}, heads {hq} and {k.shape[2]}: sizes below 2^31 are supported")
     if not 1 <= d <= MAX_HEAD or hq == 0 or k.shape[2] == 0:
         raise RuntimeError(f"heads of {d} elements: 1 to {MAX_HEAD} are supported, and one head at least")
     dev = q.device

@@ -156,6 +156,16 @@ def test_block_reads_a_prompt_in_pieces(monkeypatch):
     assert int(cache["position"]) == 60 and called == [60, 37, 17]
 
 
+def test_sizes_of_the_longest_sequences():
+    """Lengths near 2^31: a chunk more is a chunk's bytes more."""
+    lib = aussm_b200._lib.load()
+    keep = lambda l: lib.aussm_b200_delta_keep_bytes(aussm_b200._lib.DeltaProblem(16, l, 1, 1, 8, 8, 0))
+    one = (keep(64 * 2 * 10 ** 6) - keep(64 * 10 ** 6)) // 10 ** 6
+    for l in (2 ** 28, 2 ** 31 - 64, 2 ** 31 - 63, 2 ** 31 - 1):
+        assert keep(l) - keep(64 * 10 ** 6) == one * ((l + 63) // 64 - 10 ** 6), l
+    assert lib.aussm_b200_delta_keep_bytes(aussm_b200._lib.DeltaProblem(33, 2 ** 31 - 1, 1, 1, 8, 8, 0)) == 0      # 33 * 2^25 chunks
+
+
 def test_the_blocks_frequencies_serve_training_after_inference():
     from aussm_b200 import models
     block = models.GatedDeltaBlock(32, n_heads=2, rotary_dim=8)
