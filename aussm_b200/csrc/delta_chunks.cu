@@ -24,13 +24,13 @@ DeltaPlan delta_plan(const aussm_b200_delta_t& p) {
     if (blocks * 3 <= 148) {
         segs = 148 / blocks;
         if (segs > d.n / 4) segs = d.n / 4;
-        if (segs < 3) segs = 1;
+        if (segs < 3) segs = 1;        // three segments or more of at least four chunks stay three or more when rounded up
     }
     d.span = (int)((d.n + segs - 1) / segs);
     d.segs = (d.n + d.span - 1) / d.span;
     const size_t bh = (size_t)p.B * p.HV, ends = d.segs > 1 ? up256((d.segs - 1) * bh * p.DK * p.DV * sizeof(float)) : 0;
     d.transitions = d.heads * d.rec.bytes();
-    d.ends = d.transitions + (d.segs > 2 ? d.segs * bh * d.rec.key * d.rec.key * sizeof(float) : 0);
+    d.ends = d.transitions + (d.segs > 1 ? d.segs * bh * d.rec.key * d.rec.key * sizeof(float) : 0);
     d.fwd_bytes = d.news = d.ends + ends;
     d.states = d.news + up256(pieces * DeltaPlan::news_bytes());
     d.keep_bytes = d.states + up256(pieces * DeltaPlan::state_bytes(d.rec.key));

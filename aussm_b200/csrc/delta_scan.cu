@@ -700,11 +700,11 @@ cudaError_t scan(ScanParams a, const DeltaPlan& plan, float* m, float* ends, cud
     const int heads = a.p.B * a.p.HV, segs = plan.segs;
     a.span = plan.span;
     a.segs = segs;
-    if (segs > 1) {
+    if (segs > 1) {                          // three or more
         const size_t m_stride = (size_t)heads * KEY * KEY, end_stride = (size_t)heads * a.p.DK * a.p.DV;
         ScanParams q = a;
         q.out = nullptr; q.rows = nullptr; q.states = nullptr;
-        if (!BWD && segs > 2) {              // what the segments between the first and the last do to a state
+        if (!BWD) {                          // what the segments between the first and the last do to a state
             q.transition = 1; q.first_seg = 1; q.seg_out = m; q.seg_stride = m_stride;
             delta_scan_kernel<T, KEY, BWD><<<dim3(heads, 1, segs - 2), THREADS, smem, st>>>(q);
             count_launch();
@@ -712,13 +712,11 @@ cudaError_t scan(ScanParams a, const DeltaPlan& plan, float* m, float* ends, cud
         q.transition = 0; q.first_seg = 0; q.seg_out = ends; q.seg_stride = end_stride;
         delta_scan_kernel<T, KEY, BWD><<<dim3(heads, plan.slices, segs - 1), THREADS, smem, st>>>(q);
         count_launch();
-        if (segs > 2) {
-            // 8 columns a block are quicker than 16 while each has an SM (4 heads of 128, 36 segments: 102 against 125 us,
-            // 32 heads, 4 segments: 29 against 18 us)
-            e = heads * ((a.p.DV + 7) / 8) <= 148 ? chain<KEY, BWD, 8>(m, ends, heads, a.p.DK, a.p.DV, segs, st)
-                                                  : chain<KEY, BWD, 16>(m, ends, heads, a.p.DK, a.p.DV, segs, st);
-            if (e != cudaSuccess) return e;
-        }
+        // 8 columns a block are quicker than 16 while each has an SM (4 heads of 128, 36 segments: 102 against 125 us,
+        // 32 heads, 4 segments: 29 against 18 us)
+        e = heads * ((a.p.DV + 7) / 8) <= 148 ? chain<KEY, BWD, 8>(m, ends, heads, a.p.DK, a.p.DV, segs, st)
+                                              : chain<KEY, BWD, 16>(m, ends, heads, a.p.DK, a.p.DV, segs, st);
+        if (e != cudaSuccess) return e;
         a.seg_in = ends - end_stride;        // segment z starts from the state behind segment z - 1
         a.seg_stride = end_stride;
     }
