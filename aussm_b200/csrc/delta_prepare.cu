@@ -6,8 +6,8 @@
 // blocks above the diagonal.  Differences of the sums of g are taken from pairs of floats: sums reach thousands, and
 // e^(G_i - G_j) has to be right to 24 bits where G_i - G_j is small.
 //
-// What bounds it: 3900 instructions a warp at 0.41 a cycle and SM quarter, barriers and shared memory between them.  2048
-// chunk heads of 128: 144 us, 268 MB of records written (1.9 TB/s); 8192 that share 4096 key heads: 462 us.
+// What bounds it: 4200 instructions a warp at 0.42 a cycle and SM quarter, barriers and shared memory between them.  2048
+// chunk heads of 128: 151 us, 272 MB of records written (1.8 TB/s); 8192 that share 4096 key heads: 477 us.
 #include "delta_tiles.cuh"
 #include "host_common.cuh"
 
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 zero8(fq[x]);
             }
         }
-        // (asking for beta of every row beforehand takes 2 % longer)
+        // (asking for beta of every row beforehand takes 1 % longer)
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
             const int row = (tid + x * NT) / (KEY / 8);

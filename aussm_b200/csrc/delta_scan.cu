@@ -16,11 +16,13 @@
 // parts of V' and of V.  Every wait is bounded: one that runs out sets the status word and the block ends.
 //
 // The roles walk different code, chunk after chunk, out of one instruction cache: with every loop unrolled the issue of 36
-// MMAs took 4700 cycles instead of 1700.  Only what must be (registers that are indexed) is unrolled, and the state's
+// MMAs took 4700 cycles instead of 2500.  Only what must be (registers that are indexed) is unrolled, and the state's
 // conversions, the longest straight line, are cut into halves that run side by side (quarters take as long).
 //
-// What bounds it: the instructions that turn float32 rows into FP16 parts and back, 5400 an SM quarter and chunk at 0.45 a
-// cycle (the tensor core is busy 27 % of the time, DRAM 30 %).  A chunk takes 4.4 us (8000 cycles; its MMAs alone 4000).
+// What bounds it: a chain of conversions (float32 rows to FP16 parts and back) and products.  A training pass of 8 chunks a
+// block issues 3800 instructions an SM quarter and chunk at 0.37 a cycle, 10400 cycles a chunk with the start and everything
+// kept for the backward pass; the tensor core is busy 29 % of the time (backward 26 %).  Reading 64 chunks a block takes 4.3 us,
+// 7900 cycles, a chunk, of which its MMAs alone would take 4000.
 #include "common.cuh"
 #include "delta.cuh"
 #include "host_common.cuh"

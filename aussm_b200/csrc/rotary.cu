@@ -6,7 +6,7 @@
 //
 // Bound: memory, every element read once and written once.  4 x 4096 steps, 16 heads of 128 in float32: forward 44 us
 // (6.1 TB/s), backward 83 us (4.9 TB/s, three streams and the weights' sums); 2 x 65536 steps, 12 heads of 128 in bfloat16,
-// forward 211 us (3.8 TB/s: half as many bytes for the same instructions).  A group of 8, 16 or 32 lanes holds a head, both
+// forward 211 us (3.8 TB/s: half as many bytes for the same scalar float32 arithmetic, 71 % of the issue slots).  A group of 8, 16 or 32 lanes holds a head, both
 // elements of a pair in the same lane: the norm is a few shuffles, the rotation none.  The lane's angles and weights serve
 // the heads of a token that the group walks: all of them where the tokens fill the GPU, fewer otherwise.  Angles are reduced
 // in 64 bits: position * (frequency / 2 pi), less its nearest integer, so a position of 2^22 is turned as exactly as 1.

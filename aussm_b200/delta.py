@@ -7,8 +7,9 @@ Per batch entry and value head, with ``a_t = exp(g_t)`` and the state ``S`` (dk,
     o_t = scale S_t^T q_t
 
 ``gated_delta_rule`` takes whole sequences (a chunk of 64 steps at a time, forward and backward),
-``gated_delta_step`` one or a few new steps of many sequences.  Both agree with the recurrence to float32 accuracy for
-every input type.  CUDA tensors only; all arithmetic runs in libaussm_b200.so.
+``gated_delta_step`` one or a few new steps of many sequences, in float32.  The products of the rule carry 22 bits of their
+operands (two FP16 parts each) and float32 sums: results differ from the recurrence by about 1e-6, a plain float32 chunk form by
+4e-7, for every input type, before the rounding to 16 bits.  CUDA tensors only; all arithmetic runs in libaussm_b200.so.
 """
 from __future__ import annotations
 
@@ -187,10 +188,21 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     ``q, k`` are ``(b, l, hk, dk)`` and ``v`` ``(b, l, hv, dv)``, of one type (float32, bfloat16 or float16) and any
     strides; ``hv`` is a multiple of ``hk`` and value head ``h`` reads key head ``h // (hv // hk)``.  ``g`` (logarithm of
     the decay; -inf forgets the state) and ``beta`` (step size) are ``(b, l, hv)`` float32.  Keys are meant to have unit
-    length (``rotary.qk_norm_rotate``) and ``beta`` to lie in 0..2: otherwise the recurrence itself diverges.  A padded
-    step is one with ``g = beta = 0``: it leaves the state as it is.  ``scale`` defaults to ``dk ** -0.5``.
-    ``initial_state`` is ``(b, hv, dk, dv)`` float32 (None: zero).  A step and value head of 128 takes 2 KB of workspace
-    (with gradients 3.7 KB until the backward pass): a very long sequence can be read in pieces that hand the state on.
+    length (``rotary.qk_norm_rotate``) and ``beta`` to lie in 0..2 (larger keys: ``beta |k|^2``): otherwise the recurrence
+    itself diverges.  A padded step is one with ``g = beta = 0``: it leaves the state as it is, whatever its key and value hold
+    (what is not finite in them counts as zero; of a key, where ``beta`` is zero for all value heads that share it).
+    ``scale`` defaults to ``dk ** -0.5``.  ``initial_state`` is ``(b, hv, dk, dv)`` float32 (None: zero).
+
+    Outputs and gradients of ``q`` are right to their own query's size, whatever the other steps hold.  Everything else that
+    is summed over the 64 steps of a chunk is rounded to the largest of the terms: an outlying value shows in its value column
+    with about 1e-7 of itself from its step on (as in any float32 sum), but also with about 1e-11 of itself in the steps
+    before it in its chunk, which counts from 1e6 times the others on; so do outlying gradients.  An entry that is not finite
+    makes what depends on it non-finite, and may do so for the steps before it in its chunk (a query: only its own output,
+    and gradients of the chunks up to its own).
+
+    A step and value head of 128 keys and values takes 2.1 KB of workspace; with gradients 3.6 KB are kept until the backward
+    pass, which takes another 1.5 KB (256 values: 5.2 and 3.1 KB).  A very long sequence can be read in pieces that hand the state
+    on.
 
     Returns ``o`` ``(b, l, hv, dv)`` of the inputs' type, or ``(o, final_state)``."""
     _refuse_traced("gated_delta_rule", q, k, v, g, beta, initial_state)

@@ -117,7 +117,8 @@ def qk_norm_rotate(q: Tensor, k: Tensor, frequencies: Optional[Tensor] = None, p
     ``q_weight, k_weight``: ``(d,)`` float32, shared by the heads.  ``frequencies``: up to ``d / 2`` float64 radians per
     position (None: no rotation); their ``n`` pairs are elements ``(i, i + n)`` of the head, or ``(2i, 2i + 1)`` when
     ``interleaved``; the rest of the head is not rotated.  ``positions``: int64 ``(l,)`` or ``(b, l)`` (None: 0, 1, ...),
-    reduced in 64 bits, so far ones are as exact as near ones.  ``magnitude`` multiplies the rotated part.  Types and
+    reduced in 64 bits, so far ones are as exact as near ones (up to 2^28; behind it a bit is lost with every doubling).  The
+    squares of a head add up in float32: elements below 1e19.  ``magnitude`` multiplies the rotated part.  Types and
     strides as in ``gated_delta_rule``; results are contiguous."""
     _refuse_traced("qk_norm_rotate", q, k, frequencies, positions, q_weight, k_weight)
     if not isinstance(q, Tensor) or not q.is_cuda:

@@ -374,9 +374,13 @@ int aussm_b200_rms_norm_bwd(const float* g, const float* extra, /* may be NULL *
  * and the other strides (batch, step, head; elements) are in the problem.  o and
  * the gradients of q, k, v are contiguous, of the same type.  g, beta, dg, dbeta:
  * (B, L, HV) float32 contiguous; states: (B, HV, DK, DV) float32 contiguous.  1 <=
- * DK <= AUSSM_MAX_DELTA_KEY, 1 <= DV <= AUSSM_MAX_DELTA_VALUE.  All arithmetic has
- * float32 accuracy whatever `dtype` is; outputs are rounded once.
- * exp(g) below about 1e-38 counts as zero (g = -inf forgets the state).
+ * DK <= AUSSM_MAX_DELTA_KEY, 1 <= DV <= AUSSM_MAX_DELTA_VALUE.  Products carry 22 bits
+ * of their operands (two FP16 parts) and float32 sums whatever `dtype` is, the single
+ * steps float32; outputs are rounded once.  o and dq are right to the size of their own
+ * query; other sums over the 64 steps of a chunk are rounded to the largest term.
+ * exp(g) below about 1e-38 counts as zero (g = -inf forgets the state).  Keys and values
+ * of a step with beta = 0 count as zero where they are not finite (keys: where beta is
+ * zero for all value heads that share them).
  * `keep` is what the backward call reads of its forward call (aussm_b200_delta_
  * keep_bytes bytes; NULL when there will be none); the backward call leaves it as it
  * is.  Deterministic: no atomics.  keep and workspace are 256-byte aligned. */

@@ -227,6 +227,19 @@ def test_a_large_value_shows_in_its_column_and_chunk(size):
     assert float((s - s64).abs()[..., 11].max()) <= FWD * put
 
 
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e9, 1e12])
+def test_a_large_value_before_its_step(size):
+    """Steps before it in its chunk share its scale: their parts are off by 2^-38 of the value at most, each of up to 64 of them
+    that a result adds up."""
+    d = make(70, 1, 130, 1, 1, 64, 64)
+    d["v"][0, 120, 0, 11] *= size
+    put = float(d["beta"][0, 120, 0] * d["v"][0, 120, 0, 11].abs())
+    o, _, _ = run(d)
+    o64, _, _ = truth(d)
+    before = o64[0, 64:120, 0, 11]
+    assert float((o[0, 64:120, 0, 11] - before).abs().max()) <= 64 * 2 ** -38 * put + FWD * float(before.abs().max())
+
+
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
 @pytest.mark.parametrize("name", ["v", "k", "beta", "g"])
 def test_what_is_not_finite_is_never_hidden(name, bad):
