@@ -7,7 +7,7 @@
 // e^(G_i - G_j) has to be right to 24 bits where G_i - G_j is small.
 //
 // What bounds it: 4200 instructions a warp at 0.42 a cycle and SM quarter, barriers and shared memory between them.  2048
-// chunk heads of 128: 151 us, 272 MB of records written (1.8 TB/s); 8192 that share 4096 key heads: 477 us.
+// chunk heads of 128: 147 us, 272 MB of records written (1.9 TB/s); 8192 that share 4096 key heads: 471 us.
 #include "delta_tiles.cuh"
 #include "host_common.cuh"
 
@@ -176,12 +176,6 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 zero8(fq[x]);
             }
         }
-        // (asking for beta of every row beforehand takes 1 % longer)
-#pragma unroll
-        for (int x = 0; x < PIECES; ++x) {
-            const int row = (tid + x * NT) / (KEY / 8);
-            if (!finite8(fk[x]) && row < rows && all_idle(a.in.beta + ((long long)b * p.L + t0 + row) * p.HV + hk * r, r)) keep_finite8(fk[x]);
-        }
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
             const uint32_t mk = row_max<KEY / 8>(max8(fk[x], 0u));
@@ -208,8 +202,10 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
     // K K^T and Q K^T on and below the diagonal blocks: warp = rows rb*16.., columns half*32..
     const int rb = warp & 3, half = warp >> 2;
     const uint32_t ks = smem_addr(kr), qs = smem_addr(qr), ts = smem_addr(tr);
-    float kk[4][4] = {}, qk[4][4] = {};
-    {
+    float kk[4][4], qk[4][4];
+    for (bool again = false;; again = true) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) kk[x >> 2][x & 3] = qk[x >> 2][x & 3] = 0.f;
 #pragma unroll
         for (int k0 = 0; k0 < KEY; k0 += 16) {
             uint32_t kh[4], kl[4], qh[4], ql[4];
@@ -237,6 +233,20 @@ __global__ void __launch_bounds__(NT, 2) delta_prepare_kernel(const PrepareParam
                 }
             }
         }
+        // |k_i|^2 tells of a key that is not finite: once more without it, if it is one that counts as zero.  (Looking at the
+        // elements before they are stored takes 3 % longer.)
+        bool bad = false;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) bad = bad || rank_of(kk[x >> 2][x & 3]) < 0x01000000u;
+        if (again || !__syncthreads_or(bad)) break;
+        for (int piece = tid; piece < C * KEY / 8; piece += NT) {
+            const int row = piece / (KEY / 8);
+            if (row >= rows || !all_idle(a.in.beta + ((long long)b * p.L + t0 + row) * p.HV + hk * r, r)) continue;
+            __half* at = reinterpret_cast<__half*>(kr + panel_at(row, piece % (KEY / 8) * 8));
+            for (int i = 0; i < 8; ++i)
+                if (__hisinf(at[i]) || __hisnan(at[i])) at[i] = at[LO / 2 + i] = __float2half(0.f);
+        }
+        __syncthreads();
     }
     const float unk = pow2_float(-ek), unq = pow2_float(-13);
 
