@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
             const size_t piece = at * a.slices + (v0 >> 7);
             const bool there = dv < cols;
             float shrink[5];
-            auto unit = [&](int y, uint32_t m) {            // exponent of operand y, and what its sums so far shrink by
+            auto unit = [&](int y, uint32_t m) {         // exponent of operand y, and what its sums so far shrink by
                 const int now = min(e[y], rank_exponent(m));
                 shrink[y] = v0 ? pow2_float(max(-126, now - e[y])) : 0.f;
                 e[y] = now;
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         }
         // E1 = scale D dO V'^T (gradient of Q K^T), E = -beta D X V'^T (gradient of K K^T), F = their part in G_i - G_j
         uint32_t m[1] = {}, mrow[2] = {};
-        float bsum[2] = {};                   // dbeta of rows g and g + 8: sum of -D X V'^T K K^T
+        float bsum[2] = {};                              // dbeta of rows g and g + 8: sum of -D X V'^T K K^T
         {
             const uint8_t* pt = reinterpret_cast<const uint8_t*>(head) + a.rec.p();
             const float unp = head[kUnP], fx = pow2_float(-e[1]) * pow2_float(-e[2]);
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
         }
         block_max<WARPS>(m, red + 2 * WARPS);
         // E1's rows have exponents e1 of their own in E1 K, where they meet no other; in E1^T Q the rows of Q make up for them,
-        // as q 2^(-e1 - top) with the largest of these in the usual range.  Rows 2^24 below that one add nothing.
+        // as q 2^(-e1 - top) with the largest of these in the usual range (in two steps where 2^down is no FP16 number).
         const int e2 = rank_exponent(m[0]);
         auto e1_of = [&](int i) { return rank_exponent(max(max(e1max[0][i], e1max[1][i]), max(e1max[2][i], e1max[3][i]))); };
         const int e1[2] = {e1_of(rb * 16 + g), e1_of(rb * 16 + g + 8)};
@@ -426,14 +426,14 @@ __global__ void __launch_bounds__(NT, 1) delta_grads_kernel(const GradParams a) 
 #pragma unroll
         for (int y = 0; y < C * KEY / 8 / NT; ++y) {
             const int piece = tid + y * NT, row = piece / (KEY / 8), down = -e1_of(row) - eqs[row] - top;
-            const __half2 f = __float2half2_rn(down < -24 ? 0.f : pow2_float(down));
+            const __half2 f = __float2half2_rn(pow2_float(max(-24, down))), f2 = __float2half2_rn(pow2_float(max(-24, down + 24)));
 #pragma unroll
             for (int lo = 0; lo <= ST_LO; lo += ST_LO) {
                 uint4* at_q = reinterpret_cast<uint4*>(sm + Smem::kQ + lo + panel_at(row, piece % (KEY / 8) * 8));
                 uint4 x = *at_q;
                 __half2* h2 = reinterpret_cast<__half2*>(&x);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) h2[i] = __hmul2(h2[i], f);
+                for (int i = 0; i < 4; ++i) h2[i] = down < -24 ? __hmul2(__hmul2(h2[i], f), f2) : __hmul2(h2[i], f);
                 *at_q = x;
             }
         }

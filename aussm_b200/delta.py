@@ -194,7 +194,7 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     ``scale`` defaults to ``dk ** -0.5``.  ``initial_state`` is ``(b, hv, dk, dv)`` float32 (None: zero).
 
     Outputs and gradients of ``q`` are right to their own query's size, whatever the other steps hold.  Everything else that
-    is summed over the 64 steps of a chunk is rounded to the largest of the terms: an outlying value shows in its value column
+    is summed over the steps of a chunk (64) is rounded to the largest term in the chunk: an outlying value shows in its value column
     with about 1e-7 of itself from its step on (as in any float32 sum), but also with about 1e-11 of itself in the steps
     before it in its chunk, which counts from 1e6 times the others on; so do outlying gradients.  An entry that is not finite
     makes what depends on it non-finite, and may do so for the steps before it in its chunk (a query: only its own output,

@@ -377,7 +377,7 @@ int aussm_b200_rms_norm_bwd(const float* g, const float* extra, /* may be NULL *
  * DK <= AUSSM_MAX_DELTA_KEY, 1 <= DV <= AUSSM_MAX_DELTA_VALUE.  Products carry 22 bits
  * of their operands (two FP16 parts) and float32 sums whatever `dtype` is, the single
  * steps float32; outputs are rounded once.  o and dq are right to the size of their own
- * query; other sums over the 64 steps of a chunk are rounded to the largest term.
+ * query; other sums over the steps of a chunk (64) are rounded to its largest term.
  * exp(g) below about 1e-38 counts as zero (g = -inf forgets the state).  Keys and values
  * of a step with beta = 0 count as zero where they are not finite (keys: where beta is
  * zero for all value heads that share them).
