@@ -7,7 +7,7 @@
 // steps in 16 bytes, so V', X and the states lie transposed and are read with transposing fragment loads), their FP16 parts
 // go to shared memory under one power of two per tile, of dO per row (it only shrinks from slice to slice: sums in one unit)
 // and mma.sync runs the three products of parts.  Then K K^T, and dO V'^T and X V'^T, masked and decayed, meet Q and K.
-// What bounds it: 6800 instructions a warp (conversions, fragments, 490 of them MMAs) at 0.33 a cycle and SM quarter, loads
+// What bounds it: 6800 instructions a warp (conversions, fragments, 490 of them MMAs) at 0.34 a cycle and SM quarter, loads
 // and work taking turns: 46 us a block of 64 x 128 x 128, of which 9 are its 384 KB at the DRAM's pace.  Spills gone, operands
 // by asynchronous copies or the next block's brought to the L2: 633, 699, 673 us against 638 (2048 chunk heads of 128).
 // The gradient of g_t is summed over just the pairs and states it stands for (see the end): sums over all pairs of which

@@ -20,8 +20,8 @@
 // conversions, the longest straight line, are cut into halves that run side by side (quarters take as long).
 //
 // What bounds it: a chain of conversions (float32 rows to FP16 parts and back) and products.  A training pass of 8 chunks a
-// block issues 3800 instructions an SM quarter and chunk at 0.37 a cycle, 10400 cycles a chunk with the start and everything
-// kept for the backward pass; the tensor core is busy 29 % of the time (backward 26 %).  Reading 64 chunks a block takes 4.3 us,
+// block issues 3800 instructions an SM quarter and chunk at 0.38 a cycle, 10100 cycles a chunk with the start and everything
+// kept for the backward pass; the tensor core is busy 30 % of the time (backward 26 %).  Reading 64 chunks a block takes 4.3 us,
 // 7900 cycles, a chunk, of which its MMAs alone would take 4000.
 #include "common.cuh"
 #include "delta.cuh"
